@@ -125,7 +125,8 @@ TE_API te_status te_attn_engine_set_wait_limit(te_attn_engine *engine, uint32_t 
  * but "0"), the reference's switch (c/src/qwen.c:47-73, 2216-2304); then the
  * engine prints its totals to stderr when freed.  The report is one line,
  * "tinyengine_profile: device_ms=T decode=ms/calls append=... merge=...
- * prefill_prep=... prefill_attn=... matvec=... exchange=... step=...", the reference's
+ * prefill_prep=... prefill_attn=... matvec=... exchange=... step=...
+ * kv4_decode=... kv4_append=... kv4_read=...", the reference's
  * "name=ms/calls" format.  te_attn_engine_profile_report synchronises the
  * engine's stream and writes that line to buf (TE_STATUS_INVALID_ARGUMENT if
  * it does not fit). */
@@ -417,6 +418,93 @@ TE_API te_status te_qwen_step_create(te_kv_cache *cache, const te_qwen_step_desc
 TE_API te_status te_qwen_step_run(te_qwen_step *step, size_t seq, const int64_t *token, float *hidden,
                                   float *logits, int64_t *next_token, uint32_t flags);
 TE_API void te_qwen_step_free(te_qwen_step *step);
+
+/* 4-bit KV cache ------------------------------------------------------------
+ *
+ * The paged cache held as GGUF Q4_0 blocks: each key or value row of a kv head
+ * is head_dim / 32 blocks of 32 values, a block a binary16 scale d and 32
+ * codes c in 0..15 that stand for (c - 8) d -- 4.5 bits a value, 3.56 times
+ * less to hold and to read than the f16 cache.  Writing a row quantises it:
+ * d = f16(m / -8), m the block's value of largest magnitude (the lowest index
+ * on ties; d saturates at +-65504), c = clamp(rint(x / d), -8, 7) + 8 with
+ * the correctly rounded fp32 quotient, rint half to even, c = 8 where d = 0;
+ * a block with a NaN or infinity gets d = NaN (it reads back as NaN).  Keys
+ * are rotated (and biased) in fp32 before they are quantised.  No reference
+ * counterpart for the cache (the reference holds fp32 or f16 keys and values);
+ * the block format is its Q4_0 (c/src/ops.c:18-21, :584-599).
+ *
+ * te_kv4_cache is a cache of its own, described by a te_kv_cache_desc
+ * (head_dim 64 or 128, page_tokens a multiple of 64); pages, sequences, RoPE
+ * offsets and biases work as for te_kv_cache, and the functions of the same
+ * name suffix take the same arguments.  The pool may exceed 2^32 bytes.
+ * Device pointers, 16-byte aligned unless stated; work is queued on the
+ * engine's stream and the calls return without synchronising.  Free a cache
+ * before its engine. */
+#define TE_ATTN_OUTPUT_F16    (1u << 11) /* te_kv4_append, te_kv4_cache_read: returned rows are binary16 */
+
+typedef struct te_kv4_cache te_kv4_cache;
+
+TE_API te_status te_kv4_cache_create(te_attn_engine *engine, const te_kv_cache_desc *desc,
+                                     te_kv4_cache **out_cache);
+TE_API void te_kv4_cache_free(te_kv4_cache *cache);
+TE_API te_status te_kv4_cache_seq_reset(te_kv4_cache *cache, size_t seq, size_t position_offset);
+TE_API te_status te_kv4_cache_seq_truncate(te_kv4_cache *cache, size_t seq, size_t length);
+TE_API te_status te_kv4_cache_seq_length(const te_kv4_cache *cache, size_t seq, size_t *out_length);
+TE_API te_status te_kv4_cache_reserve(te_kv4_cache *cache, size_t seq, size_t tokens);
+TE_API te_status te_kv4_cache_set_qkv_bias(te_kv4_cache *cache, size_t layer_begin, size_t n_layers,
+                                           size_t heads, const float *q_bias, const float *k_bias,
+                                           const float *v_bias);
+
+/* Appends n_tokens rows per layer, quantised, at local token indices length ..
+ * length + n_tokens - 1: k and v are [n_layers][n_tokens] rows of
+ * kv_heads * head_dim values (fp32, or binary16 with TE_ATTN_INPUT_F16),
+ * token_stride values apart (0: contiguous; a multiple of 16 bytes, at least
+ * one row), so that the k and v columns of a wider projection output are taken
+ * in place.  With k_stored and v_stored non-NULL the call also returns the
+ * rows as the cache now holds them, [n_layers][n_tokens][kv_heads][head_dim]
+ * fp32 or binary16 (TE_ATTN_OUTPUT_F16), rounded to nearest: a prompt pass can
+ * attend to exactly what later steps will.  Flags: TE_ATTN_ADVANCE,
+ * TE_ATTN_INPUT_F16, TE_ATTN_OUTPUT_F16, TE_ATTN_NO_ROPE, TE_ATTN_QKV_BIAS. */
+TE_API te_status te_kv4_append(te_kv4_cache *cache, size_t layer_begin, size_t n_layers, size_t seq,
+                               const void *k, const void *v, size_t n_tokens, size_t token_stride,
+                               void *k_stored, void *v_stored, uint32_t flags);
+
+/* The values of tokens [token_begin, +n_tokens) of every layer in
+ * [layer_begin, +n_layers): k and v [n_layers][n_tokens][kv_heads][head_dim]
+ * fp32 (exact) or binary16 (TE_ATTN_OUTPUT_F16, rounded to nearest).  With
+ * te_kv_cache_write_f16 this fills an f16 cache from a 4-bit one. */
+TE_API te_status te_kv4_cache_read(te_kv4_cache *cache, size_t layer_begin, size_t n_layers, size_t seq,
+                                   size_t token_begin, size_t n_tokens, void *k, void *v, uint32_t flags);
+
+/* The stored blocks themselves, [n_layers][n_tokens][kv_heads][head_dim / 32]
+ * GGUF Q4_0 blocks of 18 bytes (2-byte aligned device pointers): saves and
+ * restores a sequence without loss.  A write maps pages and grows the
+ * sequence's length to token_begin + n_tokens when that is larger;
+ * token_begin may not be past the current length. */
+TE_API te_status te_kv4_cache_write_q4_0(te_kv4_cache *cache, size_t layer_begin, size_t n_layers, size_t seq,
+                                         size_t token_begin, size_t n_tokens, const void *k_blocks,
+                                         const void *v_blocks);
+TE_API te_status te_kv4_cache_read_q4_0(te_kv4_cache *cache, size_t layer_begin, size_t n_layers, size_t seq,
+                                        size_t token_begin, size_t n_tokens, void *k_blocks, void *v_blocks);
+
+/* te_attention_decode over a 4-bit cache: one query token per sequence over
+ * layers [layer_begin, +n_layers); q, k_new and v_new fp32, or all binary16
+ * with TE_ATTN_INPUT_F16; out fp32.  With k_new / v_new each sequence's new
+ * token is quantised into the cache by the same launch and attended as stored.
+ * Any number of query heads per kv head.  A sequence that holds no token (and
+ * appends none) gives zeros, or a partial record {0, -inf, 0}.  The queries
+ * and the softmax weights enter the tensor cores as two binary16 parts each
+ * (about 22 bits), the codes exactly; scores, softmax statistics and sums are
+ * fp32.  Partial records (TE_ATTN_PARTIAL) have te_attention_decode's layout
+ * and meaning, except that m is a common reference exponent of the row, at
+ * most 5 below its largest score, instead of the largest score itself:
+ * te_attention_merge_partials takes both.  Results are bit-identical across
+ * repeated calls.  Flags: TE_ATTN_ADVANCE, TE_ATTN_PARTIAL, TE_ATTN_NO_ROPE,
+ * TE_ATTN_QKV_BIAS, TE_ATTN_INPUT_F16. */
+TE_API te_status te_kv4_attention_decode(te_kv4_cache *cache, size_t layer_begin, size_t n_layers,
+                                         const uint32_t *seq_ids, size_t n_seqs, const int64_t *q_positions,
+                                         const void *q, const void *k_new, const void *v_new, size_t heads,
+                                         float *out, uint32_t flags);
 
 /*
  * Allocation-free decode for callers that cannot allocate device memory:

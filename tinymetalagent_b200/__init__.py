@@ -11,6 +11,7 @@ from .runtime import (  # noqa: F401
     TE_ATTN_HOST_BUFFERS,
     TE_ATTN_INPUT_F16,
     TE_ATTN_NO_ROPE,
+    TE_ATTN_OUTPUT_F16,
     TE_ATTN_PARTIAL,
     TE_ATTN_QKV_BIAS,
     TE_ATTN_RMSNORM_INPUT,
@@ -18,6 +19,7 @@ from .runtime import (  # noqa: F401
     TE_ATTN_EXACT_Q,
     TE_ATTN_STEP_HEAD,
     AttnEngine,
+    KV4Cache,
     KVCache,
     QwenStep,
     TinyEngineError,

@@ -1,0 +1,1062 @@
+// Kernels of the 4-bit KV cache (layout: te_kv4.h): the quantising append,
+// the read-back, the raw Q4_0 import/export, and the decode attention that
+// consumes the codes on the tensor cores without widening the cache.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "te_internal.h"
+#include "te_kv4.h"
+#include "te_ptx.cuh"
+#include "te_rope.cuh"
+
+namespace te {
+namespace {
+
+// ---- quantising one row -----------------------------------------------------
+
+// Codes and scale of the 32-value block held by 8 consecutive lanes, 4 values
+// each: m = the value of largest magnitude (the lowest index on ties), d =
+// f16(m / -8) saturated to the finite range, c = clamp(rint(x / d), -8, 7) + 8
+// with the correctly rounded quotient.  d is held as the cache holds it, so a
+// value is off by at most |d| / 2 (|d| at the far end of the block's range).
+// A block with a value that is not finite gets d = NaN: it stands for no
+// number, and what reads it shows that.
+__device__ __forceinline__ void q4_quantise(const float (&x)[4], int lane, uint32_t (&c)[4], __half& d) {
+  auto mag = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    if (mag(x[i]) > mag(m)) m = x[i];
+  }
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) {
+    const float o = __shfl_xor_sync(0xffffffffu, m, off);
+    if (mag(o) > mag(m) || (mag(o) == mag(m) && (lane & off))) m = o;
+  }
+  const bool finite = mag(m) < 0x7f800000u;
+  d = finite ? __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.f), 65504.f)) : __ushort_as_half((unsigned short)0x7fff);
+  const float df = __half2float(d);
+  const bool zero = !finite || df == 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float r = fminf(fmaxf(rintf(__fdiv_rn(x[i], df)), -8.f), 7.f);
+    c[i] = zero ? 8u : (uint32_t)((int)r + 8);
+  }
+}
+
+// The value a code stands for (exact in fp32: 4 by 11 bits).
+__device__ __forceinline__ float q4_value(uint32_t c, float d) { return (float)((int)c - 8) * d; }
+
+// Bits of 4 consecutive codes in their K word (dims 8t + 4h .. + 3, h the half
+// of the word's 8 dims) and in their V halfword.
+__device__ __forceinline__ uint32_t k_bits(const uint32_t (&c)[4], int h) {
+  return (c[0] | c[1] << 16 | c[2] << 4 | c[3] << 20) << (8 * h);
+}
+__device__ __forceinline__ uint32_t v_bits(const uint32_t (&c)[4]) {
+  return c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12;
+}
+
+// One token's key and value row, spread over a warp: lane l holds 4 values
+// of each.  head_dim 128: dims 4l .. 4l+3 of the key and of the value;
+// head_dim 64: the key in lanes 0-15, the value in lanes 16-31 (k unused in
+// the upper lanes, v in the lower).
+template <int HD>
+struct RowDims {
+  static constexpr int kLanes = HD / 4;
+  static __device__ __forceinline__ int dim(int lane) { return (lane % kLanes) * 4; }
+  static __device__ __forceinline__ bool has_k(int lane) { return HD == 128 || lane < 16; }
+  static __device__ __forceinline__ bool has_v(int lane) { return HD == 128 || lane >= 16; }
+};
+
+__device__ __forceinline__ void load4(const void* base, size_t idx, int f16, float (&v)[4]) {
+  if (f16) {
+    const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(base) + idx);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  } else {
+    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + idx);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  }
+}
+__device__ __forceinline__ void store4(void* base, size_t idx, int f16, const float (&v)[4]) {
+  if (f16) {
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(base) + idx) =
+        make_uint2(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]));
+  } else {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + idx) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+__device__ __forceinline__ void add_bias4(float (&v)[4], const float* b) {
+  const float4 x = *reinterpret_cast<const float4*>(b);
+  v[0] = __fadd_rn(v[0], x.x); v[1] = __fadd_rn(v[1], x.y); v[2] = __fadd_rn(v[2], x.z); v[3] = __fadd_rn(v[3], x.w);
+}
+
+// Rotates the key row (4 dims a lane) at cos/sin rows c, s with the
+// reference's fp32 expressions; the partner dim is half a row of lanes away.
+template <int HD>
+__device__ __forceinline__ void rope4(float (&k)[4], const float* cr, const float* sr, int lane) {
+  constexpr int half_lanes = HD / 8;
+  const bool upper = (lane & half_lanes) != 0;
+  const int d = RowDims<HD>::dim(lane) % (HD / 2);
+  const float4 c = *reinterpret_cast<const float4*>(cr + d);
+  const float4 s = *reinterpret_cast<const float4*>(sr + d);
+  const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float o = __shfl_xor_sync(0xffffffffu, k[i], half_lanes);
+    k[i] = upper ? rope_hi(o, k[i], cv[i], sv[i]) : rope_lo(k[i], o, cv[i], sv[i]);
+  }
+}
+
+// Quantises the row and writes its codes and scales at token slot `tok` of the
+// tile at `tile` (shared or global memory).  The whole warp calls it.  On
+// return k and v hold the values the codes stand for.
+template <int HD>
+__device__ __forceinline__ void store_row(unsigned char* tile, int tok, int lane, float (&k)[4], float (&v)[4]) {
+  constexpr int CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
+  using R = RowDims<HD>;
+  const int j = tok >> 3, g = tok & 7, tp = (tok & 7) >> 1, e = tok & 1;
+  const int dim = R::dim(lane), b = dim >> 5;
+  auto put_k = [&](const uint32_t(&c)[4], __half d) {
+    uint32_t w = k_bits(c, lane & 1);
+    w |= __shfl_xor_sync(0xffffffffu, w, 1);
+    if (R::has_k(lane)) {
+      if ((lane & 1) == 0) {
+        *reinterpret_cast<uint32_t*>(tile + kv4_word_at(HD, j, 4 * g + ((dim & 31) >> 3), b)) = w;
+      }
+      if ((lane & 7) == 0) {
+        *reinterpret_cast<__half*>(tile + 2 * CB + kv4_scale_at(HD, j, tp, b, e)) = d;
+      }
+    }
+  };
+  auto put_v = [&](const uint32_t(&c)[4], __half d) {
+    if (R::has_v(lane)) {
+      *reinterpret_cast<uint16_t*>(tile + CB + kv4_word_at(HD, j, 4 * ((dim & 31) >> 2) + tp, b) + 2 * e) =
+          (uint16_t)v_bits(c);
+      if ((lane & 7) == 0) {
+        *reinterpret_cast<__half*>(tile + 2 * CB + SB + kv4_scale_at(HD, j, tp, b, e)) = d;
+      }
+    }
+  };
+  uint32_t c[4];
+  __half d;
+  if constexpr (HD == 128) {
+    q4_quantise(k, lane, c, d);
+    put_k(c, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = q4_value(c[i], __half2float(d));
+    q4_quantise(v, lane, c, d);
+    put_v(c, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q4_value(c[i], __half2float(d));
+  } else {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = R::has_k(lane) ? k[i] : v[i];
+    q4_quantise(x, lane, c, d);
+    put_k(c, d);
+    put_v(c, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = v[i] = q4_value(c[i], __half2float(d));
+  }
+}
+
+// A token's raw key and value rows at element offset `at`, with bias and RoPE.
+template <int HD>
+__device__ __forceinline__ void load_row(const void* kp, const void* vp, size_t at, int f16, const float* kb,
+                                         const float* vb, const float* cr, const float* sr, int lane, float (&k)[4],
+                                         float (&v)[4]) {
+  using R = RowDims<HD>;
+  const int dim = R::dim(lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] = v[i] = 0.f;
+  if (R::has_k(lane)) load4(kp, at + dim, f16, k);
+  if (R::has_v(lane)) load4(vp, at + dim, f16, v);
+  if (kb) {
+    if (R::has_k(lane)) add_bias4(k, kb + dim);
+    if (R::has_v(lane)) add_bias4(v, vb + dim);
+  }
+  if (cr) rope4<HD>(k, cr, sr, lane);
+}
+
+// Quotient of a tile index by tiles_per_page: the product with the rounded-up
+// reciprocal is at most one too large (its excess is below t / 2^32 < 1).
+__device__ __forceinline__ int kv4_page_of(const Kv4Pool& p, int tile) {
+  int q = (int)__umulhi((uint32_t)tile, p.tpp_magic);
+  if (q * p.tiles_per_page > tile) --q;
+  return q;
+}
+
+__device__ __forceinline__ unsigned char* tile_ptr(const Kv4Pool& p, const int32_t* page_row, int layer, int kvh,
+                                                   int tile, int tile_bytes) {
+  const int page = kv4_page_of(p, tile);
+  const int in = tile - page * p.tiles_per_page;
+  const long long rec = ((long long)layer * p.num_pages + page_row[page]) * p.kv_heads + kvh;
+  return p.base + (rec * p.tiles_per_page + in) * tile_bytes;
+}
+
+// ---- append -------------------------------------------------------------------
+
+constexpr int kRowWarps = 4;
+
+// One warp per (layer, kv head, tile of 16 tokens): the tile is assembled in
+// shared memory (with the tokens it already holds, if any) and written whole.
+template <int HD>
+__global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
+  constexpr int TB = kv4_tile_bytes(HD);
+  __shared__ __align__(16) unsigned char tiles[kRowWarps][TB];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = p.first / kKv4Tile;
+  const int n_tiles = (p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1;
+  const long long items = (long long)n_tiles * p.pool.kv_heads * p.n_layers;
+  const long long item = (long long)blockIdx.x * kRowWarps + warp;
+  if (item >= items) return;
+  const int kvh = (int)(item % p.pool.kv_heads);
+  const long long r = item / p.pool.kv_heads;
+  const int tile = t0 + (int)(r % n_tiles);
+  const int ll = (int)(r / n_tiles);
+  const int layer = p.layer_begin + ll;
+  unsigned char* dst = tile_ptr(p.pool, p.page_row, layer, kvh, tile, TB);
+  unsigned char* sm = tiles[warp];
+  const int lo = max(p.first - tile * kKv4Tile, 0);
+  const int hi = min(p.first + p.n_tokens - tile * kKv4Tile, kKv4Tile);
+  if (lo > 0 || hi < kKv4Tile) {
+    for (int i = lane * 16; i < TB; i += 512) {
+      *reinterpret_cast<uint4*>(sm + i) = *reinterpret_cast<const uint4*>(dst + i);
+    }
+    __syncwarp();
+  }
+  const size_t brow = ((size_t)layer * p.pool.kv_heads + kvh) * HD;
+  const float* kb = p.k_bias ? p.k_bias + brow : nullptr;
+  const float* vb = p.v_bias ? p.v_bias + brow : nullptr;
+  using R = RowDims<HD>;
+#pragma unroll 4
+  for (int i = lo; i < hi; ++i) {
+    const int tok = tile * kKv4Tile + i - p.first;  // index among the new tokens
+    const long long row = (long long)ll * p.n_tokens + tok;
+    const size_t at = (size_t)(row * p.token_stride) + (size_t)kvh * HD;
+    const float* cr = p.rope ? p.rope_cos + (size_t)(p.first_pos + tok) * (HD / 2) : nullptr;
+    const float* sr = p.rope ? p.rope_sin + (size_t)(p.first_pos + tok) * (HD / 2) : nullptr;
+    float k[4], v[4];
+    load_row<HD>(p.k, p.v, at, p.input_f16, kb, vb, cr, sr, lane, k, v);
+    store_row<HD>(sm, i, lane, k, v);
+    if (p.k_rows) {
+      const size_t o = ((size_t)row * p.pool.kv_heads + kvh) * HD + R::dim(lane);
+      if (R::has_k(lane)) store4(p.k_rows, o, p.rows_f16, k);
+      if (R::has_v(lane)) store4(p.v_rows, o, p.rows_f16, v);
+    }
+  }
+  __syncwarp();
+  for (int i = lane * 16; i < TB; i += 512) {
+    *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(sm + i);
+  }
+}
+
+// ---- read ---------------------------------------------------------------------
+
+// One warp per (layer, kv head, tile): lane 4g + t expands its K words (dims
+// 8t.. of token g) and V words (dims 4g.. of tokens 2t, 2t + 1).
+template <int HD>
+__global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
+  constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int t0 = p.first / kKv4Tile;
+  const int n_tiles = (p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1;
+  const long long items = (long long)n_tiles * p.pool.kv_heads * p.n_layers;
+  const long long item = (long long)blockIdx.x * kRowWarps + warp;
+  if (item >= items) return;
+  const int kvh = (int)(item % p.pool.kv_heads);
+  const long long r = item / p.pool.kv_heads;
+  const int tile = t0 + (int)(r % n_tiles);
+  const int ll = (int)(r / n_tiles);
+  const unsigned char* src = tile_ptr(p.pool, p.page_row, p.layer_begin + ll, kvh, tile, TB);
+  auto row_of = [&](int tok) -> long long {  // element offset of tile token tok's row, or -1 outside the range
+    const int i = tile * kKv4Tile + tok - p.first;
+    return i >= 0 && i < p.n_tokens ? (((long long)ll * p.n_tokens + i) * p.pool.kv_heads + kvh) * HD : -1;
+  };
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const long long kr = row_of(8 * j + g);
+    const long long v0 = row_of(8 * j + 2 * t), v1 = row_of(8 * j + 2 * t + 1);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(src + kv4_word_at(HD, j, lane, b));
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(src + CB + kv4_word_at(HD, j, lane, b));
+      const float kd = __half2float(
+          *reinterpret_cast<const __half*>(src + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1)));
+      const float2 vd = __half22float2(
+          *reinterpret_cast<const __half2*>(src + 2 * CB + SB + kv4_scale_at(HD, j, t, b, 0)));
+      if (kr >= 0) {
+        float x[4], y[4];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          x[2 * q] = q4_value((kw >> (4 * q)) & 15u, kd);
+          x[2 * q + 1] = q4_value((kw >> (4 * q + 16)) & 15u, kd);
+          y[2 * q] = q4_value((kw >> (4 * q + 8)) & 15u, kd);
+          y[2 * q + 1] = q4_value((kw >> (4 * q + 24)) & 15u, kd);
+        }
+        store4(p.k_rows, (size_t)kr + 32 * b + 8 * t, p.rows_f16, x);
+        store4(p.k_rows, (size_t)kr + 32 * b + 8 * t + 4, p.rows_f16, y);
+      }
+      float x[4], y[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        x[q] = q4_value((vw >> (4 * q)) & 15u, vd.x);
+        y[q] = q4_value((vw >> (4 * q + 16)) & 15u, vd.y);
+      }
+      if (v0 >= 0) store4(p.v_rows, (size_t)v0 + 32 * b + 4 * g, p.rows_f16, x);
+      if (v1 >= 0) store4(p.v_rows, (size_t)v1 + 32 * b + 4 * g, p.rows_f16, y);
+    }
+  }
+}
+
+// ---- raw Q4_0 blocks ------------------------------------------------------------
+
+// One thread per (layer, token, kv head, block): both sides.  A raw block is
+// 18 bytes, 2-byte aligned: the scale, then byte i = code i | code (i + 16) << 4.
+template <int HD>
+__global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int to_pool) {
+  constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
+  const long long n = (long long)p.n_layers * p.n_tokens * p.pool.kv_heads * NB;
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int b = (int)(i % NB);
+  long long r = i / NB;
+  const int kvh = (int)(r % p.pool.kv_heads);
+  r /= p.pool.kv_heads;
+  const int tok = p.first + (int)(r % p.n_tokens);
+  const int layer = p.layer_begin + (int)(r / p.n_tokens);
+  unsigned char* tile = tile_ptr(p.pool, p.page_row, layer, kvh, tok / kKv4Tile, TB);
+  const int s = tok % kKv4Tile, j = s >> 3, g = s & 7, tp = g >> 1, e = s & 1;
+  // code index of the block -> its word (byte offset) and nibble shift
+  auto k_word = [&](int t) { return reinterpret_cast<uint32_t*>(tile + kv4_word_at(HD, j, 4 * g + t, b)); };
+  auto v_half = [&](int gg) {
+    return reinterpret_cast<uint16_t*>(tile + CB + kv4_word_at(HD, j, 4 * gg + tp, b) + 2 * e);
+  };
+  uint16_t* kd = reinterpret_cast<uint16_t*>(tile + 2 * CB + kv4_scale_at(HD, j, tp, b, e));
+  uint16_t* vd = reinterpret_cast<uint16_t*>(tile + 2 * CB + SB + kv4_scale_at(HD, j, tp, b, e));
+  if (to_pool) {
+    const uint16_t* kr = reinterpret_cast<const uint16_t*>(p.k) + i * 9;
+    const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.v) + i * 9;
+    uint32_t kc[32], vc[32];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t kx = kr[1 + q], vx = vr[1 + q];
+      kc[2 * q] = kx & 15u; kc[2 * q + 1] = (kx >> 8) & 15u;
+      kc[2 * q + 16] = (kx >> 4) & 15u; kc[2 * q + 17] = kx >> 12;
+      vc[2 * q] = vx & 15u; vc[2 * q + 1] = (vx >> 8) & 15u;
+      vc[2 * q + 16] = (vx >> 4) & 15u; vc[2 * q + 17] = vx >> 12;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t a[4] = {kc[8 * t], kc[8 * t + 1], kc[8 * t + 2], kc[8 * t + 3]};
+      const uint32_t c[4] = {kc[8 * t + 4], kc[8 * t + 5], kc[8 * t + 6], kc[8 * t + 7]};
+      *k_word(t) = k_bits(a, 0) | k_bits(c, 1);
+    }
+#pragma unroll
+    for (int gg = 0; gg < 8; ++gg) {
+      const uint32_t a[4] = {vc[4 * gg], vc[4 * gg + 1], vc[4 * gg + 2], vc[4 * gg + 3]};
+      *v_half(gg) = (uint16_t)v_bits(a);
+    }
+    *kd = kr[0];
+    *vd = vr[0];
+  } else {
+    uint16_t* kr = reinterpret_cast<uint16_t*>(p.k_rows) + i * 9;
+    uint16_t* vr = reinterpret_cast<uint16_t*>(p.v_rows) + i * 9;
+    uint32_t kc[32], vc[32];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t w = *k_word(t);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        kc[8 * t + 2 * q] = (w >> (4 * q)) & 15u;
+        kc[8 * t + 2 * q + 1] = (w >> (4 * q + 16)) & 15u;
+      }
+    }
+#pragma unroll
+    for (int gg = 0; gg < 8; ++gg) {
+      const uint32_t w = *v_half(gg);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vc[4 * gg + q] = (w >> (4 * q)) & 15u;
+    }
+    kr[0] = *kd;
+    vr[0] = *vd;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      kr[1 + q] = (uint16_t)(kc[2 * q] | kc[2 * q + 16] << 4 | kc[2 * q + 1] << 8 | kc[2 * q + 17] << 12);
+      vr[1 + q] = (uint16_t)(vc[2 * q] | vc[2 * q + 16] << 4 | vc[2 * q + 1] << 8 | vc[2 * q + 17] << 12);
+    }
+  }
+}
+
+// ---- decode attention -------------------------------------------------------------
+//
+// out = softmax(q K^T / sqrt(hd)) V per query head, over a group's cached
+// tokens and the token the call appends.  Both products run on mma.sync
+// m16n8k16 with fp32 accumulators, fed with the codes themselves:
+//
+//   S: A = the group's queries as f16 hi (rows 0-7) and lo (rows 8-15) parts,
+//      scaled by a power of two per head; B = K codes minus 8.
+//      Per block of 32 dims S += d (A B) in fp32.
+//   O^T: A = V codes minus 8, rows = dims; B = P d as f16 hi + lo parts (an
+//      error-free product: hi = f16(P d), lo = f16 of the rest), so the
+//      weights keep about 22 bits.
+//
+// The C fragment of S holds, in lane 4g + t, head g and tokens 2t, 2t + 1:
+// exactly what the B fragment of O^T wants, so the weights never leave their
+// registers.  The online softmax keeps a reference exponent per head and
+// moves it (rescaling O) only when a score exceeds it by more than 2^5.
+template <int HD>
+struct Dec {
+  static constexpr int kWarps = 8;
+  static constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
+  static constexpr int NB = HD / 32;
+  static constexpr int kRing = HD == 128 ? 5 : 10;  // tiles in flight per warp
+  static constexpr int kItems = NB * 2 * 32;        // float4 items of a warp's O
+  static constexpr int ring_off = 0;
+  static constexpr int new_off = kWarps * kRing * TB;
+  static constexpr int red_off = new_off + TB;
+  static constexpr int stat_off = red_off + (kWarps / 2) * kItems * 16;
+  static constexpr int bar_off = stat_off + 2 * kWarps * kKv4Heads * 4 + 16;
+  static constexpr int smem = bar_off + kWarps * kRing * 8;
+};
+static_assert(Dec<128>::smem <= 115712 && Dec<64>::smem <= 115712, "two CTAs per SM");
+
+struct Seg {
+  long long next;      // first unit after the segment
+  int ll, kvh, hb, si;
+  int t0, t1;          // tiles of the sequence in this segment
+  int part, parts;     // this segment's part of its group (parts == 1: all of it)
+  long long c0;        // CTA of the group's first part
+  bool last;           // holds the group's last unit (and so the appended token)
+  long long group_id;
+};
+
+// The CTA whose range [b T / G, (b + 1) T / G) holds unit u.
+__device__ __forceinline__ long long kv4_cta_of(long long u, long long total, long long grid) {
+  return div_nonneg((u + 1) * grid - 1, total);
+}
+
+__device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, long long u, long long u1) {
+  Seg s;
+  const long long blk = div_nonneg(u, p.block_units);
+  const int rem = (int)(u - blk * p.block_units);
+  int lo = 0, hi = p.n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.seqs[mid].unit_begin <= rem) lo = mid; else hi = mid - 1;
+  }
+  s.si = lo;
+  const int len = p.seqs[lo].len;
+  const long long gb = blk * p.block_units + p.seqs[lo].unit_begin;
+  const long long ge = gb + kv4_units(len);
+  s.next = ge < u1 ? ge : u1;
+  s.t0 = (int)(u - gb) * kKv4UnitTiles;
+  s.t1 = min((int)(s.next - gb) * kKv4UnitTiles, (len + kKv4Tile - 1) / kKv4Tile);
+  s.last = s.next == ge;
+  const uint32_t lk = (uint32_t)blk / (uint32_t)p.head_blocks;
+  s.hb = (int)((uint32_t)blk - lk * (uint32_t)p.head_blocks);
+  s.ll = (int)(lk / (uint32_t)p.pool.kv_heads);
+  s.kvh = (int)lk - s.ll * p.pool.kv_heads;
+  s.c0 = kv4_cta_of(gb, p.total_units, p.grid);
+  s.parts = (int)(kv4_cta_of(ge - 1, p.total_units, p.grid) - s.c0) + 1;
+  s.part = (int)(blockIdx.x - s.c0);
+  s.group_id = blk * p.n_seqs + lo;
+  return s;
+}
+
+__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// The four f16 pairs of a word: c - 8, and 16 (c - 8) for the upper nibbles, exactly: a code under the exponent
+// of 1024 is 1024 + c (or + 16 c), and one subtraction leaves a normal number.  Codes read as f16 subnormals
+// would need no subtraction for the keys, but the tensor core aligns the 16 products of a step by their
+// operands' nominal exponents: subnormals lose 7 to 10 bits of the fp32 sum (measured: the output was 8e-6
+// off, against 1e-6 now).
+__device__ __forceinline__ void centred(uint32_t x, uint32_t (&c)[4]) {
+  const uint32_t y = x >> 8;
+  c[0] = h2_add((x & 0x000f000fu) | 0x64006400u, 0xe408e408u);
+  c[1] = h2_add((x & 0x00f000f0u) | 0x64006400u, 0xe480e480u);
+  c[2] = h2_add((y & 0x000f000fu) | 0x64006400u, 0xe408e408u);
+  c[3] = h2_add((y & 0x00f000f0u) | 0x64006400u, 0xe480e480u);
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t h2_maxabs(uint32_t a, uint32_t b) {
+  const __half2 x = __habs2(*reinterpret_cast<const __half2*>(&a));
+  const __half2 y = __habs2(*reinterpret_cast<const __half2*>(&b));
+  const __half2 m = __hmax2(x, y);
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// 2^k as fp32, -126 <= k <= 127.
+__device__ __forceinline__ float pow2i(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
+
+template <int HD>
+struct WarpState {
+  static constexpr int NB = HD / 32;
+  uint32_t qa[NB][2][4];  // A fragments of the queries: block, k16 step
+  float f;                // S f = score in exp2 units
+  float o[NB][2][4];      // O^T accumulators: block, m16 tile
+  float m, l;             // reference exponent and sum of this lane's weights, head g
+  float mb;               // 8 - m
+  float vlim;             // largest |V scale| the current vexp allows
+  uint32_t vmul;          // 2^vexp twice, f16
+  int vexp;
+};
+
+constexpr float kSlack = 5.f;      // scores may exceed the reference by this before it moves
+constexpr float kWeightExp = 8.f;  // weights are 2^(score - m + 8): at most 2^13, exact products far above f16's floor
+
+// Queries of the segment's heads as A fragments, scaled per head by a power of two (largest value in [2^11, 2^12)).
+template <int HD>
+__device__ __forceinline__ void load_queries(const Kv4DecodeParams& p, const Seg& s, int lane, WarpState<HD>& w) {
+  constexpr int NB = HD / 32;
+  const int g = lane >> 2, t = lane & 3;
+  const int heads = p.pool.kv_heads * p.group;
+  const int hg = s.hb * p.block_heads + g;  // head within the kv head's group
+  const bool have = g < p.block_heads && hg < p.group;
+  float v[NB][8];
+  if (have) {
+    const int head = s.kvh * p.group + hg;
+    const size_t row = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * heads + head) * HD;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) load8(p.q, row + 32 * b + 8 * t, p.input_f16, v[b]);
+    if (p.q_bias) {
+      const float* br = p.q_bias + ((size_t)(p.layer_begin + s.ll) * heads + head) * HD;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) add_bias8(v[b], br + 32 * b + 8 * t);
+    }
+    if (p.rope) {
+      const float* cr = p.rope_cos + (size_t)p.seqs[s.si].q_pos * (HD / 2);
+      const float* sr = p.rope_sin + (size_t)p.seqs[s.si].q_pos * (HD / 2);
+#pragma unroll
+      for (int b = 0; b < NB / 2; ++b) rope8(v[b], v[b + NB / 2], cr, sr, 32 * b + 8 * t);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[b][i]));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int k = top > 0.f ? min(max(11 - exponent_of(top), -100), 126) : 0;
+  const float sc = pow2i(k);
+  w.f = p.scale_log2 * pow2i(-k);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        // the nibbles of the second pair of a step read 16 c: its queries enter divided by 16
+        const float mul = r ? 0.0625f : 1.f;
+        const float x = v[b][4 * st + 2 * r] * sc * mul, y = v[b][4 * st + 2 * r + 1] * sc * mul;
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 hf = __half22float2(h);
+        const __half2 q = __floats2half2_rn(x - hf.x, y - hf.y);
+        hi[r] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[r] = *reinterpret_cast<const uint32_t*>(&q);
+      }
+      w.qa[b][st][0] = hi[0];
+      w.qa[b][st][1] = lo[0];
+      w.qa[b][st][2] = hi[1];
+      w.qa[b][st][3] = lo[1];
+    }
+  }
+}
+
+template <int HD>
+__device__ __forceinline__ void reset_state(WarpState<HD>& w) {
+#pragma unroll
+  for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w.o[b][i][r] = 0.f;
+  w.m = -INFINITY;
+  w.mb = INFINITY;
+  w.l = 0.f;
+  w.vlim = 0.f;
+  w.vmul = 0;
+  w.vexp = 0;
+}
+
+// Words of a lane: NB per n8 half / token-pair half j.
+template <int HD>
+__device__ __forceinline__ void lds_words(uint32_t addr, int lane, uint32_t (&w)[2][HD / 32]) {
+  if constexpr (HD == 128) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 v = lds128(addr + j * 512 + lane * 16);
+      w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+    }
+  } else {
+    const uint4 v = lds128(addr + lane * 16);
+    w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+  }
+}
+template <int HD>
+__device__ __forceinline__ void lds_scales(uint32_t addr, int t, uint32_t (&w)[2][HD / 32]) {
+  if constexpr (HD == 128) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 v = lds128(addr + j * 64 + t * 16);
+      w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+    }
+  } else {
+    const uint4 v = lds128(addr + t * 16);
+    w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+  }
+}
+
+// Attends the first `valid` (1..16) tokens of the tile at shared address `addr`.
+template <int HD>
+__device__ __forceinline__ void attend_tile(uint32_t addr, int valid, int lane, WarpState<HD>& w) {
+  using D = Dec<HD>;
+  constexpr int NB = D::NB;
+  const int t = lane & 3;
+  uint32_t kw[2][NB], ks[2][NB], vs[2][NB];
+  lds_words<HD>(addr, lane, kw);
+  lds_scales<HD>(addr + 2 * D::CB, t, ks);
+  lds_scales<HD>(addr + 2 * D::CB + D::SB, t, vs);
+
+  // scores: s[j] = tokens 8j + 2t, 8j + 2t + 1 of head g
+  uint64_t s2[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    s2[j] = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t c[4];
+      centred(kw[j][b], c);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816(acc, w.qa[b][0], c[0], c[1]);
+      mma_16816(acc, w.qa[b][1], c[2], c[3]);
+      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ks[j][b]));
+      const uint64_t d2 = f2_pack(d.x, d.y);
+      s2[j] = f2_fma(d2, f2_pack(acc[0], acc[1]), s2[j]);
+      s2[j] = f2_fma(d2, f2_pack(acc[2], acc[3]), s2[j]);
+    }
+  }
+  float s[4];
+  f2_unpack(s2[0], s[0], s[1]);
+  f2_unpack(s2[1], s[2], s[3]);
+  if (valid < kKv4Tile) {  // tokens past the sequence: no weight, whatever the tile holds there
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = 8 * (i >> 1) + 2 * t + (i & 1) < valid;
+      if (!in) {
+        s[i] = -INFINITY;
+        const uint32_t keep = (i & 1) ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vs[i >> 1][b] &= keep;
+      }
+    }
+  }
+  const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * w.f;
+  uint32_t vm = h2_maxabs(vs[0][0], vs[1][0]);
+#pragma unroll
+  for (int b = 1; b < NB; ++b) vm = h2_maxabs(vm, h2_maxabs(vs[0][b], vs[1][b]));
+  const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
+  const float vtop = fmaxf(vmf.x, vmf.y);
+  if (__any_sync(0xffffffffu, top > w.m + kSlack || vtop > w.vlim)) {
+    float tm = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
+    float alpha = 1.f;
+    if (tm > w.m + kSlack) {
+      alpha = ex2(w.m - tm);
+      w.m = tm;
+      w.mb = kWeightExp - tm;
+    }
+    float vx = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+    vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, 2));
+    float beta = 1.f;
+    if (vx > w.vlim) {
+      const int e = min(exponent_of(vx), 15);
+      const int k = min(max(-1 - e, -16), 15);  // |V scale| 2^k in [0.5, 1) now, at most 4 until it moves again
+      beta = w.vlim > 0.f ? pow2i(k - w.vexp) : 1.f;
+      w.vexp = k;
+      w.vlim = pow2i(e + 3);
+      const __half2 h = __float2half2_rn(pow2i(k));
+      w.vmul = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    w.l *= alpha;
+    const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t) * beta;
+    const float a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4) * beta;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w.o[b][i][0] *= a0;
+        w.o[b][i][1] *= a1;
+        w.o[b][i][2] *= a0;
+        w.o[b][i][3] *= a1;
+      }
+  }
+  float pr[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pr[i] = ex2(fmaf(s[i], w.f, w.mb));
+  w.l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+  uint32_t ph[2], pl[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __half2 h = __floats2half2_rn(pr[2 * j], pr[2 * j + 1]);
+    const float2 hf = __half22float2(h);
+    ph[j] = *reinterpret_cast<const uint32_t*>(&h);
+    pl[j] = pack_half2(pr[2 * j] - hf.x, pr[2 * j + 1] - hf.y);
+  }
+
+  uint32_t vw[2][NB];
+  lds_words<HD>(addr + D::CB, lane, vw);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t d = h2_mul(vs[j][b], w.vmul);
+      hi[j] = h2_mul(ph[j], d);
+      lo[j] = h2_fma(pl[j], d, h2_fma(ph[j], d, hi[j] ^ 0x80008000u));
+    }
+    uint32_t c0[4], c1[4];
+    centred(vw[0][b], c0);
+    centred(vw[1][b], c1);
+    const uint32_t a[4] = {c0[0], c0[1], c1[0], c1[1]}, c[4] = {c0[2], c0[3], c1[2], c1[3]};
+    mma_16816(w.o[b][0], a, hi[0], hi[1]);
+    mma_16816(w.o[b][1], c, hi[0], hi[1]);
+    mma_16816(w.o[b][0], a, lo[0], lo[1]);
+    mma_16816(w.o[b][1], c, lo[0], lo[1]);
+  }
+}
+
+// A warp's copies: tiles t0 + warp, + 8, ... of each segment of the CTA's range, in order, across segments.
+struct Feed {
+  long long u, u1;      // next segment's first unit, end of the CTA's range
+  int tile, t1;         // next tile and end of the current segment
+  const unsigned char* base;  // tile 0 of page 0 for the segment's layer and kv head
+  const int32_t* row;
+  int page_base;
+};
+
+template <int HD>
+__device__ __forceinline__ const unsigned char* feed_next(const Kv4DecodeParams& p, Feed& f, int warp) {
+  while (f.tile >= f.t1) {
+    if (f.u >= f.u1) return nullptr;
+    const Seg s = kv4_seg_at(p, f.u, f.u1);
+    f.u = s.next;
+    f.tile = s.t0 + warp;
+    f.t1 = s.t1;
+    const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
+    f.base = p.pool.base + rec * p.pool.tiles_per_page * Dec<HD>::TB;
+    f.row = p.page_table + (size_t)p.seqs[s.si].slot * p.max_pages_per_seq;
+    f.page_base = p.seqs[s.si].page_base;
+  }
+  const int page = kv4_page_of(p.pool, f.tile);
+  const int in = f.tile - page * p.pool.tiles_per_page;
+  const int id = f.page_base >= 0 ? f.page_base + page : f.row[page];
+  f.tile += Dec<HD>::kWarps;
+  return f.base + ((long long)id * p.pool.kv_heads * p.pool.tiles_per_page + in) * Dec<HD>::TB;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(32 * Dec<HD>::kWarps, 2) kv4_decode_kernel(const __grid_constant__ Kv4DecodeParams p) {
+  using D = Dec<HD>;
+  constexpr int NB = D::NB, W = D::kWarps, H = kKv4Heads;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + D::bar_off) + warp * D::kRing;
+  unsigned char* ring = smem + D::ring_off + warp * D::kRing * D::TB;
+  unsigned char* new_tile = smem + D::new_off;
+  float4* red = reinterpret_cast<float4*>(smem + D::red_off);
+  float* sm_m = reinterpret_cast<float*>(smem + D::stat_off);  // [W][8]
+  float* sm_l = sm_m + W * H;
+  int* sm_flag = reinterpret_cast<int*>(sm_l + W * H);
+
+  if (lane == 0) {
+    for (int i = 0; i < D::kRing; ++i) mbar_init(&bars[i], 1);
+    fence_mbarrier_init();
+    fence_proxy_async_shared();
+  }
+  __syncwarp();
+
+  const long long u1 = stage_start(blockIdx.x + 1, p.total_units, p.grid);
+  long long u = stage_start(blockIdx.x, p.total_units, p.grid);
+  const long long u_begin = u;
+  Feed feed{u, u1, 0, 0, nullptr, nullptr, -1};
+  auto issue = [&](int slot) {
+    const unsigned char* src = feed_next<HD>(p, feed, warp);
+    if (src && lane == 0) {
+      mbar_arrive_expect_tx(&bars[slot], D::TB);
+      bulk_load(ring + slot * D::TB, src, D::TB, &bars[slot]);
+    }
+    return src != nullptr;
+  };
+  int issued = 0, used = 0;      // tiles copied / consumed by this warp
+  for (int i = 0; i < D::kRing; ++i) issued += issue(i) ? 1 : 0;
+  bool ok = true;                // false: a wait ran out; the warp computes no more
+
+  WarpState<HD> w;
+  while (u < u1) {
+    const Seg s = kv4_seg_at(p, u, u1);
+    const Kv4Seq& sq = p.seqs[s.si];
+    const bool append = p.k_new != nullptr && s.last;
+    const int n_tiles = s.t1 - s.t0;
+    const bool appender = append && warp == n_tiles % W;
+    if (appender) {
+      // the new token: quantised into the cache (by the first head block) and into a tile of its own here
+      const size_t at = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * p.pool.kv_heads + s.kvh) * HD;
+      const size_t brow = ((size_t)(p.layer_begin + s.ll) * p.pool.kv_heads + s.kvh) * HD;
+      float k[4], v[4];
+      load_row<HD>(p.k_new, p.v_new, at, p.input_f16, p.k_bias ? p.k_bias + brow : nullptr,
+                   p.k_bias ? p.v_bias + brow : nullptr,
+                   p.rope ? p.rope_cos + (size_t)sq.new_pos * (HD / 2) : nullptr,
+                   p.rope ? p.rope_sin + (size_t)sq.new_pos * (HD / 2) : nullptr, lane, k, v);
+      float k2[4] = {k[0], k[1], k[2], k[3]}, v2[4] = {v[0], v[1], v[2], v[3]};
+      store_row<HD>(new_tile, 0, lane, k, v);
+      if (s.hb == 0) {
+        unsigned char* dst = tile_ptr(p.pool, p.page_table + (size_t)sq.slot * p.max_pages_per_seq, p.layer_begin + s.ll,
+                                      s.kvh, sq.len / kKv4Tile, D::TB);
+        store_row<HD>(dst, sq.len % kKv4Tile, lane, k2, v2);
+      }
+    }
+    load_queries<HD>(p, s, lane, w);
+    reset_state<HD>(w);
+    for (int tile = s.t0 + warp; tile < s.t1; tile += W) {
+      const int slot = used % D::kRing;
+      if (ok) ok = mbar_wait_warp(&bars[slot], (used / D::kRing) & 1);
+      if (!ok) {
+        if (lane == 0) set_error(p.error, 60);
+        break;
+      }
+      attend_tile<HD>(smem_u32(ring + slot * D::TB), min(sq.len - tile * kKv4Tile, kKv4Tile), lane, w);
+      __syncwarp();
+      ++used;
+      issued += issue(slot) ? 1 : 0;
+    }
+    if (appender) {
+      __syncwarp();
+      attend_tile<HD>(smem_u32(new_tile), 1, lane, w);
+    }
+
+    // merge the warps' states: m and l per head first, then O in two rounds
+    float l = w.l;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) {
+      sm_m[warp * H + g] = w.m;
+      sm_l[warp * H + g] = l;
+    }
+    __syncthreads();
+    auto part_weight = [](float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); };
+    {
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+      for (int i = 0; i < W; ++i) {
+        mx0 = fmaxf(mx0, sm_m[i * H + 2 * t]);
+        mx1 = fmaxf(mx1, sm_m[i * H + 2 * t + 1]);
+      }
+      const float vs = pow2i(-w.vexp);
+      const float c0 = part_weight(sm_m[warp * H + 2 * t], mx0) * vs;
+      const float c1 = part_weight(sm_m[warp * H + 2 * t + 1], mx1) * vs;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          w.o[b][i][0] *= c0;
+          w.o[b][i][1] *= c1;
+          w.o[b][i][2] *= c0 * 0.0625f;
+          w.o[b][i][3] *= c1 * 0.0625f;
+        }
+    }
+    auto o_item = [&](int b, int c) {
+      return make_float4(w.o[b][0][c], w.o[b][0][2 + c], w.o[b][1][c], w.o[b][1][2 + c]);
+    };
+    if (warp >= W / 2) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) red[(warp - W / 2) * D::kItems + (b * 2 + c) * 32 + lane] = o_item(b, c);
+    }
+    __syncthreads();
+    if (warp < W / 2) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float4* slot = &red[warp * D::kItems + (b * 2 + c) * 32 + lane];
+          const float4 x = *slot, y = o_item(b, c);
+          *slot = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+    }
+    __syncthreads();
+    // item i: block i / 64, heads 2 (i % 4) + (i / 32) % 2, dims 4 ((i % 32) / 4) .. + 3 of the block
+    const int i = threadIdx.x;
+    const int head = 2 * (i & 3) + ((i >> 5) & 1);
+    const int dim = 32 * (i >> 6) + 4 * ((i & 31) >> 2);
+    const bool mine = i < D::kItems;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.f;
+    if (mine) {
+      for (int k = 0; k < W / 2; ++k) {
+        const float4 x = red[k * D::kItems + i];
+        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+      }
+      for (int k = 0; k < W; ++k) top = fmaxf(top, sm_m[k * H + head]);
+      for (int k = 0; k < W; ++k) sum += sm_l[k * H + head] * part_weight(sm_m[k * H + head], top);
+    }
+    bool write = true;
+    if (s.parts > 1) {
+      // publish this part; the last of the group's parts to arrive folds them all, in part order
+      constexpr int rec = kv4_record_floats(HD);
+      // a CTA's first segment uses its slot 0, its last another one: at most two of its segments are parts
+      float* mine_rec = p.partials + ((size_t)blockIdx.x * 2 + (u == u_begin ? 0 : 1)) * rec;
+      if (mine) {
+        reinterpret_cast<float4*>(mine_rec)[i] = acc;
+        if (dim == 0) {
+          mine_rec[H * HD + head] = top;
+          mine_rec[H * HD + H + head] = sum;
+        }
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        __threadfence();
+        const uint32_t old = atomicAdd(&p.counters[s.group_id], 1u);
+        *sm_flag = old == (uint32_t)s.parts - 1u;
+        __threadfence();
+      }
+      __syncthreads();
+      write = *sm_flag != 0;
+      if (write && mine) {
+        // part k is CTA c0 + k's: its first segment unless the CTA's range began before the group
+        const long long gb = u - (long long)(s.t0 / kKv4UnitTiles);
+        auto rec_of = [&](int k) {
+          const long long c = s.c0 + k;
+          const int slot = stage_start(c, p.total_units, p.grid) >= gb ? 0 : 1;
+          return p.partials + ((size_t)c * 2 + slot) * rec;
+        };
+        float all = -INFINITY;
+        for (int k = 0; k < s.parts; ++k) all = fmaxf(all, __ldcg(rec_of(k) + H * HD + head));
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < s.parts; ++k) {
+          const float* r = rec_of(k);
+          const float wt = part_weight(__ldcg(r + H * HD + head), all);
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(r) + i);
+          acc.x = fmaf(wt, x.x, acc.x);
+          acc.y = fmaf(wt, x.y, acc.y);
+          acc.z = fmaf(wt, x.z, acc.z);
+          acc.w = fmaf(wt, x.w, acc.w);
+          sum = fmaf(wt, __ldcg(r + H * HD + H + head), sum);
+        }
+        top = all;
+      }
+      if (write && threadIdx.x == 0) p.counters[s.group_id] = 0;
+    }
+    const int hg = s.hb * p.block_heads + head;
+    if (write && mine && head < p.block_heads && hg < p.group) {
+      const size_t row = ((size_t)s.ll * p.seq_total + p.seq_base + s.si) * (p.pool.kv_heads * p.group) +
+                         s.kvh * p.group + hg;
+      if (p.partial_out) {
+        constexpr float k = 0x1p-8f;  // 2^-kWeightExp
+        float* o = p.out + row * (HD + 2);
+        o[dim] = acc.x * k;
+        o[dim + 1] = acc.y * k;
+        o[dim + 2] = acc.z * k;
+        o[dim + 3] = acc.w * k;
+        if (dim == 0) {
+          o[HD] = top;
+          o[HD + 1] = sum * k;
+        }
+      } else {
+        const float r = sum == 0.f ? 0.f : 1.f / sum;  // no token at all: zeros
+        *reinterpret_cast<float4*>(p.out + row * HD + dim) = make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r);
+      }
+    }
+    u = s.next;
+    __syncthreads();  // the merge buffers and the new token's tile are free again
+  }
+  if (!ok) {
+    // copies of this warp may still be in flight: let them land before the CTA leaves
+    for (; used < issued; ++used) (void)mbar_wait_warp(&bars[used % D::kRing], (used / D::kRing) & 1);
+  }
+}
+
+template <int HD>
+cudaError_t launch_decode_t(const Kv4DecodeParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = set_smem_limit_once(done, reinterpret_cast<const void*>(kv4_decode_kernel<HD>), Dec<HD>::smem);
+  if (e != cudaSuccess) return e;
+  kv4_decode_kernel<HD><<<p.grid, 32 * Dec<HD>::kWarps, Dec<HD>::smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+long long row_items(const Kv4RowsParams& p) {
+  const long long tiles = (p.first + p.n_tokens - 1) / kKv4Tile - p.first / kKv4Tile + 1;
+  return tiles * p.pool.kv_heads * p.n_layers;
+}
+
+}  // namespace
+
+int kv4_decode_ctas_per_sm() { return 2; }
+
+void plan_kv4_decode(Kv4DecodeParams& p, long long max_grid) {
+  int acc = 0;
+  for (int i = 0; i < p.n_seqs; ++i) {
+    p.seqs[i].unit_begin = acc;
+    acc += kv4_units(p.seqs[i].len);
+  }
+  p.block_units = acc;
+  p.total_units = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks * acc;
+  const long long want = (p.total_units + 1) / 2;  // 128 tokens a CTA: one tile a warp
+  p.grid = (int32_t)(want < max_grid ? want : max_grid);
+}
+
+cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream_t s) {
+  return head_dim == 128 ? launch_decode_t<128>(p, s) : launch_decode_t<64>(p, s);
+}
+
+cudaError_t launch_kv4_append(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
+  const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
+  if (head_dim == 128) kv4_append_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else kv4_append_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
+  const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
+  if (head_dim == 128) kv4_read_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else kv4_read_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv4_raw(const Kv4RowsParams& p, int head_dim, bool to_pool, cudaStream_t s) {
+  const long long n = (long long)p.n_layers * p.n_tokens * p.pool.kv_heads * (head_dim / 32);
+  const unsigned grid = (unsigned)((n + 127) / 128);
+  if (head_dim == 128) kv4_raw_kernel<128><<<grid, 128, 0, s>>>(p, to_pool ? 1 : 0);
+  else kv4_raw_kernel<64><<<grid, 128, 0, s>>>(p, to_pool ? 1 : 0);
+  return cudaGetLastError();
+}
+
+}  // namespace te

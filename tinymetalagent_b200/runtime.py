@@ -38,6 +38,7 @@ TE_ATTN_RMSNORM_INPUT = 1 << 7
 TE_ATTN_SWIGLU_INPUT = 1 << 8
 TE_ATTN_EXACT_Q = 1 << 9
 TE_ATTN_STEP_HEAD = 1 << 10
+TE_ATTN_OUTPUT_F16 = 1 << 11
 TE_ATTN_QUANT_GGUF_Q4_0 = 4
 TE_ATTN_QUANT_GGUF_Q8_0 = 8
 
@@ -163,6 +164,18 @@ SIGNATURES: dict[str, tuple] = {
     "te_qwen_step_create": (_int, [_vp, ctypes.POINTER(QwenStepDesc), ctypes.POINTER(_vp)]),
     "te_qwen_step_run": (_int, [_vp, _sz, _vp, _vp, _vp, _vp, ctypes.c_uint32]),
     "te_qwen_step_free": (None, [_vp]),
+    "te_kv4_cache_create": (_int, [_vp, ctypes.POINTER(KVCacheDesc), ctypes.POINTER(_vp)]),
+    "te_kv4_cache_free": (None, [_vp]),
+    "te_kv4_cache_seq_reset": (_int, [_vp, _sz, _sz]),
+    "te_kv4_cache_seq_truncate": (_int, [_vp, _sz, _sz]),
+    "te_kv4_cache_seq_length": (_int, [_vp, _sz, ctypes.POINTER(_sz)]),
+    "te_kv4_cache_reserve": (_int, [_vp, _sz, _sz]),
+    "te_kv4_cache_set_qkv_bias": (_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "te_kv4_append": (_int, [_vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _vp, ctypes.c_uint32]),
+    "te_kv4_cache_read": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, ctypes.c_uint32]),
+    "te_kv4_cache_write_q4_0": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp]),
+    "te_kv4_cache_read_q4_0": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp]),
+    "te_kv4_attention_decode": (_int, [_vp, _sz, _sz, _u32p, _sz, _i64p, _vp, _vp, _vp, _sz, _vp, ctypes.c_uint32]),
     "te_attention_decode_paged_noalloc": (_int, [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _vp]),
     "te_attention_decode_paged_noalloc_status": (_int, [_vp, ctypes.POINTER(ctypes.c_int)]),
 }
@@ -320,6 +333,10 @@ class AttnEngine:
     def kv_cache(self, **kw) -> "KVCache":
         return KVCache(self, **kw)
 
+    def kv4_cache(self, **kw) -> "KV4Cache":
+        """A paged cache held in 4 bits (te_kv4_cache_create); the arguments are kv_cache's."""
+        return KV4Cache(self, **kw)
+
     def matvec_gguf_fused(self, quant: int, w, rows: int, cols: int, x, y, flags: int, norm_weight=None,
                           eps: float = 0.0, n_vectors: int = 1) -> None:
         """y[v] = W p(x[v]) (or y[v] += that, with TE_ATTN_ACCUMULATE), p the RMSNorm (TE_ATTN_RMSNORM_INPUT,
@@ -387,6 +404,30 @@ class Exchange:
             self.handle = None
 
 
+def _bias_arrays(q_width: int, kv_width: int, q_bias, k_bias, v_bias):
+    """The three projection biases as contiguous fp32 arrays (None stays None), and their row count."""
+    import numpy as np
+    arrs = []
+    n = None
+    for b, width in ((q_bias, q_width), (k_bias, kv_width),
+                     (v_bias, kv_width)):
+        if b is None:
+            arrs.append(None)
+            continue
+        if hasattr(b, "detach"):
+            b = b.detach().float().contiguous()
+        else:
+            b = np.ascontiguousarray(np.asarray(b, dtype=np.float32))
+        rows = int(b.numel() if hasattr(b, "numel") else b.size) // width
+        n = rows if n is None else n
+        if rows * width != (b.numel() if hasattr(b, "numel") else b.size) or rows != n:
+            raise ValueError("bias shapes disagree with heads / kv_heads * head_dim")
+        arrs.append(b)
+    if n is None:
+        raise ValueError("no bias given")
+    return arrs, n
+
+
 class KVCache:
     """Paged f16 KV cache in HBM: [layers][pages][kv_heads][page_tokens][head_dim] per K and V."""
 
@@ -451,28 +492,8 @@ class KVCache:
         """fp32 projection biases of layers [layer_begin, +n): q_bias [n][heads * head_dim], k_bias and
         v_bias [n][kv_heads * head_dim] (numpy or torch; None = zeros).  Calls with TE_ATTN_QKV_BIAS add
         them to the raw q/k/v inputs before RoPE and rounding."""
-        import numpy as np
-        arrs = []
-        n = None
-        for b, width in ((q_bias, heads * self.head_dim), (k_bias, self.kv_heads * self.head_dim),
-                         (v_bias, self.kv_heads * self.head_dim)):
-            if b is None:
-                arrs.append(None)
-                continue
-            if hasattr(b, "detach"):
-                b = b.detach().float().contiguous()
-            else:
-                b = np.ascontiguousarray(np.asarray(b, dtype=np.float32))
-            rows = int(b.numel() if hasattr(b, "numel") else b.size) // width
-            n = rows if n is None else n
-            if rows * width != (b.numel() if hasattr(b, "numel") else b.size) or rows != n:
-                raise ValueError("bias shapes disagree with heads / kv_heads * head_dim")
-            arrs.append(b)
-        if n is None:
-            raise ValueError("no bias given")
-        ptr = lambda b: None if b is None else _addr(b)  # noqa: E731
-        self._c(self.lib.te_kv_cache_set_qkv_bias(self.handle, layer_begin, n, heads, ptr(arrs[0]), ptr(arrs[1]),
-                                                  ptr(arrs[2])))
+        arrs, n = _bias_arrays(heads * self.head_dim, self.kv_heads * self.head_dim, q_bias, k_bias, v_bias)
+        self._c(self.lib.te_kv_cache_set_qkv_bias(self.handle, layer_begin, n, heads, *map(_addr, arrs)))
 
     def read_f16(self, layer: int, seq: int, token_begin: int, n_tokens: int):
         import numpy as np
@@ -498,6 +519,170 @@ class KVCache:
                 flags: int = 0) -> None:
         self._c(self.lib.te_attention_prefill(self.handle, layer_begin, n_layers, seq, _addr(q), _addr(k), _addr(v),
                                               n_tokens, heads, _addr(out), flags))
+
+
+class KV4Cache:
+    """Paged KV cache held as GGUF Q4_0 blocks, 4.5 bits a value (te_kv4_cache): the writer quantises, the
+    decode attention reads the codes, `read` gives rows back.
+
+    Sequences, pages, RoPE positions, biases, flags and streams work as in KVCache: the calls queue work on
+    the engine's stream, and a caller that makes its tensors on another stream orders the two.  Tensors are
+    checked (CUDA device, type, size, layout) and refused with ValueError; raw addresses are taken as given."""
+
+    def __init__(self, engine: AttnEngine, layers: int, max_seqs: int, max_tokens_per_seq: int, kv_heads: int,
+                 head_dim: int, page_tokens: int = 128, total_pages: int = 0, max_position: int = 0,
+                 rope_theta: float = 1e6):
+        self.engine = engine
+        self.lib = engine.lib
+        d = self.lib.te_kv_cache_default_desc()
+        d.layers, d.max_seqs, d.max_tokens_per_seq = layers, max_seqs, max_tokens_per_seq
+        d.kv_heads, d.head_dim, d.page_tokens = kv_heads, head_dim, page_tokens
+        d.total_pages, d.max_position, d.rope_theta = total_pages, max_position, rope_theta
+        handle = _vp()
+        engine.check(self.lib.te_kv4_cache_create(engine.handle, ctypes.byref(d), ctypes.byref(handle)))
+        self.handle = handle
+        engine._caches.add(self)
+        self.layers, self.max_seqs, self.kv_heads, self.head_dim = layers, max_seqs, kv_heads, head_dim
+        self.page_tokens, self.max_tokens_per_seq, self.rope_theta = page_tokens, max_tokens_per_seq, rope_theta
+
+    def close(self) -> None:
+        if getattr(self, "handle", None) and getattr(self.engine, "handle", None):
+            self.lib.te_kv4_cache_free(self.handle)
+        self.handle = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _c(self, status: int) -> None:
+        self.engine.check(status)
+
+    def _tensor(self, x, name: str, values: int, *dtypes: str) -> Optional[int]:
+        """Address of a contiguous CUDA tensor of `values` values of one of `dtypes`, or of a raw address."""
+        if x is None or isinstance(x, int):
+            return x
+        if not hasattr(x, "is_cuda"):
+            raise TypeError(f"{name}: a CUDA tensor or an address")
+        if not x.is_cuda or x.device.index != self.engine.device:
+            raise ValueError(f"{name}: not on the engine's device")
+        if str(x.dtype)[6:] not in dtypes:
+            raise ValueError(f"{name}: type {x.dtype}, expected {' or '.join(dtypes)}")
+        if x.numel() != values or not x.is_contiguous():
+            raise ValueError(f"{name}: expected {values} contiguous values")
+        return x.data_ptr()
+
+    def reset(self, seq: int, position_offset: int = 0) -> None:
+        self._c(self.lib.te_kv4_cache_seq_reset(self.handle, seq, position_offset))
+
+    def truncate(self, seq: int, length: int) -> None:
+        self._c(self.lib.te_kv4_cache_seq_truncate(self.handle, seq, length))
+
+    def reserve(self, seq: int, tokens: int) -> None:
+        """Map pages for `tokens` tokens now (graph-capturable decode steps afterwards)."""
+        self._c(self.lib.te_kv4_cache_reserve(self.handle, seq, tokens))
+
+    def length(self, seq: int) -> int:
+        n = _sz()
+        self._c(self.lib.te_kv4_cache_seq_length(self.handle, seq, ctypes.byref(n)))
+        return n.value
+
+    def set_qkv_bias(self, layer_begin: int, heads: int, q_bias=None, k_bias=None, v_bias=None) -> None:
+        """fp32 projection biases, as KVCache.set_qkv_bias."""
+        arrs, n = _bias_arrays(heads * self.head_dim, self.kv_heads * self.head_dim, q_bias, k_bias, v_bias)
+        self._c(self.lib.te_kv4_cache_set_qkv_bias(self.handle, layer_begin, n, heads, *map(_addr, arrs)))
+
+    def _new_rows(self, x, name: str, n_layers: int, n_tokens: int, dtype: str):
+        """(address, token stride) of new rows: a contiguous tensor, or a view whose tokens are evenly spaced
+        (columns of a wider projection output, [.., n_tokens, kv_heads * head_dim] or [.., kv_heads, head_dim])."""
+        row = self.kv_heads * self.head_dim
+        if isinstance(x, int) or x.is_contiguous():
+            return self._tensor(x, name, n_layers * n_tokens * row, dtype), row
+        if x.dim() >= 2 and tuple(x.shape[-2:]) == (self.kv_heads, self.head_dim) and \
+                x.stride(-2) == self.head_dim:
+            lead = x.shape[:-2], x.stride()[:-2]
+        elif x.shape[-1] == row:
+            lead = x.shape[:-1], x.stride()[:-1]
+        else:
+            raise ValueError(f"{name}: expected rows of kv_heads * head_dim contiguous values")
+        # outermost first: each leading dimension must continue the even spacing of the tokens
+        stride, count = None, 1
+        for size, st in zip(reversed(lead[0]), reversed(lead[1])):
+            if size != 1:
+                if stride is None:
+                    stride = st
+                elif st != count * stride:
+                    raise ValueError(f"{name}: tokens are not evenly spaced")
+            count *= size
+        if x.stride(-1) != 1 or count != n_layers * n_tokens:
+            raise ValueError(f"{name}: expected n_layers * n_tokens rows of contiguous values")
+        if not x.is_cuda or x.device.index != self.engine.device or str(x.dtype)[6:] != dtype:
+            raise ValueError(f"{name}: expected {dtype} on the engine's device")
+        return x.data_ptr(), row if stride is None else stride
+
+    def append(self, layer_begin: int, n_layers: int, seq: int, k, v, n_tokens: int, k_stored=None, v_stored=None,
+               flags: int = 0, token_stride: int = 0) -> None:
+        """Quantises n_tokens rows per layer into the cache (te_kv4_append): k and v
+        [n_layers][n_tokens][kv_heads][head_dim] fp32, or f16 with TE_ATTN_INPUT_F16, contiguous or evenly spaced
+        views (raw addresses: token_stride values apart).  k_stored / v_stored receive the rows as the cache now
+        holds them, fp32, or f16 with TE_ATTN_OUTPUT_F16."""
+        dtype = "float16" if flags & TE_ATTN_INPUT_F16 else "float32"
+        n = n_layers * n_tokens * self.kv_heads * self.head_dim
+        kp, ks = self._new_rows(k, "k", n_layers, n_tokens, dtype)
+        vp, vs = self._new_rows(v, "v", n_layers, n_tokens, dtype)
+        if token_stride == 0:
+            if ks != vs and n_layers * n_tokens > 1:
+                raise ValueError("k and v: different token strides")
+            token_stride = ks
+        stored = "float16" if flags & TE_ATTN_OUTPUT_F16 else "float32"
+        self._c(self.lib.te_kv4_append(self.handle, layer_begin, n_layers, seq, kp, vp, n_tokens, token_stride,
+                                       self._tensor(k_stored, "k_stored", n, stored),
+                                       self._tensor(v_stored, "v_stored", n, stored), flags))
+
+    def read(self, layer_begin: int, n_layers: int, seq: int, token_begin: int, n_tokens: int, k, v,
+             flags: int = 0) -> None:
+        """Rows of tokens [token_begin, +n_tokens) into k and v [n_layers][n_tokens][kv_heads][head_dim]: fp32,
+        or f16 with TE_ATTN_OUTPUT_F16."""
+        dtype = "float16" if flags & TE_ATTN_OUTPUT_F16 else "float32"
+        n = n_layers * n_tokens * self.kv_heads * self.head_dim
+        self._c(self.lib.te_kv4_cache_read(self.handle, layer_begin, n_layers, seq, token_begin, n_tokens,
+                                           self._tensor(k, "k", n, dtype), self._tensor(v, "v", n, dtype), flags))
+
+    def _block_bytes(self, n_layers: int, n_tokens: int) -> int:
+        return n_layers * n_tokens * self.kv_heads * (self.head_dim // 32) * 18
+
+    def write_q4_0(self, layer_begin: int, n_layers: int, seq: int, token_begin: int, n_tokens: int, k, v) -> None:
+        """Raw Q4_0 blocks (uint8 tensors [n_layers][n_tokens][kv_heads][head_dim / 32][18]) into the cache."""
+        n = self._block_bytes(n_layers, n_tokens)
+        self._c(self.lib.te_kv4_cache_write_q4_0(self.handle, layer_begin, n_layers, seq, token_begin, n_tokens,
+                                                 self._tensor(k, "k", n, "uint8"), self._tensor(v, "v", n, "uint8")))
+
+    def read_q4_0(self, layer_begin: int, n_layers: int, seq: int, token_begin: int, n_tokens: int, k, v) -> None:
+        """The stored blocks of tokens [token_begin, +n_tokens) into uint8 tensors (write_q4_0's layout)."""
+        n = self._block_bytes(n_layers, n_tokens)
+        self._c(self.lib.te_kv4_cache_read_q4_0(self.handle, layer_begin, n_layers, seq, token_begin, n_tokens,
+                                                self._tensor(k, "k", n, "uint8"), self._tensor(v, "v", n, "uint8")))
+
+    def decode(self, layer_begin: int, n_layers: int, seq_ids: Sequence[int], q, out, heads: int,
+               k_new=None, v_new=None, q_positions: Optional[Sequence[int]] = None, flags: int = 0) -> None:
+        """One decode step (te_kv4_attention_decode): q [n_layers][n_seqs][heads][head_dim], k_new / v_new
+        [n_layers][n_seqs][kv_heads][head_dim] (fp32, or f16 with TE_ATTN_INPUT_F16), out fp32 in q's shape, or
+        records [..][heads][head_dim + 2] with TE_ATTN_PARTIAL."""
+        n = len(seq_ids)
+        dtype = "float16" if flags & TE_ATTN_INPUT_F16 else "float32"
+        rows = n_layers * n
+        hd, kv = self.head_dim, rows * self.kv_heads * self.head_dim
+        ids = (ctypes.c_uint32 * n)(*seq_ids)
+        qp = None
+        if q_positions is not None:
+            if len(q_positions) != n:
+                raise ValueError("one query position per sequence")
+            qp = (ctypes.c_int64 * n)(*q_positions)
+        self._c(self.lib.te_kv4_attention_decode(
+            self.handle, layer_begin, n_layers, ids, n, qp, self._tensor(q, "q", rows * heads * hd, dtype),
+            self._tensor(k_new, "k_new", kv, dtype), self._tensor(v_new, "v_new", kv, dtype), heads,
+            self._tensor(out, "out", rows * heads * (hd + (2 if flags & TE_ATTN_PARTIAL else 0)), "float32"), flags))
 
 
 class QwenStep:
