@@ -1,6 +1,6 @@
 // Kernels of the 4-bit KV cache (layout: te_kv4.h): the quantising append,
-// the read-back, the raw Q4_0 import/export, and the decode attention on the
-// tensor cores (tcgen05), which widens the codes only on their way into TMEM.
+// the read-back, the raw Q4_0 import/export, and the decode attention that
+// consumes the codes on the tensor cores without widening the cache.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -10,10 +10,6 @@
 #include "te_kv4.h"
 #include "te_ptx.cuh"
 #include "te_rope.cuh"
-
-#ifndef KV4_CTAS
-#define KV4_CTAS 3
-#endif
 
 namespace te {
 namespace {
@@ -53,9 +49,13 @@ __device__ __forceinline__ void q4_quantise(const float (&x)[4], int lane, uint3
 // The value a code stands for (exact in fp32: 4 by 11 bits).
 __device__ __forceinline__ float q4_value(uint32_t c, float d) { return (float)((int)c - 8) * d; }
 
-// Bits of 4 consecutive codes in their K word: h = 0 the lower 4 of the word's 8 codes, 1 the upper.
+// Bits of 4 consecutive codes in their K word (dims 8t + 4h .. + 3, h the half
+// of the word's 8 dims) and in their V halfword.
 __device__ __forceinline__ uint32_t k_bits(const uint32_t (&c)[4], int h) {
   return (c[0] | c[1] << 16 | c[2] << 4 | c[3] << 20) << (8 * h);
+}
+__device__ __forceinline__ uint32_t v_bits(const uint32_t (&c)[4]) {
+  return c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12;
 }
 
 // One token's key and value row, spread over a warp: lane l holds 4 values
@@ -111,402 +111,361 @@ __device__ __forceinline__ void rope4(float (&k)[4], const float* cr, const floa
   }
 }
 
-// Quantises a token's rows: kw = its K word (complete in both lanes of a pair), vc its V codes, and the scales
-// (in every lane of a block).  The whole warp calls it.  On return k and v hold the values the codes stand for.
-// At head_dim 64 the key's results are in lanes 0-15, the value's in lanes 16-31.
+// Quantises the row and writes its codes and scales at token slot `tok` of the
+// tile at `tile` (shared or global memory).  The whole warp calls it.  On
+// return k and v hold the values the codes stand for.
 template <int HD>
-__device__ __forceinline__ void quantise_row(int lane, float (&k)[4], float (&v)[4], uint32_t& kw, __half& kd,
-                                             uint32_t (&vc)[4], __half& vd) {
+__device__ __forceinline__ void store_row(unsigned char* tile, int tok, int lane, float (&k)[4], float (&v)[4]) {
+  constexpr int CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
   using R = RowDims<HD>;
-  uint32_t c[4];
-  if constexpr (HD == 128) {
-    q4_quantise(k, lane, c, kd);
-    q4_quantise(v, lane, vc, vd);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      k[i] = q4_value(c[i], __half2float(kd));
-      v[i] = q4_value(vc[i], __half2float(vd));
+  const int j = tok >> 3, g = tok & 7, tp = (tok & 7) >> 1, e = tok & 1;
+  const int dim = R::dim(lane), b = dim >> 5;
+  auto put_k = [&](const uint32_t(&c)[4], __half d) {
+    uint32_t w = k_bits(c, lane & 1);
+    w |= __shfl_xor_sync(0xffffffffu, w, 1);
+    if (R::has_k(lane)) {
+      if ((lane & 1) == 0) {
+        *reinterpret_cast<uint32_t*>(tile + kv4_word_at(HD, j, 4 * g + ((dim & 31) >> 3), b)) = w;
+      }
+      if ((lane & 7) == 0) {
+        *reinterpret_cast<__half*>(tile + 2 * CB + kv4_scale_at(HD, j, tp, b, e)) = d;
+      }
     }
+  };
+  auto put_v = [&](const uint32_t(&c)[4], __half d) {
+    if (R::has_v(lane)) {
+      *reinterpret_cast<uint16_t*>(tile + CB + kv4_word_at(HD, j, 4 * ((dim & 31) >> 2) + tp, b) + 2 * e) =
+          (uint16_t)v_bits(c);
+      if ((lane & 7) == 0) {
+        *reinterpret_cast<__half*>(tile + 2 * CB + SB + kv4_scale_at(HD, j, tp, b, e)) = d;
+      }
+    }
+  };
+  uint32_t c[4];
+  __half d;
+  if constexpr (HD == 128) {
+    q4_quantise(k, lane, c, d);
+    put_k(c, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = q4_value(c[i], __half2float(d));
+    q4_quantise(v, lane, c, d);
+    put_v(c, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q4_value(c[i], __half2float(d));
   } else {
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = R::has_k(lane) ? k[i] : v[i];
-    q4_quantise(x, lane, c, kd);
-    vd = kd;
+    q4_quantise(x, lane, c, d);
+    put_k(c, d);
+    put_v(c, d);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vc[i] = c[i];
-      k[i] = v[i] = q4_value(c[i], __half2float(kd));
-    }
+    for (int i = 0; i < 4; ++i) k[i] = v[i] = q4_value(c[i], __half2float(d));
   }
-  kw = k_bits(c, lane & 1);
-  kw |= __shfl_xor_sync(0xffffffffu, kw, 1);
 }
 
-// A token's raw key and value rows at element offset `at`.
+// A token's raw key and value rows at element offset `at`, with bias and RoPE.
 template <int HD>
-__device__ __forceinline__ void fetch_row(const void* kp, const void* vp, size_t at, int f16, int lane, float (&k)[4],
-                                          float (&v)[4]) {
+__device__ __forceinline__ void load_row(const void* kp, const void* vp, size_t at, int f16, const float* kb,
+                                         const float* vb, const float* cr, const float* sr, int lane, float (&k)[4],
+                                         float (&v)[4]) {
   using R = RowDims<HD>;
+  const int dim = R::dim(lane);
 #pragma unroll
   for (int i = 0; i < 4; ++i) k[i] = v[i] = 0.f;
-  if (R::has_k(lane)) load4(kp, at + R::dim(lane), f16, k);
-  if (R::has_v(lane)) load4(vp, at + R::dim(lane), f16, v);
-}
-// Their bias and RoPE (null pointers: none).
-template <int HD>
-__device__ __forceinline__ void prepare_row(const float* kb, const float* vb, const float* cr, const float* sr,
-                                            int lane, float (&k)[4], float (&v)[4]) {
-  using R = RowDims<HD>;
+  if (R::has_k(lane)) load4(kp, at + dim, f16, k);
+  if (R::has_v(lane)) load4(vp, at + dim, f16, v);
   if (kb) {
-    if (R::has_k(lane)) add_bias4(k, kb + R::dim(lane));
-    if (R::has_v(lane)) add_bias4(v, vb + R::dim(lane));
+    if (R::has_k(lane)) add_bias4(k, kb + dim);
+    if (R::has_v(lane)) add_bias4(v, vb + dim);
   }
   if (cr) rope4<HD>(k, cr, sr, lane);
 }
 
-// Quotient of a unit index by units_per_page: the product with the rounded-up
-// reciprocal is at most one too large (its excess is below unit / 2^32 < 1).
-__device__ __forceinline__ int kv4_page_of(const Kv4Pool& p, int unit) {
-  if (p.upp_magic == 0) return unit;
-  int q = (int)__umulhi((uint32_t)unit, p.upp_magic);
-  if (q * p.units_per_page > unit) --q;
+// Quotient of a tile index by tiles_per_page: the product with the rounded-up
+// reciprocal is at most one too large (its excess is below t / 2^32 < 1).
+__device__ __forceinline__ int kv4_page_of(const Kv4Pool& p, int tile) {
+  int q = (int)__umulhi((uint32_t)tile, p.tpp_magic);
+  if (q * p.tiles_per_page > tile) --q;
   return q;
 }
-__device__ __forceinline__ unsigned char* unit_ptr(const Kv4Pool& p, const int32_t* page_row, int layer, int kvh,
-                                                   int unit, int unit_bytes) {
-  const int page = kv4_page_of(p, unit);
-  const int in = unit - page * p.units_per_page;
+
+__device__ __forceinline__ unsigned char* tile_ptr(const Kv4Pool& p, const int32_t* page_row, int layer, int kvh,
+                                                   int tile, int tile_bytes) {
+  const int page = kv4_page_of(p, tile);
+  const int in = tile - page * p.tiles_per_page;
   const long long rec = ((long long)layer * p.num_pages + page_row[page]) * p.kv_heads + kvh;
-  return p.base + (rec * p.units_per_page + in) * unit_bytes;
+  return p.base + (rec * p.tiles_per_page + in) * tile_bytes;
 }
 
 // ---- append -------------------------------------------------------------------
 
-// One CTA per (layer, kv head, 32 tokens), a warp per 8 of them (a V word): the half unit is assembled in shared
-// memory, with the tokens it already holds if the new ones do not fill it, and written in 16-byte pieces.
+constexpr int kRowWarps = 4;
+
+// One warp per (layer, kv head, tile of 16 tokens): the tile is assembled in
+// shared memory (with the tokens it already holds, if any) and written whole.
 template <int HD>
-__global__ void __launch_bounds__(128) kv4_append_kernel(const Kv4RowsParams p) {
-  constexpr int UB = kv4_unit_bytes(HD), NB = HD / 32;
-  constexpr int kSc = 32 * NB * 2;  // bytes of one side's scales
-  __shared__ __align__(16) unsigned char sk[NB * 512], sv[HD * 16], sc[2 * kSc];
+__global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
+  constexpr int TB = kv4_tile_bytes(HD);
+  __shared__ __align__(16) unsigned char tiles[kRowWarps][TB];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h0 = p.first / 32;
-  const int n_half = (p.first + p.n_tokens - 1) / 32 - h0 + 1;
-  const long long item = blockIdx.x;
+  const int t0 = p.first / kKv4Tile;
+  const int n_tiles = (p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1;
+  const long long items = (long long)n_tiles * p.pool.kv_heads * p.n_layers;
+  const long long item = (long long)blockIdx.x * kRowWarps + warp;
+  if (item >= items) return;
   const int kvh = (int)(item % p.pool.kv_heads);
   const long long r = item / p.pool.kv_heads;
-  const int half = h0 + (int)(r % n_half);
-  const int ll = (int)(r / n_half);
+  const int tile = t0 + (int)(r % n_tiles);
+  const int ll = (int)(r / n_tiles);
   const int layer = p.layer_begin + ll;
-  const int lo = max(p.first - half * 32, 0), hi = min(p.first + p.n_tokens - half * 32, 32);
-  using R = RowDims<HD>;
-
-  // this warp's tokens: all rows in flight before the first is used
-  float k[8][4], v[8][4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int t = 8 * warp + i;
-    if (t >= lo && t < hi) {
-      const long long row = (long long)ll * p.n_tokens + (half * 32 + t - p.first);
-      fetch_row<HD>(p.k, p.v, (size_t)(row * p.token_stride) + (size_t)kvh * HD, p.input_f16, lane, k[i], v[i]);
+  unsigned char* dst = tile_ptr(p.pool, p.page_row, layer, kvh, tile, TB);
+  unsigned char* sm = tiles[warp];
+  const int lo = max(p.first - tile * kKv4Tile, 0);
+  const int hi = min(p.first + p.n_tokens - tile * kKv4Tile, kKv4Tile);
+  if (lo > 0 || hi < kKv4Tile) {
+    for (int i = lane * 16; i < TB; i += 512) {
+      *reinterpret_cast<uint4*>(sm + i) = *reinterpret_cast<const uint4*>(dst + i);
     }
-  }
-  unsigned char* unit = unit_ptr(p.pool, p.page_row, layer, kvh, half / 2, UB);
-  // global pieces of this thread: (b, token) of the K codes, dim of the V codes, 16 bytes of scales
-  const int h32 = (half & 1) * 32;
-  unsigned char* gk = unit + ((int)(threadIdx.x >> 5) * 64 + h32 + (int)(threadIdx.x & 31)) * 16;
-  unsigned char* gv = unit + kv4_v_off(HD) + ((half & 1) * HD + (int)threadIdx.x) * 16;
-  const int si = (int)threadIdx.x * 16;  // of [K scales | V scales]
-  unsigned char* gs = unit + (si < kSc ? kv4_ks_off(HD) + kv4_scale(HD, h32, 0) + si
-                                       : kv4_vs_off(HD) + kv4_scale(HD, h32, 0) + si - kSc);
-  const bool has_k = threadIdx.x < NB * 32, has_v = threadIdx.x < HD, has_s = si < 2 * kSc;
-  if (lo > 0 || hi < 32) {
-    if (has_k) *reinterpret_cast<uint4*>(sk + threadIdx.x * 16) = *reinterpret_cast<const uint4*>(gk);
-    if (has_v) *reinterpret_cast<uint4*>(sv + threadIdx.x * 16) = *reinterpret_cast<const uint4*>(gv);
-    if (has_s) *reinterpret_cast<uint4*>(sc + si) = *reinterpret_cast<const uint4*>(gs);
-    __syncthreads();
+    __syncwarp();
   }
   const size_t brow = ((size_t)layer * p.pool.kv_heads + kvh) * HD;
   const float* kb = p.k_bias ? p.k_bias + brow : nullptr;
-  const float* vb = p.k_bias ? p.v_bias + brow : nullptr;
-  const int dim = R::dim(lane), b = dim >> 5;
-  uint32_t vw[4] = {0u, 0u, 0u, 0u}, mask = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int t = 8 * warp + i;
-    if (t < lo || t >= hi) continue;  // the same for the whole warp
-    const int tok = half * 32 + t - p.first;
+  const float* vb = p.v_bias ? p.v_bias + brow : nullptr;
+  using R = RowDims<HD>;
+#pragma unroll 4
+  for (int i = lo; i < hi; ++i) {
+    const int tok = tile * kKv4Tile + i - p.first;  // index among the new tokens
+    const long long row = (long long)ll * p.n_tokens + tok;
+    const size_t at = (size_t)(row * p.token_stride) + (size_t)kvh * HD;
     const float* cr = p.rope ? p.rope_cos + (size_t)(p.first_pos + tok) * (HD / 2) : nullptr;
     const float* sr = p.rope ? p.rope_sin + (size_t)(p.first_pos + tok) * (HD / 2) : nullptr;
-    prepare_row<HD>(kb, vb, cr, sr, lane, k[i], v[i]);
-    uint32_t kw, vc[4];
-    __half kd, vd;
-    quantise_row<HD>(lane, k[i], v[i], kw, kd, vc, vd);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) vw[j] |= vc[j] << (4 * kv4_nibble(i));
-    mask |= 15u << (4 * kv4_nibble(i));
-    if (R::has_k(lane) && (lane & 1) == 0) {
-      *reinterpret_cast<uint32_t*>(sk + (b * 32 + t) * 16 + ((dim & 31) >> 3) * 4) = kw;
-    }
-    if ((lane & 7) == 0) {
-      if (R::has_k(lane)) *reinterpret_cast<__half*>(sc + kv4_scale(HD, t, b)) = kd;
-      if (R::has_v(lane)) *reinterpret_cast<__half*>(sc + kSc + kv4_scale(HD, t, b)) = vd;
-    }
+    float k[4], v[4];
+    load_row<HD>(p.k, p.v, at, p.input_f16, kb, vb, cr, sr, lane, k, v);
+    store_row<HD>(sm, i, lane, k, v);
     if (p.k_rows) {
-      const size_t o = (((size_t)ll * p.n_tokens + tok) * p.pool.kv_heads + kvh) * HD + dim;
-      if (R::has_k(lane)) store4(p.k_rows, o, p.rows_f16, k[i]);
-      if (R::has_v(lane)) store4(p.v_rows, o, p.rows_f16, v[i]);
+      const size_t o = ((size_t)row * p.pool.kv_heads + kvh) * HD + R::dim(lane);
+      if (R::has_k(lane)) store4(p.k_rows, o, p.rows_f16, k);
+      if (R::has_v(lane)) store4(p.v_rows, o, p.rows_f16, v);
     }
   }
-  if (R::has_v(lane) && mask != 0u) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(sv + (dim + j) * 16 + warp * 4);
-      *w = mask == 0xffffffffu ? vw[j] : (*w & ~mask) | vw[j];
-    }
+  __syncwarp();
+  for (int i = lane * 16; i < TB; i += 512) {
+    *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(sm + i);
   }
-  __syncthreads();
-  if (has_k) *reinterpret_cast<uint4*>(gk) = *reinterpret_cast<const uint4*>(sk + threadIdx.x * 16);
-  if (has_v) *reinterpret_cast<uint4*>(gv) = *reinterpret_cast<const uint4*>(sv + threadIdx.x * 16);
-  if (has_s) *reinterpret_cast<uint4*>(gs) = *reinterpret_cast<const uint4*>(sc + si);
 }
 
 // ---- read ---------------------------------------------------------------------
 
-// One CTA per (layer, kv head, 32 tokens), a warp per 8 of them; a lane holds 4 dims, so that a token's row leaves
-// as one contiguous store.
+// One warp per (layer, kv head, tile): lane 4g + t expands its K words (dims
+// 8t.. of token g) and V words (dims 4g.. of tokens 2t, 2t + 1).
 template <int HD>
-__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4RowsParams p) {
-  constexpr int UB = kv4_unit_bytes(HD);
+__global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
+  constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h0 = p.first / 32;
-  const int n_half = (p.first + p.n_tokens - 1) / 32 - h0 + 1;
-  const long long item = blockIdx.x;
+  const int g = lane >> 2, t = lane & 3;
+  const int t0 = p.first / kKv4Tile;
+  const int n_tiles = (p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1;
+  const long long items = (long long)n_tiles * p.pool.kv_heads * p.n_layers;
+  const long long item = (long long)blockIdx.x * kRowWarps + warp;
+  if (item >= items) return;
   const int kvh = (int)(item % p.pool.kv_heads);
   const long long r = item / p.pool.kv_heads;
-  const int half = h0 + (int)(r % n_half);
-  const int ll = (int)(r / n_half);
-  const unsigned char* unit = unit_ptr(p.pool, p.page_row, p.layer_begin + ll, kvh, half / 2, UB);
-  using R = RowDims<HD>;
-  const int dim = R::dim(lane), b = dim >> 5;
-  const int r0 = (half & 1) * 32 + 8 * warp;  // this warp's first token in the unit
-  uint32_t vw[4];
-  if (R::has_v(lane)) {
+  const int tile = t0 + (int)(r % n_tiles);
+  const int ll = (int)(r / n_tiles);
+  const unsigned char* src = tile_ptr(p.pool, p.page_row, p.layer_begin + ll, kvh, tile, TB);
+  auto row_of = [&](int tok) -> long long {  // element offset of tile token tok's row, or -1 outside the range
+    const int i = tile * kKv4Tile + tok - p.first;
+    return i >= 0 && i < p.n_tokens ? (((long long)ll * p.n_tokens + i) * p.pool.kv_heads + kvh) * HD : -1;
+  };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      vw[j] = *reinterpret_cast<const uint32_t*>(unit + kv4_v_off(HD) + kv4_v_word(HD, dim + j, r0 >> 3));
-    }
-  }
+  for (int j = 0; j < 2; ++j) {
+    const long long kr = row_of(8 * j + g);
+    const long long v0 = row_of(8 * j + 2 * t), v1 = row_of(8 * j + 2 * t + 1);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int tok = half * 32 + 8 * warp + i - p.first;
-    if (tok < 0 || tok >= p.n_tokens) continue;
-    const size_t o = (((size_t)ll * p.n_tokens + tok) * p.pool.kv_heads + kvh) * HD + dim;
-    float x[4];
-    if (R::has_k(lane)) {
-      const uint32_t w =
-          *reinterpret_cast<const uint32_t*>(unit + kv4_k_word(r0 + i, b, (dim & 31) >> 3)) >> (8 * (lane & 1));
-      const float d = __half2float(*reinterpret_cast<const __half*>(unit + kv4_ks_off(HD) + kv4_scale(HD, r0 + i, b)));
-      x[0] = q4_value(w & 15u, d);
-      x[1] = q4_value((w >> 16) & 15u, d);
-      x[2] = q4_value((w >> 4) & 15u, d);
-      x[3] = q4_value((w >> 20) & 15u, d);
-      store4(p.k_rows, o, p.rows_f16, x);
-    }
-    if (R::has_v(lane)) {
-      const float d = __half2float(*reinterpret_cast<const __half*>(unit + kv4_vs_off(HD) + kv4_scale(HD, r0 + i, b)));
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(src + kv4_word_at(HD, j, lane, b));
+      const uint32_t vw = *reinterpret_cast<const uint32_t*>(src + CB + kv4_word_at(HD, j, lane, b));
+      const float kd = __half2float(
+          *reinterpret_cast<const __half*>(src + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1)));
+      const float2 vd = __half22float2(
+          *reinterpret_cast<const __half2*>(src + 2 * CB + SB + kv4_scale_at(HD, j, t, b, 0)));
+      if (kr >= 0) {
+        float x[4], y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = q4_value((vw[j] >> (4 * kv4_nibble(i))) & 15u, d);
-      store4(p.v_rows, o, p.rows_f16, x);
+        for (int q = 0; q < 2; ++q) {
+          x[2 * q] = q4_value((kw >> (4 * q)) & 15u, kd);
+          x[2 * q + 1] = q4_value((kw >> (4 * q + 16)) & 15u, kd);
+          y[2 * q] = q4_value((kw >> (4 * q + 8)) & 15u, kd);
+          y[2 * q + 1] = q4_value((kw >> (4 * q + 24)) & 15u, kd);
+        }
+        store4(p.k_rows, (size_t)kr + 32 * b + 8 * t, p.rows_f16, x);
+        store4(p.k_rows, (size_t)kr + 32 * b + 8 * t + 4, p.rows_f16, y);
+      }
+      float x[4], y[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        x[q] = q4_value((vw >> (4 * q)) & 15u, vd.x);
+        y[q] = q4_value((vw >> (4 * q + 16)) & 15u, vd.y);
+      }
+      if (v0 >= 0) store4(p.v_rows, (size_t)v0 + 32 * b + 4 * g, p.rows_f16, x);
+      if (v1 >= 0) store4(p.v_rows, (size_t)v1 + 32 * b + 4 * g, p.rows_f16, y);
     }
   }
 }
 
 // ---- raw Q4_0 blocks ------------------------------------------------------------
 
-// One thread per (layer, kv head, 8 tokens, block): both sides.  A raw block is 18 bytes, 2-byte aligned: the
-// scale, then byte i = code i | code (i + 16) << 4.
+// One thread per (layer, token, kv head, block): both sides.  A raw block is
+// 18 bytes, 2-byte aligned: the scale, then byte i = code i | code (i + 16) << 4.
 template <int HD>
 __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int to_pool) {
-  constexpr int UB = kv4_unit_bytes(HD), NB = HD / 32;
-  const int g0 = p.first / 8;
-  const int n_groups = (p.first + p.n_tokens - 1) / 8 - g0 + 1;
-  const long long n = (long long)p.n_layers * n_groups * p.pool.kv_heads * NB;
-  const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (id >= n) return;
-  const int b = (int)(id % NB);
-  long long r = id / NB;
+  constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
+  const long long n = (long long)p.n_layers * p.n_tokens * p.pool.kv_heads * NB;
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int b = (int)(i % NB);
+  long long r = i / NB;
   const int kvh = (int)(r % p.pool.kv_heads);
   r /= p.pool.kv_heads;
-  const int group = g0 + (int)(r % n_groups);
-  const int ll = (int)(r / n_groups);
-  unsigned char* unit = unit_ptr(p.pool, p.page_row, p.layer_begin + ll, kvh, group / 8, UB);
-  const int y = group % 8;
-  const int lo = max(p.first - group * 8, 0), hi = min(p.first + p.n_tokens - group * 8, 8);
-  auto raw_at = [&](int i) {  // raw block of the group's token i, in 2-byte units
-    const long long tok = (long long)ll * p.n_tokens + (group * 8 + i - p.first);
-    return ((tok * p.pool.kv_heads + kvh) * NB + b) * 9;
+  const int tok = p.first + (int)(r % p.n_tokens);
+  const int layer = p.layer_begin + (int)(r / p.n_tokens);
+  unsigned char* tile = tile_ptr(p.pool, p.page_row, layer, kvh, tok / kKv4Tile, TB);
+  const int s = tok % kKv4Tile, j = s >> 3, g = s & 7, tp = g >> 1, e = s & 1;
+  // code index of the block -> its word (byte offset) and nibble shift
+  auto k_word = [&](int t) { return reinterpret_cast<uint32_t*>(tile + kv4_word_at(HD, j, 4 * g + t, b)); };
+  auto v_half = [&](int gg) {
+    return reinterpret_cast<uint16_t*>(tile + CB + kv4_word_at(HD, j, 4 * gg + tp, b) + 2 * e);
   };
-  auto v_word = [&](int c) {
-    return reinterpret_cast<uint32_t*>(unit + kv4_v_off(HD) + kv4_v_word(HD, 32 * b + c, y));
-  };
-  uint32_t vw[32];
+  uint16_t* kd = reinterpret_cast<uint16_t*>(tile + 2 * CB + kv4_scale_at(HD, j, tp, b, e));
+  uint16_t* vd = reinterpret_cast<uint16_t*>(tile + 2 * CB + SB + kv4_scale_at(HD, j, tp, b, e));
   if (to_pool) {
-    uint32_t mask = 0u;
+    const uint16_t* kr = reinterpret_cast<const uint16_t*>(p.k) + i * 9;
+    const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.v) + i * 9;
+    uint32_t kc[32], vc[32];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) vw[c] = 0u;
-    for (int i = lo; i < hi; ++i) {
-      const uint16_t* kr = reinterpret_cast<const uint16_t*>(p.k) + raw_at(i);
-      const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.v) + raw_at(i);
-      const int tok = 8 * y + i, sh = 4 * kv4_nibble(i);
-      uint32_t kc[32];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t kx = kr[1 + q], vx = vr[1 + q];
-        kc[2 * q] = kx & 15u;
-        kc[2 * q + 1] = (kx >> 8) & 15u;
-        kc[2 * q + 16] = (kx >> 4) & 15u;
-        kc[2 * q + 17] = kx >> 12;
-        vw[2 * q] |= (vx & 15u) << sh;
-        vw[2 * q + 1] |= ((vx >> 8) & 15u) << sh;
-        vw[2 * q + 16] |= ((vx >> 4) & 15u) << sh;
-        vw[2 * q + 17] |= (vx >> 12) << sh;
-      }
-      mask |= 15u << sh;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t a[4] = {kc[8 * t], kc[8 * t + 1], kc[8 * t + 2], kc[8 * t + 3]};
-        const uint32_t c[4] = {kc[8 * t + 4], kc[8 * t + 5], kc[8 * t + 6], kc[8 * t + 7]};
-        *reinterpret_cast<uint32_t*>(unit + kv4_k_word(tok, b, t)) = k_bits(a, 0) | k_bits(c, 1);
-      }
-      *reinterpret_cast<uint16_t*>(unit + kv4_ks_off(HD) + kv4_scale(HD, tok, b)) = kr[0];
-      *reinterpret_cast<uint16_t*>(unit + kv4_vs_off(HD) + kv4_scale(HD, tok, b)) = vr[0];
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t kx = kr[1 + q], vx = vr[1 + q];
+      kc[2 * q] = kx & 15u; kc[2 * q + 1] = (kx >> 8) & 15u;
+      kc[2 * q + 16] = (kx >> 4) & 15u; kc[2 * q + 17] = kx >> 12;
+      vc[2 * q] = vx & 15u; vc[2 * q + 1] = (vx >> 8) & 15u;
+      vc[2 * q + 16] = (vx >> 4) & 15u; vc[2 * q + 17] = vx >> 12;
     }
 #pragma unroll
-    for (int c = 0; c < 32; ++c) *v_word(c) = mask == 0xffffffffu ? vw[c] : (*v_word(c) & ~mask) | vw[c];
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t a[4] = {kc[8 * t], kc[8 * t + 1], kc[8 * t + 2], kc[8 * t + 3]};
+      const uint32_t c[4] = {kc[8 * t + 4], kc[8 * t + 5], kc[8 * t + 6], kc[8 * t + 7]};
+      *k_word(t) = k_bits(a, 0) | k_bits(c, 1);
+    }
+#pragma unroll
+    for (int gg = 0; gg < 8; ++gg) {
+      const uint32_t a[4] = {vc[4 * gg], vc[4 * gg + 1], vc[4 * gg + 2], vc[4 * gg + 3]};
+      *v_half(gg) = (uint16_t)v_bits(a);
+    }
+    *kd = kr[0];
+    *vd = vr[0];
   } else {
+    uint16_t* kr = reinterpret_cast<uint16_t*>(p.k_rows) + i * 9;
+    uint16_t* vr = reinterpret_cast<uint16_t*>(p.v_rows) + i * 9;
+    uint32_t kc[32], vc[32];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) vw[c] = *v_word(c);
-    for (int i = lo; i < hi; ++i) {
-      uint16_t* kr = reinterpret_cast<uint16_t*>(p.k_rows) + raw_at(i);
-      uint16_t* vr = reinterpret_cast<uint16_t*>(p.v_rows) + raw_at(i);
-      const int tok = 8 * y + i, sh = 4 * kv4_nibble(i);
-      uint32_t kc[32];
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t w = *k_word(t);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(unit + kv4_k_word(tok, b, t));
-#pragma unroll
-        for (int c = 0; c < 8; ++c) kc[8 * t + c] = (w >> (4 * kv4_nibble(c))) & 15u;
+      for (int q = 0; q < 4; ++q) {
+        kc[8 * t + 2 * q] = (w >> (4 * q)) & 15u;
+        kc[8 * t + 2 * q + 1] = (w >> (4 * q + 16)) & 15u;
       }
-      kr[0] = *reinterpret_cast<const uint16_t*>(unit + kv4_ks_off(HD) + kv4_scale(HD, tok, b));
-      vr[0] = *reinterpret_cast<const uint16_t*>(unit + kv4_vs_off(HD) + kv4_scale(HD, tok, b));
+    }
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        kr[1 + q] = (uint16_t)(kc[2 * q] | kc[2 * q + 16] << 4 | kc[2 * q + 1] << 8 | kc[2 * q + 17] << 12);
-        vr[1 + q] = (uint16_t)(((vw[2 * q] >> sh) & 15u) | ((vw[2 * q + 16] >> sh) & 15u) << 4 |
-                               ((vw[2 * q + 1] >> sh) & 15u) << 8 | ((vw[2 * q + 17] >> sh) & 15u) << 12);
-      }
+    for (int gg = 0; gg < 8; ++gg) {
+      const uint32_t w = *v_half(gg);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vc[4 * gg + q] = (w >> (4 * q)) & 15u;
+    }
+    kr[0] = *kd;
+    vr[0] = *vd;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      kr[1 + q] = (uint16_t)(kc[2 * q] | kc[2 * q + 16] << 4 | kc[2 * q + 1] << 8 | kc[2 * q + 17] << 12);
+      vr[1 + q] = (uint16_t)(vc[2 * q] | vc[2 * q + 16] << 4 | vc[2 * q + 1] << 8 | vc[2 * q + 17] << 12);
     }
   }
 }
 
 // ---- decode attention -------------------------------------------------------------
 //
-// out = softmax(q K^T / sqrt(hd)) V per query head, over a group's cached tokens and the token the call appends.
-// A CTA of 128 threads takes 128 tokens a step (two units), one token a thread, and up to 8 query heads:
+// out = softmax(q K^T / sqrt(hd)) V per query head, over a group's cached
+// tokens and the token the call appends.  Both products run on mma.sync
+// m16n8k16 with fp32 accumulators, fed with the codes themselves:
 //
-//   S = K q^T: A = the K codes minus 8, widened to f16 and put into TMEM by the thread whose token they are;
-//      B = the queries in shared memory, f16 hi and lo parts of 8 heads (N = 16), scaled by a power of two per head;
-//      one product per block of 32 dims, so that the thread multiplies by its token's scales on the way out:
-//      score = sum_b d_b (hi + lo), fp32.
-//   O^T = V^T P: A = the V codes minus 8 (M = dims, the same TMEM columns); B = the weights in shared memory:
-//      P d for each block of dims, f16 hi + lo parts by an error-free product (hi = f16(P d), lo = f16 of the
-//      rest, about 22 bits), N = blocks * 16.  The rows of block b need its 16 columns only; the rest of the
-//      product is computed and not read -- the tensor pipe is far from its limit (at head_dim 64 the rows are
-//      the dims of the step's two units, each with columns of its own).
+//   S: A = the group's queries as f16 hi (rows 0-7) and lo (rows 8-15) parts,
+//      scaled by a power of two per head; B = K codes minus 8.
+//      Per block of 32 dims S += d (A B) in fp32.
+//   O^T: A = V codes minus 8, rows = dims; B = P d as f16 hi + lo parts (an
+//      error-free product: hi = f16(P d), lo = f16 of the rest), so the
+//      weights keep about 22 bits.
 //
-// Each product starts from zero and is added to fp32 registers: a long accumulation inside the tensor core
-// truncates at every step.  The online softmax keeps a reference exponent per head for the whole CTA and moves it
-// only when a score exceeds it by more than 2^3.
+// The C fragment of S holds, in lane 4g + t, head g and tokens 2t, 2t + 1:
+// exactly what the B fragment of O^T wants, so the weights never leave their
+// registers.  The online softmax keeps a reference exponent per head and
+// moves it (rescaling O) only when a score exceeds it by more than 2^5.
 template <int HD>
 struct Dec {
-  static constexpr int kThreads = 128, kCtas = KV4_CTAS, kRing = 2;
+  static constexpr int kWarps = 8;
+  static constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
   static constexpr int NB = HD / 32;
-  static constexpr int UB = kv4_unit_bytes(HD);
-  static constexpr int kStageBytes = 2 * UB;
-  static constexpr int kPRows = HD == 128 ? 128 : 64;  // K extent of the second product
-  static constexpr int kColA = 0, kColD = 64;          // TMEM columns: the A operand, the products
-  static constexpr int p_off = 0;                      // weights: rows of 128 bytes, 128B swizzle
-  static constexpr int q_off = kPRows * 128;           // queries: (HD / 64) chunks of 16 rows of 128 bytes, 128B swizzle
-  static constexpr int ring_off = q_off + (HD / 64) * 2048;
-  static constexpr int f_off = ring_off + kRing * kStageBytes;  // per head: S f = score in exp2 units
-  static constexpr int mb_off = f_off + 32;                     // per head: kWeightExp - reference exponent
-  static constexpr int red_off = mb_off + 32;                   // [4 warps][9]
-  static constexpr int flag_off = red_off + 160;                // fold flags [2], abort, TMEM address
-  static constexpr int bar_off = flag_off + 16;                 // full[kRing], product 1, product 2
-  static constexpr int pend_off = bar_off + (kRing + 2) * 8;    // two Seg
-  static constexpr int smem = pend_off + 2 * 64;
+  static constexpr int kRing = HD == 128 ? 5 : 10;  // tiles in flight per warp
+  static constexpr int kItems = NB * 2 * 32;        // float4 items of a warp's O
+  static constexpr int ring_off = 0;
+  static constexpr int new_off = kWarps * kRing * TB;
+  static constexpr int red_off = new_off + TB;
+  static constexpr int stat_off = red_off + (kWarps / 2) * kItems * 16;
+  static constexpr int bar_off = stat_off + 2 * kWarps * kKv4Heads * 4 + 16;
+  static constexpr int smem = bar_off + kWarps * kRing * 8;
 };
-static_assert((Dec<128>::smem + 1024) * Dec<128>::kCtas <= 228 * 1024 && Dec<128>::kCtas * 128 <= 512, "CTAs per SM");
-
-constexpr float kSlack = 3.f;       // scores may exceed the reference by this before it moves
-constexpr float kWeightExp = 11.f;  // weights are 2^(score - m + 11): at most 2^14, products with a scale at most 2^15
+static_assert(Dec<128>::smem <= 115712 && Dec<64>::smem <= 115712, "two CTAs per SM");
 
 struct Seg {
-  int ll, kvh, hb, si;  // local layer, kv head, head block, sequence
-  int s0, s1, n;        // stages of the segment, stages of its group
-  int next;             // the CTA's next stage (global index), its end when there is none
-  int parts, c0;        // CTAs that share the group, the first of them
-  int gb;               // stream split: the group's first stage (global index)
-  int group_id;
+  long long next;      // first unit after the segment
+  int ll, kvh, hb, si;
+  int t0, t1;          // tiles of the sequence in this segment
+  int part, parts;     // this segment's part of its group (parts == 1: all of it)
+  long long c0;        // CTA of the group's first part
+  bool last;           // holds the group's last unit (and so the appended token)
+  long long group_id;
 };
 
-static_assert(sizeof(Seg) <= 64, "pending segments");
-
-// Stream split: the CTA whose range [b T / G, (b + 1) T / G) holds stage u.
-__device__ __forceinline__ int kv4_cta_of(int u, long long total, int grid) {
-  return (int)div_nonneg((long long)(u + 1) * grid - 1, total);
+// The CTA whose range [b T / G, (b + 1) T / G) holds unit u.
+__device__ __forceinline__ long long kv4_cta_of(long long u, long long total, long long grid) {
+  return div_nonneg((u + 1) * grid - 1, total);
 }
 
-// The segment of this CTA that begins at u (stream split), or its only one (aligned split).
-__device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u1) {
+__device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, long long u, long long u1) {
   Seg s;
-  const bool aligned = p.block_parts != 0;
-  const int per = aligned ? p.block_parts : p.block_stages;
-  const int at = aligned ? (int)blockIdx.x : u;
-  const uint32_t blk = (uint32_t)at / (uint32_t)per;
-  const int rem = at - (int)blk * per;
+  const long long blk = div_nonneg(u, p.block_units);
+  const int rem = (int)(u - blk * p.block_units);
   int lo = 0, hi = p.n_seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    const int begin = aligned ? p.seqs[mid].part_begin : p.seqs[mid].stage_begin;
-    if (begin <= rem) lo = mid; else hi = mid - 1;
+    if (p.seqs[mid].unit_begin <= rem) lo = mid; else hi = mid - 1;
   }
   s.si = lo;
-  s.n = kv4_stages(p.seqs[lo].len + (p.k_new ? 1 : 0));
-  if (aligned) {
-    const int part = rem - p.seqs[lo].part_begin;
-    s.parts = (lo + 1 < p.n_seqs ? p.seqs[lo + 1].part_begin : per) - p.seqs[lo].part_begin;
-    s.c0 = (int)blockIdx.x - part;
-    s.s0 = (int)div_nonneg((long long)part * s.n, s.parts);
-    s.s1 = (int)div_nonneg((long long)(part + 1) * s.n, s.parts);
-    s.gb = 0;
-    s.next = u1;
-  } else {
-    s.gb = (int)blk * per + p.seqs[lo].stage_begin;
-    s.next = min(s.gb + s.n, u1);
-    s.s0 = u - s.gb;
-    s.s1 = s.next - s.gb;
-    s.c0 = kv4_cta_of(s.gb, p.total_stages, p.grid);
-    s.parts = kv4_cta_of(s.gb + s.n - 1, p.total_stages, p.grid) - s.c0 + 1;
-  }
-  if (p.seqs[lo].len == 0 && !p.k_new) s.s1 = s.s0;  // nothing to attend: zeros
-  const uint32_t lk = blk / (uint32_t)p.head_blocks;
-  s.hb = (int)(blk - lk * (uint32_t)p.head_blocks);
+  const int len = p.seqs[lo].len;
+  const long long gb = blk * p.block_units + p.seqs[lo].unit_begin;
+  const long long ge = gb + kv4_units(len);
+  s.next = ge < u1 ? ge : u1;
+  s.t0 = (int)(u - gb) * kKv4UnitTiles;
+  s.t1 = min((int)(s.next - gb) * kKv4UnitTiles, (len + kKv4Tile - 1) / kKv4Tile);
+  s.last = s.next == ge;
+  const uint32_t lk = (uint32_t)blk / (uint32_t)p.head_blocks;
+  s.hb = (int)((uint32_t)blk - lk * (uint32_t)p.head_blocks);
   s.ll = (int)(lk / (uint32_t)p.pool.kv_heads);
   s.kvh = (int)lk - s.ll * p.pool.kv_heads;
-  s.group_id = (int)blk * p.n_seqs + lo;
+  s.c0 = kv4_cta_of(gb, p.total_units, p.grid);
+  s.parts = (int)(kv4_cta_of(ge - 1, p.total_units, p.grid) - s.c0) + 1;
+  s.part = (int)(blockIdx.x - s.c0);
+  s.group_id = blk * p.n_seqs + lo;
   return s;
 }
 
@@ -514,6 +473,18 @@ __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+// The four f16 pairs of a word: c - 8, and 16 (c - 8) for the upper nibbles, exactly: a code under the exponent
+// of 1024 is 1024 + c (or + 16 c), and one subtraction leaves a normal number.  Codes read as f16 subnormals
+// would need no subtraction for the keys, but the tensor core aligns the 16 products of a step by their
+// operands' nominal exponents: subnormals lose 7 to 10 bits of the fp32 sum (measured: the output was 8e-6
+// off, against 1e-6 now).
+__device__ __forceinline__ void centred(uint32_t x, uint32_t (&c)[4]) {
+  const uint32_t y = x >> 8;
+  c[0] = h2_add((x & 0x000f000fu) | 0x64006400u, 0xe408e408u);
+  c[1] = h2_add((x & 0x00f000f0u) | 0x64006400u, 0xe480e480u);
+  c[2] = h2_add((y & 0x000f000fu) | 0x64006400u, 0xe408e408u);
+  c[3] = h2_add((y & 0x00f000f0u) | 0x64006400u, 0xe480e480u);
 }
 __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -523,12 +494,6 @@ __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// a b - c in f16x2, one rounding.
-__device__ __forceinline__ uint32_t h2_fms(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
 __device__ __forceinline__ uint32_t h2_maxabs(uint32_t a, uint32_t b) {
@@ -541,678 +506,500 @@ __device__ __forceinline__ uint32_t h2_maxabs(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float pow2i(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
 
-// (x & m) | o as one operation: o comes in a register, since an instruction holds one immediate.
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(m), "r"(o));
-  return d;
-}
-__device__ __forceinline__ uint32_t code_magic() {  // opaque to the compiler, so that it stays in a register
-  uint32_t m;
-  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m));
-  return m;
-}
-// The four f16 pairs of a word: c - 8, and 16 (c - 8) for the odd pairs, exactly: a code under the exponent of
-// 1024 is 1024 + c (or + 16 c), and one subtraction leaves a normal number.  Codes read as f16 subnormals would
-// need no subtraction, but the tensor core aligns the products of a step by their operands' nominal exponents:
-// subnormals lose 7 to 10 bits of the fp32 sum (measured: the output was 8e-6 off, against 1e-6).
-__device__ __forceinline__ void centred(uint32_t x, uint32_t magic, uint32_t* c) {
-  const uint32_t y = x >> 8;
-  c[0] = h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u);
-  c[1] = h2_add(and_or(x, 0x00f000f0u, magic), 0xe480e480u);
-  c[2] = h2_add(and_or(y, 0x000f000fu, magic), 0xe408e408u);
-  c[3] = h2_add(and_or(y, 0x00f000f0u, magic), 0xe480e480u);
-}
-// The 16 f16 pairs of a 16-byte chunk.
-__device__ __forceinline__ void centred_chunk(uint32_t addr, uint32_t magic, uint32_t* c) {
-  const uint4 x = lds128(addr);
-  centred(x.x, magic, c);
-  centred(x.y, magic, c + 4);
-  centred(x.z, magic, c + 8);
-  centred(x.w, magic, c + 12);
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
-        "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-      : "r"(taddr));
-}
-// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16, one CTA.
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// A query head's raw row, 4 dims a lane (lanes 0-15 at head_dim 64); zeros for a head the group has not.
 template <int HD>
-__device__ __forceinline__ void fetch_query(const Kv4DecodeParams& p, const Seg& s, int h, int lane, float (&v)[4]) {
-  const int hg = s.hb * p.block_heads + h;
-  v[0] = v[1] = v[2] = v[3] = 0.f;
-  if (h < p.block_heads && hg < p.group && lane < HD / 4) {
-    const size_t row = ((size_t)s.ll * p.seq_total + p.seq_base + s.si) * (p.pool.kv_heads * p.group) +
-                       s.kvh * p.group + hg;
-    load4(p.q, row * HD + 4 * lane, p.input_f16, v);
-  }
-}
+struct WarpState {
+  static constexpr int NB = HD / 32;
+  uint32_t qa[NB][2][4];  // A fragments of the queries: block, k16 step
+  float f;                // S f = score in exp2 units
+  float o[NB][2][4];      // O^T accumulators: block, m16 tile
+  float m, l;             // reference exponent and sum of this lane's weights, head g
+  float mb;               // 8 - m
+  float vlim;             // largest |V scale| the current vexp allows
+  uint32_t vmul;          // 2^vexp twice, f16
+  int vexp;
+};
 
-// Bias, RoPE, the head's power of two (largest value in [2^11, 2^12)) and the f16 hi / lo split: writes rows h and
-// 8 + h of the B operand (dims of odd pairs divided by 16: their codes come as 16 c) and the factor that turns S
-// into exp2 units.
+constexpr float kSlack = 5.f;      // scores may exceed the reference by this before it moves
+constexpr float kWeightExp = 8.f;  // weights are 2^(score - m + 8): at most 2^13, exact products far above f16's floor
+
+// Queries of the segment's heads as A fragments, scaled per head by a power of two (largest value in [2^11, 2^12)).
 template <int HD>
-__device__ __forceinline__ void stage_query(const Kv4DecodeParams& p, const Seg& s, int h, int lane, float (&v)[4],
-                                            unsigned char* qs, float* f) {
-  const int hg = s.hb * p.block_heads + h;
-  const bool have = h < p.block_heads && hg < p.group;
-  if (have && p.q_bias && lane < HD / 4) {
-    add_bias4(v, p.q_bias + ((size_t)(p.layer_begin + s.ll) * (p.pool.kv_heads * p.group) + s.kvh * p.group + hg) * HD +
-                     4 * lane);
-  }
-  if (p.rope) {
-    rope4<HD>(v, p.rope_cos + (size_t)p.seqs[s.si].q_pos * (HD / 2), p.rope_sin + (size_t)p.seqs[s.si].q_pos * (HD / 2),
-              lane);
-  }
-  float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+__device__ __forceinline__ void load_queries(const Kv4DecodeParams& p, const Seg& s, int lane, WarpState<HD>& w) {
+  constexpr int NB = HD / 32;
+  const int g = lane >> 2, t = lane & 3;
+  const int heads = p.pool.kv_heads * p.group;
+  const int hg = s.hb * p.block_heads + g;  // head within the kv head's group
+  const bool have = g < p.block_heads && hg < p.group;
+  float v[NB][8];
+  if (have) {
+    const int head = s.kvh * p.group + hg;
+    const size_t row = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * heads + head) * HD;
 #pragma unroll
-  for (int off = 1; off < HD / 4; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    for (int b = 0; b < NB; ++b) load8(p.q, row + 32 * b + 8 * t, p.input_f16, v[b]);
+    if (p.q_bias) {
+      const float* br = p.q_bias + ((size_t)(p.layer_begin + s.ll) * heads + head) * HD;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) add_bias8(v[b], br + 32 * b + 8 * t);
+    }
+    if (p.rope) {
+      const float* cr = p.rope_cos + (size_t)p.seqs[s.si].q_pos * (HD / 2);
+      const float* sr = p.rope_sin + (size_t)p.seqs[s.si].q_pos * (HD / 2);
+#pragma unroll
+      for (int b = 0; b < NB / 2; ++b) rope8(v[b], v[b + NB / 2], cr, sr, 32 * b + 8 * t);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[b][i]));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const int k = top > 0.f ? min(max(11 - exponent_of(top), -100), 126) : 0;
   const float sc = pow2i(k);
-  if (lane == 0) f[h] = p.scale_log2 * pow2i(-k);
-  uint32_t hi[2], lo[2];
+  w.f = p.scale_log2 * pow2i(-k);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float mul = r ? 0.0625f : 1.f;
-    const float x = v[2 * r] * sc * mul, y = v[2 * r + 1] * sc * mul;
-    const __half2 a = __floats2half2_rn(x, y);
-    const float2 af = __half22float2(a);
-    hi[r] = *reinterpret_cast<const uint32_t*>(&a);
-    lo[r] = pack_half2(x - af.x, y - af.y);
-  }
-  if (lane < HD / 4) {
-    const int d = 4 * lane;
-    unsigned char* at = qs + (d >> 6) * 2048 + h * 128 + ((((d & 63) >> 3) ^ h) * 16) + (d & 7) * 2;
-    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-    *reinterpret_cast<uint2*>(at + 1024) = make_uint2(lo[0], lo[1]);
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        // the nibbles of the second pair of a step read 16 c: its queries enter divided by 16
+        const float mul = r ? 0.0625f : 1.f;
+        const float x = v[b][4 * st + 2 * r] * sc * mul, y = v[b][4 * st + 2 * r + 1] * sc * mul;
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 hf = __half22float2(h);
+        const __half2 q = __floats2half2_rn(x - hf.x, y - hf.y);
+        hi[r] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[r] = *reinterpret_cast<const uint32_t*>(&q);
+      }
+      w.qa[b][st][0] = hi[0];
+      w.qa[b][st][1] = lo[0];
+      w.qa[b][st][2] = hi[1];
+      w.qa[b][st][3] = lo[1];
+    }
   }
 }
 
-// The copies of a CTA: the stages of its segments in order, across segments (kept by thread 0).
+template <int HD>
+__device__ __forceinline__ void reset_state(WarpState<HD>& w) {
+#pragma unroll
+  for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w.o[b][i][r] = 0.f;
+  w.m = -INFINITY;
+  w.mb = INFINITY;
+  w.l = 0.f;
+  w.vlim = 0.f;
+  w.vmul = 0;
+  w.vexp = 0;
+}
+
+// Words of a lane: NB per n8 half / token-pair half j.
+template <int HD>
+__device__ __forceinline__ void lds_words(uint32_t addr, int lane, uint32_t (&w)[2][HD / 32]) {
+  if constexpr (HD == 128) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 v = lds128(addr + j * 512 + lane * 16);
+      w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+    }
+  } else {
+    const uint4 v = lds128(addr + lane * 16);
+    w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+  }
+}
+template <int HD>
+__device__ __forceinline__ void lds_scales(uint32_t addr, int t, uint32_t (&w)[2][HD / 32]) {
+  if constexpr (HD == 128) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 v = lds128(addr + j * 64 + t * 16);
+      w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+    }
+  } else {
+    const uint4 v = lds128(addr + t * 16);
+    w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+  }
+}
+
+// Attends the first `valid` (1..16) tokens of the tile at shared address `addr`.
+template <int HD>
+__device__ __forceinline__ void attend_tile(uint32_t addr, int valid, int lane, WarpState<HD>& w) {
+  using D = Dec<HD>;
+  constexpr int NB = D::NB;
+  const int t = lane & 3;
+  uint32_t kw[2][NB], ks[2][NB], vs[2][NB];
+  lds_words<HD>(addr, lane, kw);
+  lds_scales<HD>(addr + 2 * D::CB, t, ks);
+  lds_scales<HD>(addr + 2 * D::CB + D::SB, t, vs);
+
+  // scores: s[j] = tokens 8j + 2t, 8j + 2t + 1 of head g
+  uint64_t s2[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    s2[j] = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t c[4];
+      centred(kw[j][b], c);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816(acc, w.qa[b][0], c[0], c[1]);
+      mma_16816(acc, w.qa[b][1], c[2], c[3]);
+      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ks[j][b]));
+      const uint64_t d2 = f2_pack(d.x, d.y);
+      s2[j] = f2_fma(d2, f2_pack(acc[0], acc[1]), s2[j]);
+      s2[j] = f2_fma(d2, f2_pack(acc[2], acc[3]), s2[j]);
+    }
+  }
+  float s[4];
+  f2_unpack(s2[0], s[0], s[1]);
+  f2_unpack(s2[1], s[2], s[3]);
+  if (valid < kKv4Tile) {  // tokens past the sequence: no weight, whatever the tile holds there
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = 8 * (i >> 1) + 2 * t + (i & 1) < valid;
+      if (!in) {
+        s[i] = -INFINITY;
+        const uint32_t keep = (i & 1) ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vs[i >> 1][b] &= keep;
+      }
+    }
+  }
+  const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * w.f;
+  uint32_t vm = h2_maxabs(vs[0][0], vs[1][0]);
+#pragma unroll
+  for (int b = 1; b < NB; ++b) vm = h2_maxabs(vm, h2_maxabs(vs[0][b], vs[1][b]));
+  const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
+  const float vtop = fmaxf(vmf.x, vmf.y);
+  if (__any_sync(0xffffffffu, top > w.m + kSlack || vtop > w.vlim)) {
+    float tm = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
+    float alpha = 1.f;
+    if (tm > w.m + kSlack) {
+      alpha = ex2(w.m - tm);
+      w.m = tm;
+      w.mb = kWeightExp - tm;
+    }
+    float vx = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+    vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, 2));
+    float beta = 1.f;
+    if (vx > w.vlim) {
+      const int e = min(exponent_of(vx), 15);
+      const int k = min(max(-1 - e, -16), 15);  // |V scale| 2^k in [0.5, 1) now, at most 4 until it moves again
+      beta = w.vlim > 0.f ? pow2i(k - w.vexp) : 1.f;
+      w.vexp = k;
+      w.vlim = pow2i(e + 3);
+      const __half2 h = __float2half2_rn(pow2i(k));
+      w.vmul = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    w.l *= alpha;
+    const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t) * beta;
+    const float a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4) * beta;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w.o[b][i][0] *= a0;
+        w.o[b][i][1] *= a1;
+        w.o[b][i][2] *= a0;
+        w.o[b][i][3] *= a1;
+      }
+  }
+  float pr[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pr[i] = ex2(fmaf(s[i], w.f, w.mb));
+  w.l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+  uint32_t ph[2], pl[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __half2 h = __floats2half2_rn(pr[2 * j], pr[2 * j + 1]);
+    const float2 hf = __half22float2(h);
+    ph[j] = *reinterpret_cast<const uint32_t*>(&h);
+    pl[j] = pack_half2(pr[2 * j] - hf.x, pr[2 * j + 1] - hf.y);
+  }
+
+  uint32_t vw[2][NB];
+  lds_words<HD>(addr + D::CB, lane, vw);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t d = h2_mul(vs[j][b], w.vmul);
+      hi[j] = h2_mul(ph[j], d);
+      lo[j] = h2_fma(pl[j], d, h2_fma(ph[j], d, hi[j] ^ 0x80008000u));
+    }
+    uint32_t c0[4], c1[4];
+    centred(vw[0][b], c0);
+    centred(vw[1][b], c1);
+    const uint32_t a[4] = {c0[0], c0[1], c1[0], c1[1]}, c[4] = {c0[2], c0[3], c1[2], c1[3]};
+    mma_16816(w.o[b][0], a, hi[0], hi[1]);
+    mma_16816(w.o[b][1], c, hi[0], hi[1]);
+    mma_16816(w.o[b][0], a, lo[0], lo[1]);
+    mma_16816(w.o[b][1], c, lo[0], lo[1]);
+  }
+}
+
+// A warp's copies: tiles t0 + warp, + 8, ... of each segment of the CTA's range, in order, across segments.
 struct Feed {
-  int u, u1;                  // next segment's first stage, end of the CTA's range
-  int stage, s1;              // next stage and end of the current segment
-  int units;                  // units of the sequence that hold attended tokens
-  const unsigned char* base;  // page 0 of the segment's layer, at its kv head
+  long long u, u1;      // next segment's first unit, end of the CTA's range
+  int tile, t1;         // next tile and end of the current segment
+  const unsigned char* base;  // tile 0 of page 0 for the segment's layer and kv head
   const int32_t* row;
   int page_base;
 };
 
 template <int HD>
-__device__ __forceinline__ void feed_issue(const Kv4DecodeParams& p, Feed& f, unsigned char* dst, uint64_t* bar) {
-  using D = Dec<HD>;
-  while (f.stage >= f.s1) {
-    if (f.u >= f.u1) return;
+__device__ __forceinline__ const unsigned char* feed_next(const Kv4DecodeParams& p, Feed& f, int warp) {
+  while (f.tile >= f.t1) {
+    if (f.u >= f.u1) return nullptr;
     const Seg s = kv4_seg_at(p, f.u, f.u1);
     f.u = s.next;
-    f.stage = s.s0;
-    f.s1 = s.s1;
-    f.units = (p.seqs[s.si].len + (p.k_new ? 1 : 0) + kKv4Unit - 1) / kKv4Unit;
+    f.tile = s.t0 + warp;
+    f.t1 = s.t1;
     const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
-    f.base = p.pool.base + rec * p.pool.units_per_page * D::UB;
+    f.base = p.pool.base + rec * p.pool.tiles_per_page * Dec<HD>::TB;
     f.row = p.page_table + (size_t)p.seqs[s.si].slot * p.max_pages_per_seq;
     f.page_base = p.seqs[s.si].page_base;
   }
-  const int u0 = 2 * f.stage;
-  const int n = min(2, f.units - u0);
-  mbar_arrive_expect_tx(bar, n * D::UB);
-  for (int i = 0; i < n; ++i) {
-    const int page = kv4_page_of(p.pool, u0 + i);
-    const int in = u0 + i - page * p.pool.units_per_page;
-    const int id = f.page_base >= 0 ? f.page_base + page : f.row[page];
-    bulk_load(dst + i * D::UB,
-              f.base + ((long long)id * p.pool.kv_heads * p.pool.units_per_page + in) * D::UB, D::UB, bar);
-  }
-  ++f.stage;
-}
-
-// Quantises the appended token (warp 0): into its slot of the stage in shared memory, so that the step attends it
-// as stored, and (first head block) into the cache.
-template <int HD>
-__device__ __forceinline__ void place_new_token(const Kv4DecodeParams& p, const Seg& s, unsigned char* stage, int lane) {
-  using R = RowDims<HD>;
-  constexpr int UB = kv4_unit_bytes(HD);
-  const Kv4Seq& sq = p.seqs[s.si];
-  const size_t at = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * p.pool.kv_heads + s.kvh) * HD;
-  const size_t brow = ((size_t)(p.layer_begin + s.ll) * p.pool.kv_heads + s.kvh) * HD;
-  float k[4], v[4];
-  fetch_row<HD>(p.k_new, p.v_new, at, p.input_f16, lane, k, v);
-  prepare_row<HD>(p.k_bias ? p.k_bias + brow : nullptr, p.k_bias ? p.v_bias + brow : nullptr,
-                  p.rope ? p.rope_cos + (size_t)sq.new_pos * (HD / 2) : nullptr,
-                  p.rope ? p.rope_sin + (size_t)sq.new_pos * (HD / 2) : nullptr, lane, k, v);
-  uint32_t kw, vc[4];
-  __half kd, vd;
-  quantise_row<HD>(lane, k, v, kw, kd, vc, vd);
-  const int unit = sq.len / kKv4Unit, r = sq.len % kKv4Unit;
-  unsigned char* sm = stage + (unit & 1) * UB;
-  unsigned char* gm = s.hb == 0 ? unit_ptr(p.pool, p.page_table + (size_t)sq.slot * p.max_pages_per_seq,
-                                           p.layer_begin + s.ll, s.kvh, unit, UB)
-                                : nullptr;
-  const int dim = R::dim(lane), b = dim >> 5;
-  if (R::has_k(lane) && (lane & 1) == 0) {
-    const int o = kv4_k_word(r, b, (dim & 31) >> 3);
-    *reinterpret_cast<uint32_t*>(sm + o) = kw;
-    if (gm) *reinterpret_cast<uint32_t*>(gm + o) = kw;
-  }
-  if (R::has_v(lane)) {
-    // the token's nibble of each dim's word: its byte also holds the token two places on or back, which the stage has
-    const int nib = kv4_nibble(r & 7);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int o = kv4_v_off(HD) + kv4_v_word(HD, dim + j, r >> 3) + (nib >> 1);
-      const uint32_t old = sm[o];
-      const unsigned char byte = (unsigned char)((nib & 1) ? (old & 0x0fu) | vc[j] << 4 : (old & 0xf0u) | vc[j]);
-      sm[o] = byte;
-      if (gm) gm[o] = byte;
-    }
-  }
-  if ((lane & 7) == 0) {
-    if (R::has_k(lane)) {
-      const int o = kv4_ks_off(HD) + kv4_scale(HD, r, b);
-      *reinterpret_cast<__half*>(sm + o) = kd;
-      if (gm) *reinterpret_cast<__half*>(gm + o) = kd;
-    }
-    if (R::has_v(lane)) {
-      const int o = kv4_vs_off(HD) + kv4_scale(HD, r, b);
-      *reinterpret_cast<__half*>(sm + o) = vd;
-      if (gm) *reinterpret_cast<__half*>(gm + o) = vd;
-    }
-  }
+  const int page = kv4_page_of(p.pool, f.tile);
+  const int in = f.tile - page * p.pool.tiles_per_page;
+  const int id = f.page_base >= 0 ? f.page_base + page : f.row[page];
+  f.tile += Dec<HD>::kWarps;
+  return f.base + ((long long)id * p.pool.kv_heads * p.pool.tiles_per_page + in) * Dec<HD>::TB;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(128, KV4_CTAS) kv4_decode_kernel(const __grid_constant__ Kv4DecodeParams p) {
+__global__ void __launch_bounds__(32 * Dec<HD>::kWarps, 2) kv4_decode_kernel(const __grid_constant__ Kv4DecodeParams p) {
   using D = Dec<HD>;
-  constexpr int NB = D::NB, UB = D::UB, H = kKv4Heads;
-  constexpr int rec = kv4_record_floats(HD);
-  extern __shared__ __align__(1024) unsigned char smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  unsigned char* ps = smem + D::p_off;
-  unsigned char* qs = smem + D::q_off;
-  unsigned char* ring = smem + D::ring_off;
-  float* sm_f = reinterpret_cast<float*>(smem + D::f_off);
-  float* sm_mb = reinterpret_cast<float*>(smem + D::mb_off);
-  float* sm_red = reinterpret_cast<float*>(smem + D::red_off);
-  volatile int* sm_flag = reinterpret_cast<volatile int*>(smem + D::flag_off);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + D::bar_off);
-  uint64_t* done1 = full + D::kRing;
-  uint64_t* done2 = done1 + 1;
-  Seg* pending = reinterpret_cast<Seg*>(smem + D::pend_off);
+  constexpr int NB = D::NB, W = D::kWarps, H = kKv4Heads;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + D::bar_off) + warp * D::kRing;
+  unsigned char* ring = smem + D::ring_off + warp * D::kRing * D::TB;
+  unsigned char* new_tile = smem + D::new_off;
+  float4* red = reinterpret_cast<float4*>(smem + D::red_off);
+  float* sm_m = reinterpret_cast<float*>(smem + D::stat_off);  // [W][8]
+  float* sm_l = sm_m + W * H;
+  int* sm_flag = reinterpret_cast<int*>(sm_l + W * H);
 
-  // the CTA's range of stages (stream split; an aligned CTA has one segment)
-  const bool aligned = p.block_parts != 0;
-  const int u_begin = aligned ? 0 : (int)stage_start(blockIdx.x, p.total_stages, p.grid);
-  const int u1 = aligned ? 1 : (int)stage_start(blockIdx.x + 1, p.total_stages, p.grid);
-  Feed feed{};
-  feed.u = u_begin;
-  feed.u1 = u1;
-  if (tid == 0) {
-    for (int i = 0; i < D::kRing + 2; ++i) mbar_init(&full[i], 1);
-    sm_flag[2] = 0;
+  if (lane == 0) {
+    for (int i = 0; i < D::kRing; ++i) mbar_init(&bars[i], 1);
     fence_mbarrier_init();
     fence_proxy_async_shared();
   }
   __syncwarp();
-  if (warp == 0) {
-    tmem_alloc(reinterpret_cast<uint32_t*>(smem + D::flag_off) + 3, 128);
-    tmem_relinquish();
-    tc_fence_before();
-  }
-  griddep_launch_dependents();
-  griddep_wait();  // below: the first access to global memory
-  int issued = 0;
-  if (tid == 0) {
-    for (; issued < D::kRing; ++issued) feed_issue<HD>(p, feed, ring + issued * D::kStageBytes, &full[issued]);
-  }
-  Seg s = kv4_seg_at(p, u_begin, u1);
-  float qr[2][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) fetch_query<HD>(p, s, 2 * warp + i, lane, qr[i]);
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *(reinterpret_cast<uint32_t*>(smem + D::flag_off) + 3);
-  const uint32_t my_a = tmem + ((uint32_t)(warp * 32) << 16) + D::kColA;
-  const uint32_t my_d = tmem + ((uint32_t)(warp * 32) << 16) + D::kColD;
-  const uint32_t magic = code_magic();
-  // A wait that runs out sets the error word and the CTA's abort flag; the CTA then goes through the rest of its
-  // steps without waiting (its results are void), so that every barrier below stays matched.
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!mbar_try_wait(bar, parity) && !sm_flag[2] && !mbar_wait(bar, parity)) {
-      sm_flag[2] = 1;
-      set_error(p.error, 60);
+
+  const long long u1 = stage_start(blockIdx.x + 1, p.total_units, p.grid);
+  long long u = stage_start(blockIdx.x, p.total_units, p.grid);
+  const long long u_begin = u;
+  Feed feed{u, u1, 0, 0, nullptr, nullptr, -1};
+  auto issue = [&](int slot) {
+    const unsigned char* src = feed_next<HD>(p, feed, warp);
+    if (src && lane == 0) {
+      mbar_arrive_expect_tx(&bars[slot], D::TB);
+      bulk_load(ring + slot * D::TB, src, D::TB, &bars[slot]);
     }
-    __syncwarp();  // warp-collective TMEM accesses follow
+    return src != nullptr;
   };
+  int issued = 0, used = 0;      // tiles copied / consumed by this warp
+  for (int i = 0; i < D::kRing; ++i) issued += issue(i) ? 1 : 0;
+  bool ok = true;                // false: a wait ran out; the warp computes no more
 
-  const int row = tid & 63, unit = tid >> 6;  // this thread's token in the stage
-  const int k_scale = unit * UB + kv4_ks_off(HD) + kv4_scale(HD, row, 0);
-  const int v_scale = unit * UB + kv4_vs_off(HD) + kv4_scale(HD, row, 0);
-  // this thread's row of the weights, and its chunks' swizzle; odd pairs of tokens meet 16 (c - 8)
-  const int prow = HD == 128 ? tid : row;
-  const uint32_t p_addr = smem_u32(ps) + prow * 128;
-  const int p_chunk = HD == 128 ? 0 : unit * 4;
-  const float v_div = (tid & 2) ? 0.0625f : 1.f;
-
-  int slot = 0;
-  uint32_t phase = 0, phase1 = 0, phase2 = 0;
-  int n_pending = 0;   // partial segments of this CTA, whose groups may be its to fold (kept in shared memory)
-
-  while (true) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) stage_query<HD>(p, s, 2 * warp + i, lane, qr[i], qs, sm_f);
-    if (tid < H) sm_mb[tid] = INFINITY;
-    fence_proxy_async_shared();
-    const int attended = p.seqs[s.si].len + (p.k_new ? 1 : 0);
-    const bool more = s.next < u1;
-    Seg nx = s;
-    if (more) {  // the next segment's query rows travel while this one is attended
-      nx = kv4_seg_at(p, s.next, u1);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) fetch_query<HD>(p, nx, 2 * warp + i, lane, qr[i]);
+  WarpState<HD> w;
+  while (u < u1) {
+    const Seg s = kv4_seg_at(p, u, u1);
+    const Kv4Seq& sq = p.seqs[s.si];
+    const bool append = p.k_new != nullptr && s.last;
+    const int n_tiles = s.t1 - s.t0;
+    const bool appender = append && warp == n_tiles % W;
+    if (appender) {
+      // the new token: quantised into the cache (by the first head block) and into a tile of its own here
+      const size_t at = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * p.pool.kv_heads + s.kvh) * HD;
+      const size_t brow = ((size_t)(p.layer_begin + s.ll) * p.pool.kv_heads + s.kvh) * HD;
+      float k[4], v[4];
+      load_row<HD>(p.k_new, p.v_new, at, p.input_f16, p.k_bias ? p.k_bias + brow : nullptr,
+                   p.k_bias ? p.v_bias + brow : nullptr,
+                   p.rope ? p.rope_cos + (size_t)sq.new_pos * (HD / 2) : nullptr,
+                   p.rope ? p.rope_sin + (size_t)sq.new_pos * (HD / 2) : nullptr, lane, k, v);
+      float k2[4] = {k[0], k[1], k[2], k[3]}, v2[4] = {v[0], v[1], v[2], v[3]};
+      store_row<HD>(new_tile, 0, lane, k, v);
+      if (s.hb == 0) {
+        unsigned char* dst = tile_ptr(p.pool, p.page_table + (size_t)sq.slot * p.max_pages_per_seq, p.layer_begin + s.ll,
+                                      s.kvh, sq.len / kKv4Tile, D::TB);
+        store_row<HD>(dst, sq.len % kKv4Tile, lane, k2, v2);
+      }
     }
-    float o[H];
-    uint64_t l2[H / 2];
-#pragma unroll
-    for (int h = 0; h < H; ++h) o[h] = 0.f;
-#pragma unroll
-    for (int h = 0; h < H / 2; ++h) l2[h] = 0;
-    float vlim = 0.f;     // largest |V scale| the current vexp allows
-    uint32_t vmul = 0;    // 2^vexp (over 16 for odd pairs of tokens), twice, f16
-    int vexp = 0;
-    bool open = false;    // a second product is in flight
-    auto take_o = [&]() {
-      wait(done2, phase2);
-      phase2 ^= 1u;
-      tc_fence_after();
-      float d[16];
-      tmem_ld16(my_d + 16 * warp, d);
-      tmem_wait_ld();
-#pragma unroll
-      for (int h = 0; h < H; ++h) o[h] += d[h] + d[8 + h];
-    };
-
-    for (int st = s.s0; st < s.s1; ++st) {
-      unsigned char* stage = ring + slot * D::kStageBytes;
-      const uint32_t sa = smem_u32(stage);
-      wait(&full[slot], phase);
-      if (p.k_new && st == s.n - 1) {
-        __syncthreads();  // every thread has seen the copy land
-        if (warp == 0) place_new_token<HD>(p, s, stage, lane);
-        fence_proxy_async_shared();  // before a later copy into this slot
-        __syncthreads();
+    load_queries<HD>(p, s, lane, w);
+    reset_state<HD>(w);
+    for (int tile = s.t0 + warp; tile < s.t1; tile += W) {
+      const int slot = used % D::kRing;
+      if (ok) ok = mbar_wait_warp(&bars[slot], (used / D::kRing) & 1);
+      if (!ok) {
+        if (lane == 0) set_error(p.error, 60);
+        break;
       }
-      const int left = attended - st * kKv4Stage;  // tokens of this stage that are attended
+      attend_tile<HD>(smem_u32(ring + slot * D::TB), min(sq.len - tile * kKv4Tile, kKv4Tile), lane, w);
+      __syncwarp();
+      ++used;
+      issued += issue(slot) ? 1 : 0;
+    }
+    if (appender) {
+      __syncwarp();
+      attend_tile<HD>(smem_u32(new_tile), 1, lane, w);
+    }
 
-      // K codes -> TMEM, one token a row
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        uint32_t c[16];
-        centred_chunk(sa + unit * UB + kv4_k_word(row, b, 0), magic, c);
-        if (b == 0 && open) take_o();  // the A columns and D are free once the last second product is done
-        tmem_st16(my_a + 16 * b, c);
+    // merge the warps' states: m and l per head first, then O in two rounds
+    float l = w.l;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) {
+      sm_m[warp * H + g] = w.m;
+      sm_l[warp * H + g] = l;
+    }
+    __syncthreads();
+    auto part_weight = [](float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); };
+    {
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+      for (int i = 0; i < W; ++i) {
+        mx0 = fmaxf(mx0, sm_m[i * H + 2 * t]);
+        mx1 = fmaxf(mx1, sm_m[i * H + 2 * t + 1]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
-        tc_fence_after();
-        constexpr uint32_t idesc = idesc_f16_f32(128, 16, false, false);
+      const float vs = pow2i(-w.vexp);
+      const float c0 = part_weight(sm_m[warp * H + 2 * t], mx0) * vs;
+      const float c1 = part_weight(sm_m[warp * H + 2 * t + 1], mx1) * vs;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint64_t b = smem_desc_sw128(smem_u32(qs) + (k >> 2) * 2048 + (k & 3) * 32, 16, 1024);
-          umma_ts(tmem + D::kColD + (k >> 1) * 16, tmem + D::kColA + k * 8, b, idesc, k & 1);
-        }
-        umma_commit(done1);
-      }
-
-      // V codes: this thread's dim (head_dim 64: of its unit), widened while the product runs
-      uint32_t vr[HD / 2];
-      if constexpr (HD == 128) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          centred_chunk(sa + (i >> 1) * UB + kv4_v_off(HD) + kv4_v_word(HD, tid, 4 * (i & 1)), magic, vr + 16 * i);
-        }
-      } else {
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          centred_chunk(sa + unit * UB + kv4_v_off(HD) + kv4_v_word(HD, row, 4 * i), magic, vr + 16 * i);
+          w.o[b][i][0] *= c0;
+          w.o[b][i][1] *= c1;
+          w.o[b][i][2] *= c0 * 0.0625f;
+          w.o[b][i][3] *= c1 * 0.0625f;
         }
-      }
-      uint32_t ks[NB / 2], vs[NB / 2];
-#pragma unroll
-      for (int i = 0; i < NB / 2; ++i) {
-        ks[i] = *reinterpret_cast<const uint32_t*>(stage + k_scale + 4 * i);
-        vs[i] = *reinterpret_cast<const uint32_t*>(stage + v_scale + 4 * i);
-      }
-      wait(done1, phase1);
-      phase1 ^= 1u;
-      tc_fence_after();
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) tmem_st16(my_a + 16 * i, vr + 16 * i);
-
-      // scores of this thread's token, 8 heads in pairs
-      uint64_t x2[H / 2];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float d[16];
-        tmem_ld16(my_d + 16 * b, d);
-        tmem_wait_ld();
-        const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(&ks[b >> 1]));
-        const float kd = (b & 1) ? kf.y : kf.x;
-        const uint64_t kd2 = f2_pack(kd, kd);
-#pragma unroll
-        for (int h = 0; h < H / 2; ++h) {
-          const uint64_t sum = f2_add(f2_pack(d[2 * h], d[2 * h + 1]), f2_pack(d[8 + 2 * h], d[9 + 2 * h]));
-          x2[h] = b == 0 ? f2_mul(kd2, sum) : f2_fma(kd2, sum, x2[h]);
-        }
-      }
-      const bool in = tid < left;
-      if (!in) {  // a token past the sequence: no weight, whatever its place holds
-        const uint64_t none = f2_pack(-INFINITY, -INFINITY);
-#pragma unroll
-        for (int h = 0; h < H / 2; ++h) x2[h] = none;
-#pragma unroll
-        for (int i = 0; i < NB / 2; ++i) vs[i] = 0u;
-      }
-      float mb[H];
-      bool need = false;
-      {
-        const uint4 a = lds128(smem_u32(sm_mb)), b = lds128(smem_u32(sm_mb) + 16);
-        const uint4 c = lds128(smem_u32(sm_f)), e = lds128(smem_u32(sm_f) + 16);
-        const uint32_t mw[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, fw[8] = {c.x, c.y, c.z, c.w, e.x, e.y, e.z, e.w};
-#pragma unroll
-        for (int h = 0; h < H; ++h) mb[h] = __uint_as_float(mw[h]);
-#pragma unroll
-        for (int h = 0; h < H / 2; ++h) {
-          x2[h] = f2_mul(x2[h], f2_pack(__uint_as_float(fw[2 * h]), __uint_as_float(fw[2 * h + 1])));
-        }
-      }
-      uint32_t vm = h2_maxabs(vs[0], vs[NB / 2 - 1]);
-      const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
-      const float vtop = fmaxf(vmf.x, vmf.y);
-      need = vtop > vlim;
-#pragma unroll
-      for (int h = 0; h < H / 2; ++h) {
-        float x, y;
-        f2_unpack(x2[h], x, y);
-        need = need || x + mb[2 * h] > kWeightExp + kSlack || y + mb[2 * h + 1] > kWeightExp + kSlack;
-      }
-      if (__syncthreads_or(need ? 1 : 0)) {
-        // the largest score of each head and the largest V scale over the stage
-        float mx[H + 1];
-#pragma unroll
-        for (int h = 0; h < H / 2; ++h) f2_unpack(x2[h], mx[2 * h], mx[2 * h + 1]);
-        mx[H] = vtop;
-#pragma unroll
-        for (int h = 0; h <= H; ++h) {
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], off));
-          if (lane == 0) sm_red[warp * (H + 1) + h] = mx[h];
-        }
-        __syncthreads();
-        float vx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vx = fmaxf(vx, sm_red[i * (H + 1) + H]);
-        float beta = 1.f;
-        if (vx > vlim) {
-          const int e = min(exponent_of(vx), 15);
-          const int k = min(max(-1 - e, -16), 15);  // |V scale| 2^k in [0.5, 1) now, at most 2 until it moves again
-          beta = vlim > 0.f ? pow2i(k - vexp) : 1.f;
-          vexp = k;
-          vlim = pow2i(e + 2);
-          const __half2 m = __float2half2_rn(pow2i(k) * v_div);
-          vmul = *reinterpret_cast<const uint32_t*>(&m);
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, sm_red[i * (H + 1) + h]);
-          float alpha = 1.f;
-          if (top + mb[h] > kWeightExp + kSlack) {
-            alpha = ex2(kWeightExp - top - mb[h]);  // 0 from the first reference (mb = +inf)
-            mb[h] = kWeightExp - top;
-          }
-          o[h] *= alpha * beta;
-          float x, y;
-          f2_unpack(l2[h >> 1], x, y);
-          if (h & 1) y *= alpha; else x *= alpha;
-          l2[h >> 1] = f2_pack(x, y);
-        }
-        __syncthreads();  // every thread has read the old references
-        if (tid == 0) {
-#pragma unroll
-          for (int h = 0; h < H; ++h) sm_mb[h] = mb[h];
-        }
-      }
-
-      // weights, and their products with the token's V scales as f16 hi + lo
-      uint32_t ph[H / 2], pl[H / 2];
-#pragma unroll
-      for (int h = 0; h < H / 2; ++h) {
-        float x, y;
-        f2_unpack(f2_add(x2[h], f2_pack(mb[2 * h], mb[2 * h + 1])), x, y);
-        const float p0 = ex2(x), p1 = ex2(y);
-        l2[h] = f2_add(l2[h], f2_pack(p0, p1));
-        const __half2 a = __floats2half2_rn(p0, p1);
-        const float2 af = __half22float2(a);
-        ph[h] = *reinterpret_cast<const uint32_t*>(&a);
-        pl[h] = pack_half2(p0 - af.x, p1 - af.y);
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const uint32_t d2 = h2_mul(vs[b >> 1], vmul);
-        const uint32_t d = prmt(d2, d2, (b & 1) ? 0x3232 : 0x1010);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          hi[h] = h2_mul(ph[h], d);
-          lo[h] = h2_fma(pl[h], d, h2_fms(ph[h], d, hi[h]));
-        }
-        sts128(p_addr + (((p_chunk + 2 * b) ^ (prow & 7)) * 16), hi[0], hi[1], hi[2], hi[3]);
-        sts128(p_addr + (((p_chunk + 2 * b + 1) ^ (prow & 7)) * 16), lo[0], lo[1], lo[2], lo[3]);
-      }
-      fence_proxy_async_shared();
-      tmem_wait_st();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
-        tc_fence_after();
-        constexpr uint32_t idesc = idesc_f16_f32(128, 64, false, true);
-#pragma unroll
-        for (int k = 0; k < D::kPRows / 16; ++k) {
-          const uint64_t b = smem_desc_sw128(smem_u32(ps) + k * 2048, 8192, 1024);
-          umma_ts(tmem + D::kColD, tmem + D::kColA + k * 8, b, idesc, k > 0);
-        }
-        umma_commit(done2);
-        if (!sm_flag[2]) feed_issue<HD>(p, feed, stage, &full[slot]);  // every read of the slot is behind the barrier
-      }
-      open = true;
-      if (++slot == D::kRing) {
-        slot = 0;
-        phase ^= 1u;
-      }
     }
-    if (open) take_o();
-
-    // sums of the weights over the threads
-    float l[H];
+    auto o_item = [&](int b, int c) {
+      return make_float4(w.o[b][0][c], w.o[b][0][2 + c], w.o[b][1][c], w.o[b][1][2 + c]);
+    };
+    if (warp >= W / 2) {
 #pragma unroll
-    for (int h = 0; h < H / 2; ++h) f2_unpack(l2[h], l[2 * h], l[2 * h + 1]);
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+        for (int c = 0; c < 2; ++c) red[(warp - W / 2) * D::kItems + (b * 2 + c) * 32 + lane] = o_item(b, c);
     }
-    if (lane == 0) {
+    __syncthreads();
+    if (warp < W / 2) {
 #pragma unroll
-      for (int h = 0; h < H; ++h) sm_red[warp * (H + 1) + h] = l[h];
-    }
-    const float vs = pow2i(-vexp);
-    if constexpr (HD == 64) {  // the two units' halves of each dim
-      float* half = reinterpret_cast<float*>(ps);  // the second product has been taken
-      if (unit == 1) {
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int h = 0; h < H; ++h) half[h * 64 + row] = o[h];
-      }
-      __syncthreads();
-      if (unit == 0) {
-#pragma unroll
-        for (int h = 0; h < H; ++h) o[h] += half[h * 64 + row];
-      }
-    } else {
-      __syncthreads();
-    }
-    const size_t out_row = ((size_t)s.ll * p.seq_total + p.seq_base + s.si) * (p.pool.kv_heads * p.group) +
-                           s.kvh * p.group + s.hb * p.block_heads;
-    const int heads = min(p.block_heads, p.group - s.hb * p.block_heads);
-    const bool dim_mine = HD == 128 || unit == 0;
-    const int dim = HD == 128 ? tid : row;
-    // a CTA's first segment uses its slot 0, its last another one: at most two of its segments are parts of groups
-    float* mine = p.partials + ((size_t)blockIdx.x * 2 + (aligned || s.gb + s.s0 == u_begin ? 0 : 1)) * rec;
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      const float sum = (sm_red[h] + sm_red[(H + 1) + h]) + (sm_red[2 * (H + 1) + h] + sm_red[3 * (H + 1) + h]);
-      const float acc = o[h] * vs;
-      const float m = kWeightExp - sm_mb[h];
-      if (s.parts > 1) {
-        if (dim_mine) mine[h * HD + dim] = acc;
-        if (tid == 0) {
-          mine[H * HD + h] = m;
-          mine[H * HD + H + h] = sum;
+        for (int c = 0; c < 2; ++c) {
+          float4* slot = &red[warp * D::kItems + (b * 2 + c) * 32 + lane];
+          const float4 x = *slot, y = o_item(b, c);
+          *slot = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
-      } else if (h < heads && dim_mine) {
-        if (p.partial_out) {
-          constexpr float k = 0x1p-11f;  // 2^-kWeightExp
-          float* dst = p.out + (out_row + h) * (HD + 2);
-          dst[dim] = acc * k;
-          if (dim == 0) {
-            dst[HD] = m;
-            dst[HD + 1] = sum * k;
-          }
-        } else {
-          p.out[(out_row + h) * HD + dim] = sum == 0.f ? 0.f : acc / sum;  // no token at all: zeros
-        }
-      }
     }
+    __syncthreads();
+    // item i: block i / 64, heads 2 (i % 4) + (i / 32) % 2, dims 4 ((i % 32) / 4) .. + 3 of the block
+    const int i = threadIdx.x;
+    const int head = 2 * (i & 3) + ((i >> 5) & 1);
+    const int dim = 32 * (i >> 6) + 4 * ((i & 31) >> 2);
+    const bool mine = i < D::kItems;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.f;
+    if (mine) {
+      for (int k = 0; k < W / 2; ++k) {
+        const float4 x = red[k * D::kItems + i];
+        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+      }
+      for (int k = 0; k < W; ++k) top = fmaxf(top, sm_m[k * H + head]);
+      for (int k = 0; k < W; ++k) sum += sm_l[k * H + head] * part_weight(sm_m[k * H + head], top);
+    }
+    bool write = true;
     if (s.parts > 1) {
-      if (tid == 0) pending[n_pending] = s;
-      ++n_pending;
-    }
-    __syncthreads();  // the reduction buffers are free again
-    if (!more) break;
-    s = nx;
-  }
-
-  // Groups shared with other CTAs: the last of a group's CTAs to arrive folds its records, in part order.
-  if (n_pending > 0) {
-    if (tid == 0) {
-      __threadfence();
-      for (int i = 0; i < n_pending; ++i) {
-        const Seg& q = pending[i];
-        sm_flag[i] = atomicAdd(&p.counters[q.group_id], 1u) == (uint32_t)q.parts - 1u;
-      }
-      __threadfence();
-    }
-    __syncthreads();
-    for (int i = 0; i < n_pending; ++i) {
-      if (sm_flag[i] == 0) continue;
-      const Seg& q = pending[i];
-      // part k is CTA c0 + k's: its first segment unless (stream split) its range began before the group
-      auto rec_of = [&](int k) {
-        const int c = q.c0 + k;
-        const int sl = aligned || stage_start(c, p.total_stages, p.grid) >= q.gb ? 0 : 1;
-        return p.partials + ((size_t)c * 2 + sl) * rec;
-      };
-      float* wt = reinterpret_cast<float*>(ring);  // [parts][8] m, then weights; [parts][8] l (no copy in flight now)
-      float* tot = sm_red;                         // [8] sums, [8] reference exponents
-      __syncthreads();
-      for (int j = tid; j < q.parts * 2 * H; j += 128) {
-        const int k = j / (2 * H), e = j - k * 2 * H;
-        wt[(e < H ? 0 : q.parts * H) + k * H + (e & 7)] = __ldcg(rec_of(k) + H * HD + e);
-      }
-      __syncthreads();
-      if (tid < H) {
-        float all = -INFINITY, sum = 0.f;
-        for (int k = 0; k < q.parts; ++k) all = fmaxf(all, wt[k * H + tid]);
-        for (int k = 0; k < q.parts; ++k) {
-          const float m = wt[k * H + tid];
-          const float e = m == -INFINITY ? 0.f : ex2(m - all);
-          wt[k * H + tid] = e;
-          sum = fmaf(e, wt[(q.parts + k) * H + tid], sum);
+      // publish this part; the last of the group's parts to arrive folds them all, in part order
+      constexpr int rec = kv4_record_floats(HD);
+      // a CTA's first segment uses its slot 0, its last another one: at most two of its segments are parts
+      float* mine_rec = p.partials + ((size_t)blockIdx.x * 2 + (u == u_begin ? 0 : 1)) * rec;
+      if (mine) {
+        reinterpret_cast<float4*>(mine_rec)[i] = acc;
+        if (dim == 0) {
+          mine_rec[H * HD + head] = top;
+          mine_rec[H * HD + H + head] = sum;
         }
-        tot[tid] = sum;
-        tot[H + tid] = all;
       }
       __syncthreads();
-      const size_t out_row = ((size_t)q.ll * p.seq_total + p.seq_base + q.si) * (p.pool.kv_heads * p.group) +
-                             q.kvh * p.group + q.hb * p.block_heads;
-      const int heads = min(p.block_heads, p.group - q.hb * p.block_heads);
-      constexpr int kPer = HD / 16;  // heads of a thread: all 8, or 4 at head_dim 64
-      const int h0 = HD == 128 ? 0 : unit * 4, dim = HD == 128 ? tid : row;
-      float acc[kPer];
-#pragma unroll
-      for (int h = 0; h < kPer; ++h) acc[h] = 0.f;
+      if (threadIdx.x == 0) {
+        __threadfence();
+        const uint32_t old = atomicAdd(&p.counters[s.group_id], 1u);
+        *sm_flag = old == (uint32_t)s.parts - 1u;
+        __threadfence();
+      }
+      __syncthreads();
+      write = *sm_flag != 0;
+      if (write && mine) {
+        // part k is CTA c0 + k's: its first segment unless the CTA's range began before the group
+        const long long gb = u - (long long)(s.t0 / kKv4UnitTiles);
+        auto rec_of = [&](int k) {
+          const long long c = s.c0 + k;
+          const int slot = stage_start(c, p.total_units, p.grid) >= gb ? 0 : 1;
+          return p.partials + ((size_t)c * 2 + slot) * rec;
+        };
+        float all = -INFINITY;
+        for (int k = 0; k < s.parts; ++k) all = fmaxf(all, __ldcg(rec_of(k) + H * HD + head));
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
 #pragma unroll 4
-      for (int k = 0; k < q.parts; ++k) {
-        const float* r = rec_of(k);
-#pragma unroll
-        for (int h = 0; h < kPer; ++h) acc[h] = fmaf(wt[k * H + h0 + h], __ldcg(r + (h0 + h) * HD + dim), acc[h]);
-      }
-#pragma unroll
-      for (int h = 0; h < kPer; ++h) {
-        if (h0 + h >= heads) continue;
-        const float sum = tot[h0 + h];
-        if (p.partial_out) {
-          constexpr float k = 0x1p-11f;
-          float* dst = p.out + (out_row + h0 + h) * (HD + 2);
-          dst[dim] = acc[h] * k;
-          if (dim == 0) {
-            dst[HD] = tot[H + h0 + h];
-            dst[HD + 1] = sum * k;
-          }
-        } else {
-          p.out[(out_row + h0 + h) * HD + dim] = sum == 0.f ? 0.f : acc[h] / sum;
+        for (int k = 0; k < s.parts; ++k) {
+          const float* r = rec_of(k);
+          const float wt = part_weight(__ldcg(r + H * HD + head), all);
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(r) + i);
+          acc.x = fmaf(wt, x.x, acc.x);
+          acc.y = fmaf(wt, x.y, acc.y);
+          acc.z = fmaf(wt, x.z, acc.z);
+          acc.w = fmaf(wt, x.w, acc.w);
+          sum = fmaf(wt, __ldcg(r + H * HD + H + head), sum);
         }
+        top = all;
       }
-      if (tid == 0) p.counters[q.group_id] = 0;
+      if (write && threadIdx.x == 0) p.counters[s.group_id] = 0;
     }
+    const int hg = s.hb * p.block_heads + head;
+    if (write && mine && head < p.block_heads && hg < p.group) {
+      const size_t row = ((size_t)s.ll * p.seq_total + p.seq_base + s.si) * (p.pool.kv_heads * p.group) +
+                         s.kvh * p.group + hg;
+      if (p.partial_out) {
+        constexpr float k = 0x1p-8f;  // 2^-kWeightExp
+        float* o = p.out + row * (HD + 2);
+        o[dim] = acc.x * k;
+        o[dim + 1] = acc.y * k;
+        o[dim + 2] = acc.z * k;
+        o[dim + 3] = acc.w * k;
+        if (dim == 0) {
+          o[HD] = top;
+          o[HD + 1] = sum * k;
+        }
+      } else {
+        const float r = sum == 0.f ? 0.f : 1.f / sum;  // no token at all: zeros
+        *reinterpret_cast<float4*>(p.out + row * HD + dim) = make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r);
+      }
+    }
+    u = s.next;
+    __syncthreads();  // the merge buffers and the new token's tile are free again
   }
-  __syncthreads();
-  if (sm_flag[2]) {
-    // a wait ran out: copies and products may still be in flight; let them land before the CTA leaves
-    for (int i = 0; i < D::kRing; ++i) (void)mbar_wait(&full[i], phase ^ (i < slot ? 1u : 0u));
-    (void)mbar_wait(done1, phase1);
-    (void)mbar_wait(done2, phase2);
-    __syncthreads();
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 128);
+  if (!ok) {
+    // copies of this warp may still be in flight: let them land before the CTA leaves
+    for (; used < issued; ++used) (void)mbar_wait_warp(&bars[used % D::kRing], (used / D::kRing) & 1);
   }
 }
 
@@ -1221,67 +1008,29 @@ cudaError_t launch_decode_t(const Kv4DecodeParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = set_smem_limit_once(done, reinterpret_cast<const void*>(kv4_decode_kernel<HD>), Dec<HD>::smem);
   if (e != cudaSuccess) return e;
-  // Programmatic dependent launch: the CTAs set up their barriers and TMEM while the previous kernel drains, and
-  // wait for it before touching global memory.
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)p.grid);
-  cfg.blockDim = dim3(Dec<HD>::kThreads);
-  cfg.dynamicSmemBytes = Dec<HD>::smem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_decode_kernel<HD>, p);
+  kv4_decode_kernel<HD><<<p.grid, 32 * Dec<HD>::kWarps, Dec<HD>::smem, s>>>(p);
+  return cudaGetLastError();
 }
 
-// Work items of the append and read kernels: (layer, kv head, 32 tokens).
-long long half_items(const Kv4RowsParams& p) {
-  return (long long)((p.first + p.n_tokens - 1) / 32 - p.first / 32 + 1) * p.pool.kv_heads * p.n_layers;
+long long row_items(const Kv4RowsParams& p) {
+  const long long tiles = (p.first + p.n_tokens - 1) / kKv4Tile - p.first / kKv4Tile + 1;
+  return tiles * p.pool.kv_heads * p.n_layers;
 }
 
 }  // namespace
 
-int kv4_decode_ctas_per_sm(int) { return KV4_CTAS; }
+int kv4_decode_ctas_per_sm() { return 2; }
 
-void plan_kv4_decode(Kv4DecodeParams& p, long long slots) {
-  const int extra = p.k_new ? 1 : 0;
-  const long long reps = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks;
-  int acc = 0, longest = 1;
+void plan_kv4_decode(Kv4DecodeParams& p, long long max_grid) {
+  int acc = 0;
   for (int i = 0; i < p.n_seqs; ++i) {
-    const int n = kv4_stages(p.seqs[i].len + extra);
-    p.seqs[i].stage_begin = acc;
-    acc += n;
-    longest = n > longest ? n : longest;
+    p.seqs[i].unit_begin = acc;
+    acc += kv4_units(p.seqs[i].len);
   }
-  p.block_stages = acc;
-  p.total_stages = reps * acc;
-  // Aligned split: every group in equal parts of at most `most` stages, one part a CTA, all resident at once.
-  auto parts_for = [&](int most) {
-    long long c = 0;
-    for (int i = 0; i < p.n_seqs; ++i) c += (kv4_stages(p.seqs[i].len + extra) + most - 1) / most;
-    return c * reps;
-  };
-  const long long ideal = (p.total_stages + slots - 1) / slots;
-  int lo = 1, hi = longest;
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (parts_for(mid) <= slots) hi = mid; else lo = mid + 1;
-  }
-  if (lo < 2 && longest >= 2) lo = 2;
-  if (parts_for(lo) <= slots && lo <= ideal + ideal / 8 + 1) {
-    int parts = 0;
-    for (int i = 0; i < p.n_seqs; ++i) {
-      p.seqs[i].part_begin = parts;
-      parts += (kv4_stages(p.seqs[i].len + extra) + lo - 1) / lo;
-    }
-    p.block_parts = parts;
-    p.grid = (int32_t)(reps * parts);
-    return;
-  }
-  p.block_parts = 0;
-  p.grid = (int32_t)(p.total_stages < slots ? p.total_stages : slots);
+  p.block_units = acc;
+  p.total_units = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks * acc;
+  const long long want = (p.total_units + 1) / 2;  // 128 tokens a CTA: one tile a warp
+  p.grid = (int32_t)(want < max_grid ? want : max_grid);
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream_t s) {
@@ -1289,22 +1038,21 @@ cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream
 }
 
 cudaError_t launch_kv4_append(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
-  const unsigned grid = (unsigned)half_items(p);
-  if (head_dim == 128) kv4_append_kernel<128><<<grid, 128, 0, s>>>(p);
-  else kv4_append_kernel<64><<<grid, 128, 0, s>>>(p);
+  const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
+  if (head_dim == 128) kv4_append_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else kv4_append_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
 
 cudaError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
-  const unsigned grid = (unsigned)half_items(p);
-  if (head_dim == 128) kv4_read_kernel<128><<<grid, 128, 0, s>>>(p);
-  else kv4_read_kernel<64><<<grid, 128, 0, s>>>(p);
+  const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
+  if (head_dim == 128) kv4_read_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else kv4_read_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
 
 cudaError_t launch_kv4_raw(const Kv4RowsParams& p, int head_dim, bool to_pool, cudaStream_t s) {
-  const long long groups = (p.first + p.n_tokens - 1) / 8 - p.first / 8 + 1;
-  const long long n = groups * p.n_layers * p.pool.kv_heads * (head_dim / 32);
+  const long long n = (long long)p.n_layers * p.n_tokens * p.pool.kv_heads * (head_dim / 32);
   const unsigned grid = (unsigned)((n + 127) / 128);
   if (head_dim == 128) kv4_raw_kernel<128><<<grid, 128, 0, s>>>(p, to_pool ? 1 : 0);
   else kv4_raw_kernel<64><<<grid, 128, 0, s>>>(p, to_pool ? 1 : 0);

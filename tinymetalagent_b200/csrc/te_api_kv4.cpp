@@ -33,9 +33,9 @@ Kv4Pool pool_of(const te_kv4_cache* c) {
   p.base = c->pool;
   p.num_pages = (int32_t)c->b.d.total_pages;
   p.kv_heads = (int32_t)c->b.d.kv_heads;
-  p.units_per_page = (int32_t)(c->b.d.page_tokens / kKv4Unit);
-  const uint64_t n = (uint64_t)p.units_per_page;
-  p.upp_magic = n == 1 ? 0u : (uint32_t)(((1ull << 32) + n - 1) / n);
+  p.page_tokens = (int32_t)c->b.d.page_tokens;
+  p.tiles_per_page = (int32_t)(c->b.d.page_tokens / kKv4Tile);
+  p.tpp_magic = (uint32_t)(((1ull << 32) + (uint64_t)p.tiles_per_page - 1) / (uint64_t)p.tiles_per_page);
   return p;
 }
 
@@ -92,11 +92,11 @@ TE_API te_status te_kv4_cache_create(te_attn_engine* e, const te_kv_cache_desc* 
   te_kv4_cache* c = nullptr;
   const size_t half = d.head_dim / 2;
   const size_t tab_floats = 2 * (size_t)d.max_position * half;
-  const double pool_bytes = (double)d.layers * (double)pages * d.kv_heads * (d.page_tokens / kKv4Unit) *
-                            kv4_unit_bytes((int)d.head_dim);
+  const double pool_bytes = (double)d.layers * (double)pages * d.kv_heads * (d.page_tokens / kKv4Tile) *
+                            kv4_tile_bytes((int)d.head_dim);
   if (pool_bytes > 1e13) return fail(e, TE_STATUS_OUT_OF_MEMORY, "4-bit KV pool too large");
-  const size_t bytes = (size_t)d.layers * pages * d.kv_heads * (d.page_tokens / kKv4Unit) *
-                       (size_t)kv4_unit_bytes((int)d.head_dim);
+  const size_t bytes = (size_t)d.layers * pages * d.kv_heads * (d.page_tokens / kKv4Tile) *
+                       (size_t)kv4_tile_bytes((int)d.head_dim);
   try {
     c = new te_kv4_cache();
     te_kv_cache& b = c->b;
@@ -395,9 +395,9 @@ TE_API te_status te_kv4_attention_decode(te_kv4_cache* c, size_t layer_begin, si
     }
     p.n_seqs = (int32_t)nb;
     p.seq_base = (int32_t)base;
-    plan_kv4_decode(p, (long long)e->sm_count * kv4_decode_ctas_per_sm((int)hd));
+    plan_kv4_decode(p, (long long)e->sm_count * kv4_decode_ctas_per_sm());
     const size_t groups = n_layers * hkv * (size_t)p.head_blocks * nb;
-    if (p.total_stages > (long long)INT32_MAX || groups > (size_t)INT32_MAX) {
+    if (p.total_units > (long long)INT32_MAX || groups > (size_t)INT32_MAX) {
       return fail(e, TE_STATUS_UNSUPPORTED, "decode call too large");
     }
     const size_t part_bytes = (size_t)p.grid * 2 * kv4_record_floats((int)hd) * sizeof(float);

@@ -1,22 +1,27 @@
 // The 4-bit KV cache: record layout and kernel parameters, shared by
 // te_api_kv4.cpp and k_kv4.cu.  Not installed; not part of the ABI.
 //
-// A key or value row of one kv head is NB = head_dim / 32 GGUF Q4_0 blocks: a
+// A key or value row of one kv head is head_dim / 32 GGUF Q4_0 blocks: a
 // binary16 scale d and 32 codes c, each standing for (c - 8) d.  The pool is
-// [layers][pages][kv_heads][page_tokens / 64] units of 64 tokens, keys and
-// values together, so that one unit is one contiguous copy of 72 hd bytes:
+// [layers][pages][kv_heads][page_tokens / 16] tiles of 16 tokens, keys and
+// values together, so that one tile is one contiguous copy:
 //
-//   K codes | V codes | K scales | V scales      32 hd, 32 hd, 4 hd, 4 hd
+//   K codes | V codes | K scales | V scales      8 * hd, 8 * hd, hd, hd bytes
 //
-// The codes lie as the tensor core's A operands want them, one row per thread
-// and 8 codes a word; a word w holds code 2p + e (p < 4, e < 2) in nibble
-// p + 4e, so that its four f16 pairs come from one mask each (w & 0x000f000f,
+// Inside a tile the codes lie as the warp-level m16n8k16 product wants them:
+// lane 4g + t of a warp (g < 8, t < 4) owns 16-byte aligned words, and each
+// 32-bit word w yields its four f16 pairs by one mask each (w & 0x000f000f,
 // w & 0x00f000f0, and the same of w >> 8).
-//   K: a row is a token.  Word (r, b, t): token r, dims 32b + 8t .. + 7, at
-//     byte (64b + r) 16 + 4t.
-//   V: a row is a dim (V^T).  Word (d, y): dim d, tokens 8y .. + 7, at byte
-//     ((y / 4) hd + d) 16 + 4 (y % 4).
-//   scale (r, b): token r, block b, at byte 2 (r NB + b).
+//   K word (j, lane, b): token 8j + g, dims 32b + 8t .. +7; dim 8t + 2p + e
+//     of the block is nibble p + 4e (p < 4, e < 2).
+//   V word (j, lane, b): tokens 8j + 2t + e, dims 32b + 4g + p; nibble p + 4e
+//     (so a token owns 16-bit halves of its own: appending it writes no
+//     byte of its neighbour).
+//   scale (j, t, b, e): token 8j + 2t + e, block b (binary16).
+// With NB = head_dim / 32 blocks, word (j, lane, b) is at byte
+//   head_dim 128: j * 512 + lane * 16 + b * 4;  head_dim 64: lane * 16 + j * 8 + b * 4
+// and scale (j, t, b, e) at the same formula with t for lane, + e * 2 (and 64
+// for 512).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -26,29 +31,31 @@
 
 namespace te {
 
-constexpr int kKv4Unit = 64;        // tokens of a unit
-constexpr int kKv4Stage = 128;      // tokens of a step of the decode kernel: the M of its matrix products
+constexpr int kKv4Tile = 16;        // tokens of a tile
+constexpr int kKv4UnitTiles = 4;    // tiles of a work unit of the decode split (64 tokens)
+constexpr int kKv4Unit = kKv4Tile * kKv4UnitTiles;
 constexpr int kKv4Heads = 8;        // query heads of a work group (larger groups take several)
 constexpr int kKv4MaxSeqs = 64;     // sequences per decode launch
 
-__host__ __device__ constexpr int kv4_unit_bytes(int hd) { return 72 * hd; }
-__host__ __device__ constexpr int kv4_v_off(int hd) { return 32 * hd; }
-__host__ __device__ constexpr int kv4_ks_off(int hd) { return 64 * hd; }
-__host__ __device__ constexpr int kv4_vs_off(int hd) { return 68 * hd; }
-// Byte of K word (r, b, t), of V word (d, y) and of scale (r, b) in their parts.
-__host__ __device__ constexpr int kv4_k_word(int r, int b, int t) { return (64 * b + r) * 16 + 4 * t; }
-__host__ __device__ constexpr int kv4_v_word(int hd, int d, int y) { return ((y >> 2) * hd + d) * 16 + 4 * (y & 3); }
-__host__ __device__ constexpr int kv4_scale(int hd, int r, int b) { return 2 * (r * (hd / 32) + b); }
-// Nibble of code i (0..7) in its word.
-__host__ __device__ constexpr int kv4_nibble(int i) { return (i >> 1) + 4 * (i & 1); }
+__host__ __device__ constexpr int kv4_code_bytes(int hd) { return 8 * hd; }   // one side's codes of a tile
+__host__ __device__ constexpr int kv4_scale_bytes(int hd) { return hd; }      // one side's scales of a tile
+__host__ __device__ constexpr int kv4_tile_bytes(int hd) { return 18 * hd; }
+// Byte of word (j, lane, b) in a side's codes, and of scale (j, t, b, e) in its scales.
+__host__ __device__ constexpr int kv4_word_at(int hd, int j, int lane, int b) {
+  return hd == 128 ? j * 512 + lane * 16 + b * 4 : lane * 16 + j * 8 + b * 4;
+}
+__host__ __device__ constexpr int kv4_scale_at(int hd, int j, int t, int b, int e) {
+  return (hd == 128 ? j * 64 + t * 16 + b * 4 : t * 16 + j * 8 + b * 4) + e * 2;
+}
 
-// Where a cache's units are.
+// Where a cache's tiles are.
 struct Kv4Pool {
   unsigned char* base;
   int32_t num_pages;        // pages per layer
   int32_t kv_heads;
-  int32_t units_per_page;
-  uint32_t upp_magic;       // ceil(2^32 / units_per_page), or 0 for one unit per page
+  int32_t tiles_per_page;
+  uint32_t tpp_magic;       // ceil(2^32 / tiles_per_page)
+  int32_t page_tokens;
 };
 
 struct Kv4Seq {
@@ -56,12 +63,10 @@ struct Kv4Seq {
   int32_t len;         // tokens cached before the call
   int32_t q_pos;       // RoPE position of the query
   int32_t new_pos;     // RoPE position of the appended token
-  int32_t stage_begin; // first stage of this sequence within a (layer, kv head, head block)
-  int32_t part_begin;  // aligned split: its first part within a (layer, kv head, head block)
+  int32_t unit_begin;  // first work unit of this sequence within a (layer, kv head, head block)
   int32_t page_base;   // >= 0: the sequence's pages are page_base, page_base + 1, ...; -1: read the table
 };
-// Stages of a sequence that attends n tokens (one at least: an empty sequence writes zeros).
-__host__ __device__ inline int kv4_stages(int n) { return n > 0 ? (n + kKv4Stage - 1) / kKv4Stage : 1; }
+__host__ __device__ inline int kv4_units(int len) { return len > 0 ? (len + kKv4Unit - 1) / kKv4Unit : 1; }
 
 struct Kv4DecodeParams {
   Kv4Pool pool;
@@ -70,7 +75,7 @@ struct Kv4DecodeParams {
   const void* k_new;          // [n_layers][n_seqs][kv_heads][hd] or null
   const void* v_new;
   float* out;                 // [..][heads][hd], or partial records [..][heads][hd + 2]
-  float* partials;            // records of split groups: [grid][2][kv4_record_floats] (aligned split: [grid])
+  float* partials;            // records of split groups: [grid][2][kv4_record_floats]
   uint32_t* counters;         // one per group, zero between launches
   const float* rope_cos;      // [max_position][hd / 2]
   const float* rope_sin;
@@ -78,14 +83,13 @@ struct Kv4DecodeParams {
   const float* k_bias;        // null, or [cache layers][kv_heads * hd]
   const float* v_bias;
   int* error;
-  long long total_stages;
+  long long total_units;
   int32_t n_seqs, seq_total, seq_base;
   int32_t layer_begin, n_layers;
   int32_t group;              // query heads per kv head
   int32_t head_blocks;        // work groups per kv head: ceil(group / 8)
   int32_t block_heads;        // query heads of a work group: ceil(group / head_blocks)
-  int32_t block_stages;       // stages of one (layer, kv head, head block)
-  int32_t block_parts;        // aligned split: CTAs of one (layer, kv head, head block); 0: stream split
+  int32_t block_units;        // work units of one (layer, kv head, head block)
   int32_t grid;
   int32_t max_pages_per_seq;
   int32_t rope, input_f16, partial_out;
@@ -96,10 +100,9 @@ static_assert(sizeof(Kv4DecodeParams) <= 4096, "decode parameters exceed the ker
 
 // Record of a part of a split group: 8 heads' accumulators, m and l.
 constexpr int kv4_record_floats(int hd) { return kKv4Heads * hd + 2 * kKv4Heads; }
-// Plans the split of p's work over `slots` resident CTAs (fills the sequences' stages and parts, block_stages,
-// block_parts, total_stages, grid).
-void plan_kv4_decode(Kv4DecodeParams& p, long long slots);
-int kv4_decode_ctas_per_sm(int head_dim);
+// Plans the split of p's work over at most max_grid CTAs (fills unit_begin, block_units, total_units, grid).
+void plan_kv4_decode(Kv4DecodeParams& p, long long max_grid);
+int kv4_decode_ctas_per_sm();
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream_t s);
 
 struct Kv4RowsParams {
