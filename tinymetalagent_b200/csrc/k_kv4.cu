@@ -11,6 +11,13 @@
 #include "te_ptx.cuh"
 #include "te_rope.cuh"
 
+// Decode launch shape.
+#ifndef KV4_WARPS
+#define KV4_WARPS 8
+#define KV4_CTAS 2
+#define KV4_RING 2
+#endif
+
 namespace te {
 namespace {
 
@@ -412,60 +419,92 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // moves it (rescaling O) only when a score exceeds it by more than 2^5.
 template <int HD>
 struct Dec {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = KV4_WARPS, kCtas = KV4_CTAS;
+  static constexpr int kStageTiles = 2;  // tiles of a copy: 32 tokens
   static constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
+  static constexpr int kStageBytes = kStageTiles * TB;
   static constexpr int NB = HD / 32;
-  static constexpr int kRing = HD == 128 ? 5 : 10;  // tiles in flight per warp
-  static constexpr int kItems = NB * 2 * 32;        // float4 items of a warp's O
+  static constexpr int kRing = KV4_RING * (128 / HD);  // stages in flight per warp
+  static constexpr int kItems = NB * 2 * 32;           // float4 items of a warp's O
   static constexpr int ring_off = 0;
-  static constexpr int new_off = kWarps * kRing * TB;
-  static constexpr int red_off = new_off + TB;
+  static constexpr int new_off = kWarps * kRing * kStageBytes;  // a stage for the appended token
+  static constexpr int q_off = new_off + kStageBytes;
+  static constexpr int red_off = q_off + NB * 2 * 512;
   static constexpr int stat_off = red_off + (kWarps / 2) * kItems * 16;
-  static constexpr int bar_off = stat_off + 2 * kWarps * kKv4Heads * 4 + 16;
+  static constexpr int f_off = stat_off + 2 * kWarps * kKv4Heads * 4;
+  static constexpr int flag_off = f_off + kKv4Heads * 4;
+  static constexpr int seg_off = flag_off + 16;        // the current segment, the next, a pending one
+  static constexpr int bar_off = seg_off + 3 * 64;
   static constexpr int smem = bar_off + kWarps * kRing * 8;
 };
-static_assert(Dec<128>::smem <= 115712 && Dec<64>::smem <= 115712, "two CTAs per SM");
+static_assert((Dec<128>::smem + 1024) * Dec<128>::kCtas <= 228 * 1024, "CTAs per SM");
+static_assert((Dec<64>::smem + 1024) * Dec<64>::kCtas <= 228 * 1024, "CTAs per SM");
+
+constexpr int kStageTokens4 = 32;
 
 struct Seg {
-  long long next;      // first unit after the segment
-  int ll, kvh, hb, si;
-  int t0, t1;          // tiles of the sequence in this segment
-  int part, parts;     // this segment's part of its group (parts == 1: all of it)
-  long long c0;        // CTA of the group's first part
-  bool last;           // holds the group's last unit (and so the appended token)
-  long long group_id;
+  int next;            // the CTA's next unit (global index), its end when there is none
+  int ll, kvh, hb, si; // local layer, kv head, head block, sequence
+  int s0, s1;          // stages (32 tokens) of the sequence in this segment
+  int first;           // 1: the CTA's first segment
+  int parts, c0;       // CTAs that share the group, the first of them
+  int gb;              // stream split: the group's first unit (global index)
+  int last;            // 1: holds the group's last unit (and so the appended token)
+  int group_id;
 };
 
-// The CTA whose range [b T / G, (b + 1) T / G) holds unit u.
-__device__ __forceinline__ long long kv4_cta_of(long long u, long long total, long long grid) {
-  return div_nonneg((u + 1) * grid - 1, total);
+static_assert(sizeof(Seg) <= 64, "segments in shared memory");
+
+// Stream split: the CTA whose range [b T / G, (b + 1) T / G) holds unit u.
+__device__ __forceinline__ int kv4_cta_of(int u, long long total, int grid) {
+  return (int)div_nonneg((long long)(u + 1) * grid - 1, total);
 }
 
-__device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, long long u, long long u1) {
+// The segment of this CTA that begins at u (stream split), or its only one (aligned split).
+__device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u_begin, int u1) {
   Seg s;
-  const long long blk = div_nonneg(u, p.block_units);
-  const int rem = (int)(u - blk * p.block_units);
+  const bool aligned = p.block_parts != 0;
+  const int per = aligned ? p.block_parts : p.block_units;
+  const int at = aligned ? (int)blockIdx.x : u;
+  const uint32_t blk = (uint32_t)at / (uint32_t)per;
+  const int rem = at - (int)blk * per;
   int lo = 0, hi = p.n_seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.seqs[mid].unit_begin <= rem) lo = mid; else hi = mid - 1;
+    const int begin = aligned ? p.seqs[mid].part_begin : p.seqs[mid].unit_begin;
+    if (begin <= rem) lo = mid; else hi = mid - 1;
   }
   s.si = lo;
   const int len = p.seqs[lo].len;
-  const long long gb = blk * p.block_units + p.seqs[lo].unit_begin;
-  const long long ge = gb + kv4_units(len);
-  s.next = ge < u1 ? ge : u1;
-  s.t0 = (int)(u - gb) * kKv4UnitTiles;
-  s.t1 = min((int)(s.next - gb) * kKv4UnitTiles, (len + kKv4Tile - 1) / kKv4Tile);
-  s.last = s.next == ge;
-  const uint32_t lk = (uint32_t)blk / (uint32_t)p.head_blocks;
-  s.hb = (int)((uint32_t)blk - lk * (uint32_t)p.head_blocks);
+  const int n = kv4_units(len);
+  int a, b;  // units of the sequence in this segment
+  if (aligned) {
+    const int part = rem - p.seqs[lo].part_begin;
+    s.parts = (lo + 1 < p.n_seqs ? p.seqs[lo + 1].part_begin : per) - p.seqs[lo].part_begin;
+    s.c0 = (int)blockIdx.x - part;
+    a = (int)div_nonneg((long long)part * n, s.parts);
+    b = (int)div_nonneg((long long)(part + 1) * n, s.parts);
+    s.gb = 0;
+    s.next = u1;
+    s.first = 1;
+  } else {
+    s.gb = (int)blk * per + p.seqs[lo].unit_begin;
+    s.next = min(s.gb + n, u1);
+    a = u - s.gb;
+    b = s.next - s.gb;
+    s.c0 = kv4_cta_of(s.gb, p.total_units, p.grid);
+    s.parts = kv4_cta_of(s.gb + n - 1, p.total_units, p.grid) - s.c0 + 1;
+    s.first = u == u_begin;
+  }
+  constexpr int kUnitStages = kKv4Unit / kStageTokens4;
+  s.s0 = a * kUnitStages;
+  s.s1 = min(b * kUnitStages, (len + kStageTokens4 - 1) / kStageTokens4);
+  s.last = b == n;
+  const uint32_t lk = blk / (uint32_t)p.head_blocks;
+  s.hb = (int)(blk - lk * (uint32_t)p.head_blocks);
   s.ll = (int)(lk / (uint32_t)p.pool.kv_heads);
   s.kvh = (int)lk - s.ll * p.pool.kv_heads;
-  s.c0 = kv4_cta_of(gb, p.total_units, p.grid);
-  s.parts = (int)(kv4_cta_of(ge - 1, p.total_units, p.grid) - s.c0) + 1;
-  s.part = (int)(blockIdx.x - s.c0);
-  s.group_id = blk * p.n_seqs + lo;
+  s.group_id = (int)blk * p.n_seqs + lo;
   return s;
 }
 
@@ -474,17 +513,28 @@ __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// (x & m) | o as one operation: o comes in a register, since an instruction holds one immediate.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(m), "r"(o));
+  return d;
+}
+__device__ __forceinline__ uint32_t code_magic() {  // opaque to the compiler, so that it stays in a register
+  uint32_t m;
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m));
+  return m;
+}
 // The four f16 pairs of a word: c - 8, and 16 (c - 8) for the upper nibbles, exactly: a code under the exponent
 // of 1024 is 1024 + c (or + 16 c), and one subtraction leaves a normal number.  Codes read as f16 subnormals
 // would need no subtraction for the keys, but the tensor core aligns the 16 products of a step by their
 // operands' nominal exponents: subnormals lose 7 to 10 bits of the fp32 sum (measured: the output was 8e-6
 // off, against 1e-6 now).
-__device__ __forceinline__ void centred(uint32_t x, uint32_t (&c)[4]) {
+__device__ __forceinline__ void centred(uint32_t x, uint32_t magic, uint32_t (&c)[4]) {
   const uint32_t y = x >> 8;
-  c[0] = h2_add((x & 0x000f000fu) | 0x64006400u, 0xe408e408u);
-  c[1] = h2_add((x & 0x00f000f0u) | 0x64006400u, 0xe480e480u);
-  c[2] = h2_add((y & 0x000f000fu) | 0x64006400u, 0xe408e408u);
-  c[3] = h2_add((y & 0x00f000f0u) | 0x64006400u, 0xe480e480u);
+  c[0] = h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u);
+  c[1] = h2_add(and_or(x, 0x00f000f0u, magic), 0xe480e480u);
+  c[2] = h2_add(and_or(y, 0x000f000fu, magic), 0xe408e408u);
+  c[3] = h2_add(and_or(y, 0x00f000f0u, magic), 0xe480e480u);
 }
 __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -495,6 +545,23 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
+}
+// a b - c in f16x2, one rounding.
+__device__ __forceinline__ uint32_t h2_fms(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// D = A B (+ D), m16n8k16, f16 operands, f32 accumulators.
+__device__ __forceinline__ void mma_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t h2_maxabs(uint32_t a, uint32_t b) {
   const __half2 x = __habs2(*reinterpret_cast<const __half2*>(&a));
@@ -508,12 +575,10 @@ __device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_u
 
 template <int HD>
 struct WarpState {
-  static constexpr int NB = HD / 32;
-  uint32_t qa[NB][2][4];  // A fragments of the queries: block, k16 step
   float f;                // S f = score in exp2 units
-  float o[NB][2][4];      // O^T accumulators: block, m16 tile
+  float o[HD / 32][2][4];    // O^T accumulators: block, m16 tile
   float m, l;             // reference exponent and sum of this lane's weights, head g
-  float mb;               // 8 - m
+  float mb;               // kWeightExp - m
   float vlim;             // largest |V scale| the current vexp allows
   uint32_t vmul;          // 2^vexp twice, f16
   int vexp;
@@ -522,68 +587,54 @@ struct WarpState {
 constexpr float kSlack = 5.f;      // scores may exceed the reference by this before it moves
 constexpr float kWeightExp = 8.f;  // weights are 2^(score - m + 8): at most 2^13, exact products far above f16's floor
 
-// Queries of the segment's heads as A fragments, scaled per head by a power of two (largest value in [2^11, 2^12)).
+// A query head's raw row, 4 dims a lane (lanes 0-15 at head_dim 64); zeros for a head the group has not.
 template <int HD>
-__device__ __forceinline__ void load_queries(const Kv4DecodeParams& p, const Seg& s, int lane, WarpState<HD>& w) {
-  constexpr int NB = HD / 32;
-  const int g = lane >> 2, t = lane & 3;
-  const int heads = p.pool.kv_heads * p.group;
-  const int hg = s.hb * p.block_heads + g;  // head within the kv head's group
-  const bool have = g < p.block_heads && hg < p.group;
-  float v[NB][8];
-  if (have) {
-    const int head = s.kvh * p.group + hg;
-    const size_t row = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * heads + head) * HD;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) load8(p.q, row + 32 * b + 8 * t, p.input_f16, v[b]);
-    if (p.q_bias) {
-      const float* br = p.q_bias + ((size_t)(p.layer_begin + s.ll) * heads + head) * HD;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) add_bias8(v[b], br + 32 * b + 8 * t);
-    }
-    if (p.rope) {
-      const float* cr = p.rope_cos + (size_t)p.seqs[s.si].q_pos * (HD / 2);
-      const float* sr = p.rope_sin + (size_t)p.seqs[s.si].q_pos * (HD / 2);
-#pragma unroll
-      for (int b = 0; b < NB / 2; ++b) rope8(v[b], v[b + NB / 2], cr, sr, 32 * b + 8 * t);
-    }
-  } else {
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
+__device__ __forceinline__ void fetch_query(const Kv4DecodeParams& p, const Seg& s, int h, int lane, float (&v)[4]) {
+  const int hg = s.hb * p.block_heads + h;
+  v[0] = v[1] = v[2] = v[3] = 0.f;
+  if (h < p.block_heads && hg < p.group && lane < HD / 4) {
+    const size_t row = ((size_t)s.ll * p.seq_total + p.seq_base + s.si) * (p.pool.kv_heads * p.group) +
+                       s.kvh * p.group + hg;
+    load4(p.q, row * HD + 4 * lane, p.input_f16, v);
   }
-  float top = 0.f;
+}
+
+// Bias, RoPE, the head's power of two (largest value in [2^11, 2^12)) and the f16 hi / lo split: writes the row's
+// part of the A fragments (lane 4h + t of block b, step st: {hi, lo, hi / 16, lo / 16} of 4 dims -- the codes of
+// the second pair come as 16 c) and the factor that turns S into exp2 units.
+template <int HD>
+__device__ __forceinline__ void stage_query(const Kv4DecodeParams& p, const Seg& s, int h, int lane, float (&v)[4],
+                                            unsigned char* qf, float* f) {
+  const int hg = s.hb * p.block_heads + h;
+  const bool have = h < p.block_heads && hg < p.group;
+  if (have && p.q_bias && lane < HD / 4) {
+    add_bias4(v, p.q_bias + ((size_t)(p.layer_begin + s.ll) * (p.pool.kv_heads * p.group) + s.kvh * p.group + hg) * HD +
+                     4 * lane);
+  }
+  if (p.rope) {
+    rope4<HD>(v, p.rope_cos + (size_t)p.seqs[s.si].q_pos * (HD / 2), p.rope_sin + (size_t)p.seqs[s.si].q_pos * (HD / 2),
+              lane);
+  }
+  float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[b][i]));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  for (int off = 1; off < HD / 4; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   const int k = top > 0.f ? min(max(11 - exponent_of(top), -100), 126) : 0;
   const float sc = pow2i(k);
-  w.f = p.scale_log2 * pow2i(-k);
+  if (lane == 0) f[h] = p.scale_log2 * pow2i(-k);
+  uint32_t w[4];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      uint32_t hi[2], lo[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        // the nibbles of the second pair of a step read 16 c: its queries enter divided by 16
-        const float mul = r ? 0.0625f : 1.f;
-        const float x = v[b][4 * st + 2 * r] * sc * mul, y = v[b][4 * st + 2 * r + 1] * sc * mul;
-        const __half2 h = __floats2half2_rn(x, y);
-        const float2 hf = __half22float2(h);
-        const __half2 q = __floats2half2_rn(x - hf.x, y - hf.y);
-        hi[r] = *reinterpret_cast<const uint32_t*>(&h);
-        lo[r] = *reinterpret_cast<const uint32_t*>(&q);
-      }
-      w.qa[b][st][0] = hi[0];
-      w.qa[b][st][1] = lo[0];
-      w.qa[b][st][2] = hi[1];
-      w.qa[b][st][3] = lo[1];
-    }
+  for (int r = 0; r < 2; ++r) {
+    const float mul = r ? 0.0625f : 1.f;
+    const float x = v[2 * r] * sc * mul, y = v[2 * r + 1] * sc * mul;
+    const __half2 hi = __floats2half2_rn(x, y);
+    const float2 hf = __half22float2(hi);
+    w[2 * r] = *reinterpret_cast<const uint32_t*>(&hi);
+    w[2 * r + 1] = pack_half2(x - hf.x, y - hf.y);
+  }
+  // dims 4 lane .. + 3: block lane / 8, lane t = (lane % 8) / 2 of the fragment, step lane % 2
+  if (lane < HD / 4) {
+    *reinterpret_cast<uint4*>(qf + ((lane >> 3) * 2 + (lane & 1)) * 512 + (4 * h + ((lane & 7) >> 1)) * 16) =
+        make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -631,54 +682,80 @@ __device__ __forceinline__ void lds_scales(uint32_t addr, int t, uint32_t (&w)[2
   }
 }
 
-// Attends the first `valid` (1..16) tokens of the tile at shared address `addr`.
-template <int HD>
-__device__ __forceinline__ void attend_tile(uint32_t addr, int valid, int lane, WarpState<HD>& w) {
+// Attends the first `valid` tokens of T consecutive tiles at shared address `addr`; the queries' A fragments are
+// at shared address `qf` (read again for each stage: 32 registers less in every warp, so that more warps fit).
+template <int HD, int T>
+__device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, int lane, uint32_t magic,
+                                       WarpState<HD>& w) {
   using D = Dec<HD>;
   constexpr int NB = D::NB;
   const int t = lane & 3;
-  uint32_t kw[2][NB], ks[2][NB], vs[2][NB];
-  lds_words<HD>(addr, lane, kw);
-  lds_scales<HD>(addr + 2 * D::CB, t, ks);
-  lds_scales<HD>(addr + 2 * D::CB + D::SB, t, vs);
-
-  // scores: s[j] = tokens 8j + 2t, 8j + 2t + 1 of head g
-  uint64_t s2[2];
+  // s[i][2j + r]: tile i, token 8j + 2t + r, head g
+  float s[T][4];
+  {
+    uint32_t kw[T][2][NB], ks[T][2][NB];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    s2[j] = 0;
+    for (int i = 0; i < T; ++i) {
+      lds_words<HD>(addr + i * D::TB, lane, kw[i]);
+      lds_scales<HD>(addr + i * D::TB + 2 * D::CB, t, ks[i]);
+    }
+    uint64_t s2[T][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      uint32_t c[4];
-      centred(kw[j][b], c);
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_16816(acc, w.qa[b][0], c[0], c[1]);
-      mma_16816(acc, w.qa[b][1], c[2], c[3]);
-      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ks[j][b]));
-      const uint64_t d2 = f2_pack(d.x, d.y);
-      s2[j] = f2_fma(d2, f2_pack(acc[0], acc[1]), s2[j]);
-      s2[j] = f2_fma(d2, f2_pack(acc[2], acc[3]), s2[j]);
-    }
-  }
-  float s[4];
-  f2_unpack(s2[0], s[0], s[1]);
-  f2_unpack(s2[1], s[2], s[3]);
-  if (valid < kKv4Tile) {  // tokens past the sequence: no weight, whatever the tile holds there
+      uint32_t qa[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = 8 * (i >> 1) + 2 * t + (i & 1) < valid;
-      if (!in) {
-        s[i] = -INFINITY;
-        const uint32_t keep = (i & 1) ? 0x0000ffffu : 0xffff0000u;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) vs[i >> 1][b] &= keep;
+      for (int st = 0; st < 2; ++st) {
+        const uint4 x = lds128(qf + (b * 2 + st) * 512 + lane * 16);
+        qa[st][0] = x.x; qa[st][1] = x.y; qa[st][2] = x.z; qa[st][3] = x.w;
       }
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t c[4];
+          centred(kw[i][j][b], magic, c);
+          float acc[4];
+          mma_zero(acc, qa[0], c[0], c[1]);
+          mma_add(acc, qa[1], c[2], c[3]);
+          const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ks[i][j][b]));
+          const uint64_t d2 = f2_pack(d.x, d.y);
+          s2[i][j] = b == 0 ? f2_mul(d2, f2_pack(acc[0], acc[1])) : f2_fma(d2, f2_pack(acc[0], acc[1]), s2[i][j]);
+          s2[i][j] = f2_fma(d2, f2_pack(acc[2], acc[3]), s2[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      f2_unpack(s2[i][0], s[i][0], s[i][1]);
+      f2_unpack(s2[i][1], s[i][2], s[i][3]);
     }
   }
-  const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * w.f;
-  uint32_t vm = h2_maxabs(vs[0][0], vs[1][0]);
+  uint32_t vs[T][2][NB];
 #pragma unroll
-  for (int b = 1; b < NB; ++b) vm = h2_maxabs(vm, h2_maxabs(vs[0][b], vs[1][b]));
+  for (int i = 0; i < T; ++i) lds_scales<HD>(addr + i * D::TB + 2 * D::CB + D::SB, t, vs[i]);
+  if (valid < kKv4Tile * T) {  // tokens past the sequence: no weight, whatever the tile holds there
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (kKv4Tile * i + 8 * (r >> 1) + 2 * t + (r & 1) >= valid) {
+          s[i][r] = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) vs[i][r >> 1][b] &= (r & 1) ? 0x0000ffffu : 0xffff0000u;
+        }
+      }
+  }
+  float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+  uint32_t vm = h2_maxabs(vs[0][0][0], vs[0][1][0]);
+#pragma unroll
+  for (int i = 0; i < T; ++i) {
+    if (i > 0) {
+      top = fmaxf(fmaxf(top, fmaxf(s[i][0], s[i][1])), fmaxf(s[i][2], s[i][3]));
+      vm = h2_maxabs(vm, h2_maxabs(vs[i][0][0], vs[i][1][0]));
+    }
+#pragma unroll
+    for (int b = 1; b < NB; ++b) vm = h2_maxabs(vm, h2_maxabs(vs[i][0][b], vs[i][1][b]));
+  }
+  top *= w.f;
   const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
   const float vtop = fmaxf(vmf.x, vmf.y);
   if (__any_sync(0xffffffffu, top > w.m + kSlack || vtop > w.vlim)) {
@@ -715,117 +792,200 @@ __device__ __forceinline__ void attend_tile(uint32_t addr, int valid, int lane, 
         w.o[b][i][3] *= a1;
       }
   }
-  float pr[4];
+  uint32_t ph[T][2], pl[T][2], vw[T][2][NB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) pr[i] = ex2(fmaf(s[i], w.f, w.mb));
-  w.l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-  uint32_t ph[2], pl[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const __half2 h = __floats2half2_rn(pr[2 * j], pr[2 * j + 1]);
-    const float2 hf = __half22float2(h);
-    ph[j] = *reinterpret_cast<const uint32_t*>(&h);
-    pl[j] = pack_half2(pr[2 * j] - hf.x, pr[2 * j + 1] - hf.y);
-  }
-
-  uint32_t vw[2][NB];
-  lds_words<HD>(addr + D::CB, lane, vw);
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    uint32_t hi[2], lo[2];
+  for (int i = 0; i < T; ++i) {
+    lds_words<HD>(addr + i * D::TB + D::CB, lane, vw[i]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint32_t d = h2_mul(vs[j][b], w.vmul);
-      hi[j] = h2_mul(ph[j], d);
-      lo[j] = h2_fma(pl[j], d, h2_fma(ph[j], d, hi[j] ^ 0x80008000u));
+      const float p0 = ex2(fmaf(s[i][2 * j], w.f, w.mb)), p1 = ex2(fmaf(s[i][2 * j + 1], w.f, w.mb));
+      w.l += p0 + p1;
+      const __half2 h = __floats2half2_rn(p0, p1);
+      const float2 hf = __half22float2(h);
+      ph[i][j] = *reinterpret_cast<const uint32_t*>(&h);
+      pl[i][j] = pack_half2(p0 - hf.x, p1 - hf.y);
     }
-    uint32_t c0[4], c1[4];
-    centred(vw[0][b], c0);
-    centred(vw[1][b], c1);
-    const uint32_t a[4] = {c0[0], c0[1], c1[0], c1[1]}, c[4] = {c0[2], c0[3], c1[2], c1[3]};
-    mma_16816(w.o[b][0], a, hi[0], hi[1]);
-    mma_16816(w.o[b][1], c, hi[0], hi[1]);
-    mma_16816(w.o[b][0], a, lo[0], lo[1]);
-    mma_16816(w.o[b][1], c, lo[0], lo[1]);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    // the tiles' products start from zero and join O by a rounded fp32 addition: a long accumulation inside
+    // the tensor core truncates at every step
+    float o0[4], o1[4];
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t d = h2_mul(vs[i][j][b], w.vmul);
+        hi[j] = h2_mul(ph[i][j], d);
+        lo[j] = h2_fma(pl[i][j], d, h2_fms(ph[i][j], d, hi[j]));
+      }
+      uint32_t c0[4], c1[4];
+      centred(vw[i][0][b], magic, c0);
+      centred(vw[i][1][b], magic, c1);
+      const uint32_t a[4] = {c0[0], c0[1], c1[0], c1[1]}, c[4] = {c0[2], c0[3], c1[2], c1[3]};
+      if (i == 0) {
+        mma_zero(o0, a, lo[0], lo[1]);
+        mma_zero(o1, c, lo[0], lo[1]);
+      } else {
+        mma_add(o0, a, lo[0], lo[1]);
+        mma_add(o1, c, lo[0], lo[1]);
+      }
+      mma_add(o0, a, hi[0], hi[1]);
+      mma_add(o1, c, hi[0], hi[1]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      f2_unpack(f2_add(f2_pack(w.o[b][0][r], w.o[b][0][r + 1]), f2_pack(o0[r], o0[r + 1])), w.o[b][0][r],
+                w.o[b][0][r + 1]);
+      f2_unpack(f2_add(f2_pack(w.o[b][1][r], w.o[b][1][r + 1]), f2_pack(o1[r], o1[r + 1])), w.o[b][1][r],
+                w.o[b][1][r + 1]);
+    }
   }
 }
 
-// A warp's copies: tiles t0 + warp, + 8, ... of each segment of the CTA's range, in order, across segments.
+// A warp's copies: stages s0 + warp, + kWarps, ... of each segment of the CTA's range, in order, across segments.
 struct Feed {
-  long long u, u1;      // next segment's first unit, end of the CTA's range
-  int tile, t1;         // next tile and end of the current segment
-  const unsigned char* base;  // tile 0 of page 0 for the segment's layer and kv head
+  int u, u0, u1;              // next segment's first unit, the CTA's range
+  int stage, s1;              // next stage and end of the current segment
+  int page, in;               // the next stage's page and stage within it
+  const unsigned char* base;  // page 0 of the segment's layer, at its kv head
+  const unsigned char* at;    // the current page, at its kv head
   const int32_t* row;
   int page_base;
 };
 
 template <int HD>
 __device__ __forceinline__ const unsigned char* feed_next(const Kv4DecodeParams& p, Feed& f, int warp) {
-  while (f.tile >= f.t1) {
+  using D = Dec<HD>;
+  const int spp = p.pool.tiles_per_page / D::kStageTiles;
+  bool moved = f.in >= spp;
+  while (f.stage >= f.s1) {
     if (f.u >= f.u1) return nullptr;
-    const Seg s = kv4_seg_at(p, f.u, f.u1);
+    const Seg s = kv4_seg_at(p, f.u, f.u0, f.u1);
     f.u = s.next;
-    f.tile = s.t0 + warp;
-    f.t1 = s.t1;
+    f.stage = s.s0 + warp;
+    f.s1 = s.s1;
     const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
-    f.base = p.pool.base + rec * p.pool.tiles_per_page * Dec<HD>::TB;
+    f.base = p.pool.base + rec * p.pool.tiles_per_page * D::TB;
     f.row = p.page_table + (size_t)p.seqs[s.si].slot * p.max_pages_per_seq;
     f.page_base = p.seqs[s.si].page_base;
+    f.page = kv4_page_of(p.pool, f.stage * D::kStageTiles);
+    f.in = f.stage - f.page * spp;
+    moved = true;
   }
-  const int page = kv4_page_of(p.pool, f.tile);
-  const int in = f.tile - page * p.pool.tiles_per_page;
-  const int id = f.page_base >= 0 ? f.page_base + page : f.row[page];
-  f.tile += Dec<HD>::kWarps;
-  return f.base + ((long long)id * p.pool.kv_heads * p.pool.tiles_per_page + in) * Dec<HD>::TB;
+  if (moved) {
+    while (f.in >= spp) {
+      f.in -= spp;
+      ++f.page;
+    }
+    const int id = f.page_base >= 0 ? f.page_base + f.page : f.row[f.page];
+    f.at = f.base + (long long)id * (p.pool.kv_heads * p.pool.tiles_per_page) * D::TB;
+  }
+  const unsigned char* src = f.at + f.in * D::kStageBytes;
+  f.stage += D::kWarps;
+  f.in += D::kWarps;
+  return src;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(32 * Dec<HD>::kWarps, 2) kv4_decode_kernel(const __grid_constant__ Kv4DecodeParams p) {
+__global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
+    kv4_decode_kernel(const __grid_constant__ Kv4DecodeParams p) {
   using D = Dec<HD>;
-  constexpr int NB = D::NB, W = D::kWarps, H = kKv4Heads;
+  constexpr int NB = D::NB, W = D::kWarps, H = kKv4Heads, HW = W / 2;
+  constexpr int rec = kv4_record_floats(HD);
+  static_assert(W % 2 == 0, "the merge pairs warps");
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + D::bar_off) + warp * D::kRing;
-  unsigned char* ring = smem + D::ring_off + warp * D::kRing * D::TB;
-  unsigned char* new_tile = smem + D::new_off;
+  unsigned char* ring = smem + D::ring_off + warp * D::kRing * D::kStageBytes;
+  unsigned char* new_stage = smem + D::new_off;
+  unsigned char* qf = smem + D::q_off;
   float4* red = reinterpret_cast<float4*>(smem + D::red_off);
   float* sm_m = reinterpret_cast<float*>(smem + D::stat_off);  // [W][8]
   float* sm_l = sm_m + W * H;
-  int* sm_flag = reinterpret_cast<int*>(sm_l + W * H);
+  float* sm_f = reinterpret_cast<float*>(smem + D::f_off);
+  int* sm_flag = reinterpret_cast<int*>(smem + D::flag_off);
+  auto seg = [&](int i) -> Seg& { return *reinterpret_cast<Seg*>(smem + D::seg_off + 64 * i); };
 
+  // Launched as a programmatic dependent: up to griddep_wait the previous kernel may still run, and nothing here
+  // touches global memory.
   if (lane == 0) {
     for (int i = 0; i < D::kRing; ++i) mbar_init(&bars[i], 1);
     fence_mbarrier_init();
     fence_proxy_async_shared();
   }
   __syncwarp();
-
-  const long long u1 = stage_start(blockIdx.x + 1, p.total_units, p.grid);
-  long long u = stage_start(blockIdx.x, p.total_units, p.grid);
-  const long long u_begin = u;
-  Feed feed{u, u1, 0, 0, nullptr, nullptr, -1};
+  const bool aligned = p.block_parts != 0;
+  const int u_begin = aligned ? 0 : (int)stage_start(blockIdx.x, p.total_units, p.grid);
+  const int u1 = aligned ? 1 : (int)stage_start(blockIdx.x + 1, p.total_units, p.grid);
+  if (threadIdx.x == 0) seg(0) = kv4_seg_at(p, u_begin, u_begin, u1);
+  Feed feed{};
+  feed.u = feed.u0 = u_begin;
+  feed.u1 = u1;
   auto issue = [&](int slot) {
     const unsigned char* src = feed_next<HD>(p, feed, warp);
     if (src && lane == 0) {
-      mbar_arrive_expect_tx(&bars[slot], D::TB);
-      bulk_load(ring + slot * D::TB, src, D::TB, &bars[slot]);
+      mbar_arrive_expect_tx(&bars[slot], D::kStageBytes);
+      bulk_load(ring + slot * D::kStageBytes, src, D::kStageBytes, &bars[slot]);
     }
     return src != nullptr;
   };
-  int issued = 0, used = 0;      // tiles copied / consumed by this warp
+  griddep_launch_dependents();
+  griddep_wait();
+  __syncthreads();
+
+  constexpr int kRows = (H + W - 1) / W;  // query heads a warp prepares
+  float qr[kRows][4];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) fetch_query<HD>(p, seg(0), warp + i * W, lane, qr[i]);
+  int issued = 0, used = 0;  // stages copied / consumed by this warp
+  int slot = 0;
+  uint32_t phase = 0;
   for (int i = 0; i < D::kRing; ++i) issued += issue(i) ? 1 : 0;
-  bool ok = true;                // false: a wait ran out; the warp computes no more
+  bool ok = true;            // false: a wait ran out; the warp computes no more
+  const uint32_t magic = code_magic();
+  int n_pending = 0;         // segments of this CTA that are parts of shared groups
+  int at_seg = 0;            // seg(at_seg): the current segment
+
+  auto part_weight = [](float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); };
+  // item i of an output: block i / 64, heads 2 (i % 4) + (i / 32) % 2, dims 4 ((i % 32) / 4) .. + 3 of the block
+  auto write_out = [&](const Seg& q, int head, int dim, const float4& acc, float top, float sum) {
+    const int hg = q.hb * p.block_heads + head;
+    if (head >= p.block_heads || hg >= p.group) return;
+    const size_t row =
+        ((size_t)q.ll * p.seq_total + p.seq_base + q.si) * (p.pool.kv_heads * p.group) + q.kvh * p.group + hg;
+    if (p.partial_out) {
+      constexpr float k = 0x1p-8f;  // 2^-kWeightExp
+      float* o = p.out + row * (HD + 2);
+      o[dim] = acc.x * k;
+      o[dim + 1] = acc.y * k;
+      o[dim + 2] = acc.z * k;
+      o[dim + 3] = acc.w * k;
+      if (dim == 0) {
+        o[HD] = top;
+        o[HD + 1] = sum * k;
+      }
+    } else {
+      const float r = sum == 0.f ? 0.f : 1.f / sum;  // no token at all: zeros
+      *reinterpret_cast<float4*>(p.out + row * HD + dim) = make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r);
+    }
+  };
 
   WarpState<HD> w;
-  while (u < u1) {
-    const Seg s = kv4_seg_at(p, u, u1);
+  while (true) {
+    const Seg& s = seg(at_seg);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (warp + i * W < H) stage_query<HD>(p, s, warp + i * W, lane, qr[i], qf, sm_f);
+    }
     const Kv4Seq& sq = p.seqs[s.si];
-    const bool append = p.k_new != nullptr && s.last;
-    const int n_tiles = s.t1 - s.t0;
-    const bool appender = append && warp == n_tiles % W;
+    const int len = sq.len;
+    const int n_stages = s.s1 - s.s0;
+    const bool appender = p.k_new != nullptr && s.last && warp == n_stages % W;
     if (appender) {
-      // the new token: quantised into the cache (by the first head block) and into a tile of its own here
+      // the new token: quantised into the cache (by the first head block) and into a stage of its own here
       const size_t at = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * p.pool.kv_heads + s.kvh) * HD;
       const size_t brow = ((size_t)(p.layer_begin + s.ll) * p.pool.kv_heads + s.kvh) * HD;
       float k[4], v[4];
@@ -834,30 +994,45 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, 2) kv4_decode_kernel(con
                    p.rope ? p.rope_cos + (size_t)sq.new_pos * (HD / 2) : nullptr,
                    p.rope ? p.rope_sin + (size_t)sq.new_pos * (HD / 2) : nullptr, lane, k, v);
       float k2[4] = {k[0], k[1], k[2], k[3]}, v2[4] = {v[0], v[1], v[2], v[3]};
-      store_row<HD>(new_tile, 0, lane, k, v);
+      store_row<HD>(new_stage, 0, lane, k, v);
       if (s.hb == 0) {
         unsigned char* dst = tile_ptr(p.pool, p.page_table + (size_t)sq.slot * p.max_pages_per_seq, p.layer_begin + s.ll,
-                                      s.kvh, sq.len / kKv4Tile, D::TB);
-        store_row<HD>(dst, sq.len % kKv4Tile, lane, k2, v2);
+                                      s.kvh, len / kKv4Tile, D::TB);
+        store_row<HD>(dst, len % kKv4Tile, lane, k2, v2);
       }
     }
-    load_queries<HD>(p, s, lane, w);
+    __syncthreads();  // the queries (and the new token) are in shared memory
+    w.f = sm_f[g];
     reset_state<HD>(w);
-    for (int tile = s.t0 + warp; tile < s.t1; tile += W) {
-      const int slot = used % D::kRing;
-      if (ok) ok = mbar_wait_warp(&bars[slot], (used / D::kRing) & 1);
-      if (!ok) {
-        if (lane == 0) set_error(p.error, 60);
-        break;
+    // this warp's stages, the appended token's after them
+    int st = s.s0 + warp;
+    bool extra = appender;
+    while (st < s.s1 || extra) {
+      const bool cached = st < s.s1;
+      uint32_t addr = smem_u32(new_stage);
+      int valid = 1;
+      if (cached) {
+        if (ok) ok = mbar_wait_warp(&bars[slot], phase);
+        if (!ok) {
+          if (lane == 0) set_error(p.error, 60);
+          break;
+        }
+        addr = smem_u32(ring + slot * D::kStageBytes);
+        valid = len - st * kStageTokens4;
+      } else {
+        extra = false;
       }
-      attend_tile<HD>(smem_u32(ring + slot * D::TB), min(sq.len - tile * kKv4Tile, kKv4Tile), lane, w);
-      __syncwarp();
-      ++used;
-      issued += issue(slot) ? 1 : 0;
-    }
-    if (appender) {
-      __syncwarp();
-      attend_tile<HD>(smem_u32(new_tile), 1, lane, w);
+      attend<HD, D::kStageTiles>(addr, smem_u32(qf), valid, lane, magic, w);
+      if (cached) {
+        __syncwarp();
+        ++used;
+        issued += issue(slot) ? 1 : 0;
+        if (++slot == D::kRing) {
+          slot = 0;
+          phase ^= 1u;
+        }
+        st += W;
+      }
     }
 
     // merge the warps' states: m and l per head first, then O in two rounds
@@ -869,9 +1044,9 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, 2) kv4_decode_kernel(con
       sm_l[warp * H + g] = l;
     }
     __syncthreads();
-    auto part_weight = [](float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); };
     {
       float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
       for (int i = 0; i < W; ++i) {
         mx0 = fmaxf(mx0, sm_m[i * H + 2 * t]);
         mx1 = fmaxf(mx1, sm_m[i * H + 2 * t + 1]);
@@ -892,114 +1067,133 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, 2) kv4_decode_kernel(con
     auto o_item = [&](int b, int c) {
       return make_float4(w.o[b][0][c], w.o[b][0][2 + c], w.o[b][1][c], w.o[b][1][2 + c]);
     };
-    if (warp >= W / 2) {
+    if (warp >= HW) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) red[(warp - W / 2) * D::kItems + (b * 2 + c) * 32 + lane] = o_item(b, c);
+        for (int c = 0; c < 2; ++c) red[(warp - HW) * D::kItems + (b * 2 + c) * 32 + lane] = o_item(b, c);
     }
     __syncthreads();
-    if (warp < W / 2) {
+    if (warp < HW) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float4* slot = &red[warp * D::kItems + (b * 2 + c) * 32 + lane];
-          const float4 x = *slot, y = o_item(b, c);
-          *slot = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+          float4* sl = &red[warp * D::kItems + (b * 2 + c) * 32 + lane];
+          const float4 x = *sl, y = o_item(b, c);
+          *sl = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
     }
+    const bool more = s.next < u1;
+    if (more && threadIdx.x == 0) seg(at_seg ^ 1) = kv4_seg_at(p, s.next, u_begin, u1);
     __syncthreads();
-    // item i: block i / 64, heads 2 (i % 4) + (i / 32) % 2, dims 4 ((i % 32) / 4) .. + 3 of the block
-    const int i = threadIdx.x;
-    const int head = 2 * (i & 3) + ((i >> 5) & 1);
-    const int dim = 32 * (i >> 6) + 4 * ((i & 31) >> 2);
-    const bool mine = i < D::kItems;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float top = -INFINITY, sum = 0.f;
-    if (mine) {
-      for (int k = 0; k < W / 2; ++k) {
+    if (more) {  // the next segment's query rows on their way
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) fetch_query<HD>(p, seg(at_seg ^ 1), warp + i * W, lane, qr[i]);
+    }
+    // a CTA's first segment uses its slot 0, its last another one: at most two of its segments are parts of groups
+    float* mine = p.partials + ((size_t)blockIdx.x * 2 + (s.first ? 0 : 1)) * rec;
+    for (int i = threadIdx.x; i < D::kItems; i += 32 * W) {
+      const int head = 2 * (i & 3) + ((i >> 5) & 1);
+      const int dim = 32 * (i >> 6) + 4 * ((i & 31) >> 2);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < HW; ++k) {
         const float4 x = red[k * D::kItems + i];
         acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
       }
+#pragma unroll
       for (int k = 0; k < W; ++k) top = fmaxf(top, sm_m[k * H + head]);
+#pragma unroll
       for (int k = 0; k < W; ++k) sum += sm_l[k * H + head] * part_weight(sm_m[k * H + head], top);
-    }
-    bool write = true;
-    if (s.parts > 1) {
-      // publish this part; the last of the group's parts to arrive folds them all, in part order
-      constexpr int rec = kv4_record_floats(HD);
-      // a CTA's first segment uses its slot 0, its last another one: at most two of its segments are parts
-      float* mine_rec = p.partials + ((size_t)blockIdx.x * 2 + (u == u_begin ? 0 : 1)) * rec;
-      if (mine) {
-        reinterpret_cast<float4*>(mine_rec)[i] = acc;
-        if (dim == 0) {
-          mine_rec[H * HD + head] = top;
-          mine_rec[H * HD + H + head] = sum;
-        }
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        __threadfence();
-        const uint32_t old = atomicAdd(&p.counters[s.group_id], 1u);
-        *sm_flag = old == (uint32_t)s.parts - 1u;
-        __threadfence();
-      }
-      __syncthreads();
-      write = *sm_flag != 0;
-      if (write && mine) {
-        // part k is CTA c0 + k's: its first segment unless the CTA's range began before the group
-        const long long gb = u - (long long)(s.t0 / kKv4UnitTiles);
-        auto rec_of = [&](int k) {
-          const long long c = s.c0 + k;
-          const int slot = stage_start(c, p.total_units, p.grid) >= gb ? 0 : 1;
-          return p.partials + ((size_t)c * 2 + slot) * rec;
-        };
-        float all = -INFINITY;
-        for (int k = 0; k < s.parts; ++k) all = fmaxf(all, __ldcg(rec_of(k) + H * HD + head));
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        sum = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < s.parts; ++k) {
-          const float* r = rec_of(k);
-          const float wt = part_weight(__ldcg(r + H * HD + head), all);
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(r) + i);
-          acc.x = fmaf(wt, x.x, acc.x);
-          acc.y = fmaf(wt, x.y, acc.y);
-          acc.z = fmaf(wt, x.z, acc.z);
-          acc.w = fmaf(wt, x.w, acc.w);
-          sum = fmaf(wt, __ldcg(r + H * HD + H + head), sum);
-        }
-        top = all;
-      }
-      if (write && threadIdx.x == 0) p.counters[s.group_id] = 0;
-    }
-    const int hg = s.hb * p.block_heads + head;
-    if (write && mine && head < p.block_heads && hg < p.group) {
-      const size_t row = ((size_t)s.ll * p.seq_total + p.seq_base + s.si) * (p.pool.kv_heads * p.group) +
-                         s.kvh * p.group + hg;
-      if (p.partial_out) {
-        constexpr float k = 0x1p-8f;  // 2^-kWeightExp
-        float* o = p.out + row * (HD + 2);
-        o[dim] = acc.x * k;
-        o[dim + 1] = acc.y * k;
-        o[dim + 2] = acc.z * k;
-        o[dim + 3] = acc.w * k;
-        if (dim == 0) {
-          o[HD] = top;
-          o[HD + 1] = sum * k;
-        }
+      if (s.parts == 1) {
+        write_out(s, head, dim, acc, top, sum);
       } else {
-        const float r = sum == 0.f ? 0.f : 1.f / sum;  // no token at all: zeros
-        *reinterpret_cast<float4*>(p.out + row * HD + dim) = make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r);
+        reinterpret_cast<float4*>(mine)[i] = acc;
+        if (dim == 0) {
+          mine[H * HD + head] = top;
+          mine[H * HD + H + head] = sum;
+        }
       }
     }
-    u = s.next;
-    __syncthreads();  // the merge buffers and the new token's tile are free again
+    if (s.parts > 1) {
+      if (n_pending == 0 && threadIdx.x == 0) seg(2) = s;
+      ++n_pending;
+    }
+    if (!more) break;
+    at_seg ^= 1;
+    __syncthreads();  // the merge buffers, the queries and the new token's stage are free again
+  }
+
+  // Groups shared with other CTAs: the last of a group's CTAs to arrive folds its records, in part order.  Left to
+  // the end, where the records have long been written and no segment of this CTA waits behind a fold.
+  if (n_pending > 0) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      const Seg &a = seg(2), &b = seg(at_seg);
+      sm_flag[0] = atomicAdd(&p.counters[a.group_id], 1u) == (uint32_t)a.parts - 1u;
+      sm_flag[1] = n_pending > 1 && atomicAdd(&p.counters[b.group_id], 1u) == (uint32_t)b.parts - 1u;
+      __threadfence();
+    }
+    __syncthreads();
+    for (int i = 0; i < 2; ++i) {
+      if (sm_flag[i] == 0) continue;
+      const Seg& q = seg(i == 0 ? 2 : at_seg);
+      // part k is CTA c0 + k's: its first segment unless (stream split) its range began before the group
+      auto rec_of = [&](int k) {
+        const int c = q.c0 + k;
+        const int sl = aligned || stage_start(c, p.total_units, p.grid) >= q.gb ? 0 : 1;
+        return p.partials + ((size_t)c * 2 + sl) * rec;
+      };
+      float* wt = reinterpret_cast<float*>(smem);  // [parts][8] m, then weights; [parts][8] l (no copy is in flight)
+      float* tot = sm_m;                           // [8] sums, [8] reference exponents
+      for (int j = threadIdx.x; j < q.parts * 2 * H; j += 32 * W) {
+        const int k = j / (2 * H), e = j - k * 2 * H;
+        wt[(e < H ? 0 : q.parts * H) + k * H + (e & 7)] = __ldcg(rec_of(k) + H * HD + e);
+      }
+      __syncthreads();
+      if (threadIdx.x < H) {
+        float all = -INFINITY, sum = 0.f;
+        for (int k = 0; k < q.parts; ++k) all = fmaxf(all, wt[k * H + threadIdx.x]);
+        for (int k = 0; k < q.parts; ++k) {
+          const float e = part_weight(wt[k * H + threadIdx.x], all);
+          wt[k * H + threadIdx.x] = e;
+          sum = fmaf(e, wt[(q.parts + k) * H + threadIdx.x], sum);
+        }
+        tot[threadIdx.x] = sum;
+        tot[H + threadIdx.x] = all;
+      }
+      __syncthreads();
+      for (int j = threadIdx.x; j < D::kItems; j += 32 * W) {
+        const int head = 2 * (j & 3) + ((j >> 5) & 1);
+        const int dim = 32 * (j >> 6) + 4 * ((j & 31) >> 2);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int k = 0; k < q.parts; ++k) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(rec_of(k)) + j);
+          const float e = wt[k * H + head];
+          acc.x = fmaf(e, x.x, acc.x);
+          acc.y = fmaf(e, x.y, acc.y);
+          acc.z = fmaf(e, x.z, acc.z);
+          acc.w = fmaf(e, x.w, acc.w);
+        }
+        write_out(q, head, dim, acc, tot[H + head], tot[head]);
+      }
+      if (threadIdx.x == 0) p.counters[q.group_id] = 0;
+      __syncthreads();
+    }
   }
   if (!ok) {
     // copies of this warp may still be in flight: let them land before the CTA leaves
-    for (; used < issued; ++used) (void)mbar_wait_warp(&bars[used % D::kRing], (used / D::kRing) & 1);
+    for (; used < issued; ++used) {
+      (void)mbar_wait_warp(&bars[slot], phase);
+      if (++slot == D::kRing) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    }
   }
 }
 
@@ -1008,8 +1202,17 @@ cudaError_t launch_decode_t(const Kv4DecodeParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = set_smem_limit_once(done, reinterpret_cast<const void*>(kv4_decode_kernel<HD>), Dec<HD>::smem);
   if (e != cudaSuccess) return e;
-  kv4_decode_kernel<HD><<<p.grid, 32 * Dec<HD>::kWarps, Dec<HD>::smem, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)p.grid);
+  cfg.blockDim = dim3(32 * Dec<HD>::kWarps);
+  cfg.dynamicSmemBytes = Dec<HD>::smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_decode_kernel<HD>, p);
 }
 
 long long row_items(const Kv4RowsParams& p) {
@@ -1019,18 +1222,43 @@ long long row_items(const Kv4RowsParams& p) {
 
 }  // namespace
 
-int kv4_decode_ctas_per_sm() { return 2; }
+int kv4_decode_ctas_per_sm() { return KV4_CTAS; }
 
-void plan_kv4_decode(Kv4DecodeParams& p, long long max_grid) {
-  int acc = 0;
+void plan_kv4_decode(Kv4DecodeParams& p, long long slots) {
+  const long long reps = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks;
+  int acc = 0, longest = 1;
   for (int i = 0; i < p.n_seqs; ++i) {
+    const int n = kv4_units(p.seqs[i].len);
     p.seqs[i].unit_begin = acc;
-    acc += kv4_units(p.seqs[i].len);
+    acc += n;
+    longest = n > longest ? n : longest;
   }
   p.block_units = acc;
-  p.total_units = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks * acc;
-  const long long want = (p.total_units + 1) / 2;  // 128 tokens a CTA: one tile a warp
-  p.grid = (int32_t)(want < max_grid ? want : max_grid);
+  p.total_units = reps * acc;
+  // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once.
+  auto parts_for = [&](int most) {
+    long long c = 0;
+    for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len) + most - 1) / most;
+    return c * reps;
+  };
+  const long long ideal = (p.total_units + slots - 1) / slots;
+  int lo = 1, hi = longest;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (parts_for(mid) <= slots) hi = mid; else lo = mid + 1;
+  }
+  if (parts_for(lo) <= slots && lo <= ideal + ideal / 8) {
+    int parts = 0;
+    for (int i = 0; i < p.n_seqs; ++i) {
+      p.seqs[i].part_begin = parts;
+      parts += (kv4_units(p.seqs[i].len) + lo - 1) / lo;
+    }
+    p.block_parts = parts;
+    p.grid = (int32_t)(reps * parts);
+    return;
+  }
+  p.block_parts = 0;
+  p.grid = (int32_t)(p.total_units < slots ? p.total_units : slots);
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream_t s) {

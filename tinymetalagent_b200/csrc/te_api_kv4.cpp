@@ -72,7 +72,7 @@ TE_API te_status te_kv4_cache_create(te_attn_engine* e, const te_kv_cache_desc* 
   te_kv_cache_desc d = *desc;
   if (d.page_tokens == 0) d.page_tokens = 128;
   if (d.layers == 0 || d.max_seqs == 0 || d.max_tokens_per_seq == 0 || d.kv_heads == 0 || !(d.rope_theta > 0.0f) ||
-      d.page_tokens % kKv4Unit != 0) {
+      d.page_tokens % kStageTokens != 0) {
     return fail(e, TE_STATUS_INVALID_ARGUMENT, "invalid cache description");
   }
   if (d.head_dim != 64 && d.head_dim != 128) return fail(e, TE_STATUS_UNSUPPORTED, "head_dim must be 64 or 128");

@@ -32,8 +32,7 @@
 namespace te {
 
 constexpr int kKv4Tile = 16;        // tokens of a tile
-constexpr int kKv4UnitTiles = 4;    // tiles of a work unit of the decode split (64 tokens)
-constexpr int kKv4Unit = kKv4Tile * kKv4UnitTiles;
+constexpr int kKv4Unit = 256;       // tokens of a work unit of the decode split: one stage of 32 for each of 8 warps
 constexpr int kKv4Heads = 8;        // query heads of a work group (larger groups take several)
 constexpr int kKv4MaxSeqs = 64;     // sequences per decode launch
 
@@ -64,6 +63,7 @@ struct Kv4Seq {
   int32_t q_pos;       // RoPE position of the query
   int32_t new_pos;     // RoPE position of the appended token
   int32_t unit_begin;  // first work unit of this sequence within a (layer, kv head, head block)
+  int32_t part_begin;  // aligned split: its first part within a (layer, kv head, head block)
   int32_t page_base;   // >= 0: the sequence's pages are page_base, page_base + 1, ...; -1: read the table
 };
 __host__ __device__ inline int kv4_units(int len) { return len > 0 ? (len + kKv4Unit - 1) / kKv4Unit : 1; }
@@ -90,6 +90,7 @@ struct Kv4DecodeParams {
   int32_t head_blocks;        // work groups per kv head: ceil(group / 8)
   int32_t block_heads;        // query heads of a work group: ceil(group / head_blocks)
   int32_t block_units;        // work units of one (layer, kv head, head block)
+  int32_t block_parts;        // aligned split: CTAs of one (layer, kv head, head block); 0: stream split
   int32_t grid;
   int32_t max_pages_per_seq;
   int32_t rope, input_f16, partial_out;
@@ -100,8 +101,9 @@ static_assert(sizeof(Kv4DecodeParams) <= 4096, "decode parameters exceed the ker
 
 // Record of a part of a split group: 8 heads' accumulators, m and l.
 constexpr int kv4_record_floats(int hd) { return kKv4Heads * hd + 2 * kKv4Heads; }
-// Plans the split of p's work over at most max_grid CTAs (fills unit_begin, block_units, total_units, grid).
-void plan_kv4_decode(Kv4DecodeParams& p, long long max_grid);
+// Plans the split of p's work over `slots` resident CTAs (fills the sequences' units and parts, block_units,
+// block_parts, total_units, grid).
+void plan_kv4_decode(Kv4DecodeParams& p, long long slots);
 int kv4_decode_ctas_per_sm();
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream_t s);
 
