@@ -209,22 +209,131 @@ __device__ __forceinline__ unsigned char* tile_ptr(const Kv4Pool& p, const int32
 
 constexpr int kRowWarps = 4;
 
-// One warp per (layer, kv head, tile of 16 tokens): the tile is assembled in
-// shared memory (with the tokens it already holds, if any) and written whole.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float fmin3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// One block in one thread: x becomes c - 8 (fp32), the result is d; q4_quantise's values, without its shuffles.
+//
+// The quotients are correctly rounded by Markstein's step: with y = RN(1 / d), q = RN(x y) and r = x - q d (exact
+// in an fma), RN(q + r y) is RN(x / d); two values at a time that is three packed operations a pair, where a
+// division is some ten instructions a value.  Adding 1.5 2^23 rounds to an integer, half to even.
+__device__ __forceinline__ __half q4_quantise32(float (&x)[32]) {
+  float mx = x[0], mn = x[0];
+#pragma unroll
+  for (int i = 1; i + 1 < 32; i += 2) {
+    mx = fmax3_nan(mx, x[i], x[i + 1]);
+    mn = fmin3_nan(mn, x[i], x[i + 1]);
+  }
+  mx = fmax3_nan(mx, x[31], x[31]);
+  mn = fmin3_nan(mn, x[31], x[31]);
+  float m = mx > -mn ? mx : mn;
+  if (mx == -mn) {  // both signs reach the largest magnitude (or all are zero): the lowest index decides
+    m = x[31];
+#pragma unroll
+    for (int i = 30; i >= 0; --i) {
+      if (fabsf(x[i]) == mx) m = x[i];
+    }
+  }
+  const bool finite = mx < INFINITY && mn > -INFINITY;  // false for NaN too
+  const __half d =
+      finite ? __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.f), 65504.f)) : __ushort_as_half((unsigned short)0x7fff);
+  const float df = __half2float(d);
+  if (!finite || df == 0.f) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = 0.f;
+    return d;
+  }
+  if (fabsf(df) < 0x1p-14f || fabsf(df) == 65504.f) {
+    // subnormal or saturated: quotients may lie far outside the codes' range
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = fminf(fmaxf(rintf(__fdiv_rn(x[i], df)), -8.f), 7.f);
+    return d;
+  }
+  // d is within 2^-11 of m / -8: every quotient rounds to -8 .. 8
+  const float inv = __frcp_rn(df);
+  const uint64_t inv2 = f2_pack(inv, inv), neg2 = f2_pack(-df, -df);
+  constexpr float kMagic = 12582912.f;
+  const uint64_t magic2 = f2_pack(kMagic, kMagic);
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const uint64_t v = f2_pack(x[i], x[i + 1]);
+    const uint64_t q = f2_mul(v, inv2);
+    const uint64_t r = f2_fma(q, neg2, v);
+    float a, b;
+    f2_unpack(f2_sub(f2_add(f2_fma(r, inv2, q), magic2), magic2), a, b);
+    x[i] = fminf(a, 7.f);  // 8 where x is as large as m and of the other sign
+    x[i + 1] = fminf(b, 7.f);
+  }
+  return d;
+}
+
+// Codes i0 .. i0 + 3 as bits 0, s1, s2, s3 and up, from c - 8 in fp32: 2^23 + 8 + (c - 8) holds c in its low bits.
+__device__ __forceinline__ uint32_t q4_bits(const float (&x)[32], int i0, int s1, int s2, int s3) {
+  auto c = [&](int i) { return __float_as_uint(x[i] + 8388616.f) - 0x4b000000u; };
+  return c(i0) + (c(i0 + 1) << s1) + (c(i0 + 2) << s2) + (c(i0 + 3) << s3);
+}
+
+__device__ __forceinline__ void load32(const void* base, size_t idx, int f16, float (&x)[32]) {
+  if (f16) {
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(base) + idx);
+    uint4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[8];
+      unpack8(u[i], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[8 * i + e] = v[e];
+    }
+  } else {
+    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + idx);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 v = p[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  }
+}
+__device__ __forceinline__ void store32(void* base, size_t idx, int f16, const float (&x)[32]) {
+  if (f16) {
+    uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<__half*>(base) + idx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = make_uint4(pack_half2(x[8 * i], x[8 * i + 1]), pack_half2(x[8 * i + 2], x[8 * i + 3]),
+                        pack_half2(x[8 * i + 4], x[8 * i + 5]), pack_half2(x[8 * i + 6], x[8 * i + 7]));
+    }
+  } else {
+    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + idx);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  }
+}
+
+// One warp per (layer, kv head, tile of 16 tokens), one block a lane: the tile is assembled in shared memory (with
+// the tokens it already holds, if the new ones do not fill it) and written whole.
 template <int HD>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
-  constexpr int TB = kv4_tile_bytes(HD);
+  constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
+  constexpr int kTokens = 32 / NB;  // tokens of a warp's step
   __shared__ __align__(16) unsigned char tiles[kRowWarps][TB];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = p.first / kKv4Tile;
-  const int n_tiles = (p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1;
-  const long long items = (long long)n_tiles * p.pool.kv_heads * p.n_layers;
-  const long long item = (long long)blockIdx.x * kRowWarps + warp;
-  if (item >= items) return;
-  const int kvh = (int)(item % p.pool.kv_heads);
-  const long long r = item / p.pool.kv_heads;
-  const int tile = t0 + (int)(r % n_tiles);
+  const uint32_t n_tiles = (uint32_t)((p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1);
+  const uint32_t item = blockIdx.x * kRowWarps + warp;
+  const uint32_t r = item / (uint32_t)p.pool.kv_heads;
+  const int kvh = (int)(item - r * (uint32_t)p.pool.kv_heads);
   const int ll = (int)(r / n_tiles);
+  const int tile = t0 + (int)(r - (uint32_t)ll * n_tiles);
+  if (ll >= p.n_layers) return;
   const int layer = p.layer_begin + ll;
   unsigned char* dst = tile_ptr(p.pool, p.page_row, layer, kvh, tile, TB);
   unsigned char* sm = tiles[warp];
@@ -236,24 +345,73 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
     }
     __syncwarp();
   }
-  const size_t brow = ((size_t)layer * p.pool.kv_heads + kvh) * HD;
-  const float* kb = p.k_bias ? p.k_bias + brow : nullptr;
-  const float* vb = p.v_bias ? p.v_bias + brow : nullptr;
-  using R = RowDims<HD>;
-#pragma unroll 4
-  for (int i = lo; i < hi; ++i) {
-    const int tok = tile * kKv4Tile + i - p.first;  // index among the new tokens
-    const long long row = (long long)ll * p.n_tokens + tok;
-    const size_t at = (size_t)(row * p.token_stride) + (size_t)kvh * HD;
-    const float* cr = p.rope ? p.rope_cos + (size_t)(p.first_pos + tok) * (HD / 2) : nullptr;
-    const float* sr = p.rope ? p.rope_sin + (size_t)(p.first_pos + tok) * (HD / 2) : nullptr;
-    float k[4], v[4];
-    load_row<HD>(p.k, p.v, at, p.input_f16, kb, vb, cr, sr, lane, k, v);
-    store_row<HD>(sm, i, lane, k, v);
+  const int b = lane % NB;
+  const size_t brow = ((size_t)layer * p.pool.kv_heads + kvh) * HD + 32 * b;
+#pragma unroll 1
+  for (int step = 0; step < 2 * kKv4Tile / kTokens; ++step) {
+    const bool value = step >= kKv4Tile / kTokens;
+    const int slot = (step % (kKv4Tile / kTokens)) * kTokens + lane / NB;  // token of the tile
+    const bool in = slot >= lo && slot < hi;
+    if (__all_sync(0xffffffffu, !in)) continue;
+    const int tok = tile * kKv4Tile + slot - p.first;  // index among the new tokens
+    float x[32];
+    if (in) {
+      const long long row = (long long)ll * p.n_tokens + tok;
+      load32(value ? p.v : p.k, (size_t)(row * p.token_stride) + (size_t)kvh * HD + 32 * b, p.input_f16, x);
+      if (p.k_bias) {
+        const float* br = (value ? p.v_bias : p.k_bias) + brow;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(br + i);
+          x[i] = __fadd_rn(x[i], v.x);
+          x[i + 1] = __fadd_rn(x[i + 1], v.y);
+          x[i + 2] = __fadd_rn(x[i + 2], v.z);
+          x[i + 3] = __fadd_rn(x[i + 3], v.w);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = 0.f;
+    }
+    if (!value && p.rope) {  // the partner dims are another lane's block of the same token
+      const size_t at = (size_t)(p.first_pos + (in ? tok : 0)) * (HD / 2) + 32 * (b % (NB / 2));
+      const bool upper = b >= NB / 2;
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(p.rope_cos + at + i);
+        const float4 s = *reinterpret_cast<const float4*>(p.rope_sin + at + i);
+        const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float o = __shfl_xor_sync(0xffffffffu, x[i + e], NB / 2);
+          x[i + e] = upper ? rope_hi(o, x[i + e], cv[e], sv[e]) : rope_lo(x[i + e], o, cv[e], sv[e]);
+        }
+      }
+    }
+    if (!in) continue;
+    const __half d = q4_quantise32(x);
+    const int j = slot >> 3, g = slot & 7;
+    if (!value) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        *reinterpret_cast<uint32_t*>(sm + kv4_word_at(HD, j, 4 * g + t, b)) =
+            q4_bits(x, 8 * t, 16, 4, 20) + (q4_bits(x, 8 * t + 4, 16, 4, 20) << 8);
+      }
+      *reinterpret_cast<__half*>(sm + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1)) = d;
+    } else {
+#pragma unroll
+      for (int gg = 0; gg < 8; ++gg) {
+        *reinterpret_cast<uint16_t*>(sm + CB + kv4_word_at(HD, j, 4 * gg + (g >> 1), b) + 2 * (g & 1)) =
+            (uint16_t)q4_bits(x, 4 * gg, 4, 8, 12);
+      }
+      *reinterpret_cast<__half*>(sm + 2 * CB + SB + kv4_scale_at(HD, j, g >> 1, b, g & 1)) = d;
+    }
     if (p.k_rows) {
-      const size_t o = ((size_t)row * p.pool.kv_heads + kvh) * HD + R::dim(lane);
-      if (R::has_k(lane)) store4(p.k_rows, o, p.rows_f16, k);
-      if (R::has_v(lane)) store4(p.v_rows, o, p.rows_f16, v);
+      const float df = __half2float(d);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] *= df;
+      store32(value ? p.v_rows : p.k_rows, (((size_t)ll * p.n_tokens + tok) * p.pool.kv_heads + kvh) * HD + 32 * b,
+              p.rows_f16, x);
     }
   }
   __syncwarp();
@@ -264,56 +422,79 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
 
 // ---- read ---------------------------------------------------------------------
 
-// One warp per (layer, kv head, tile): lane 4g + t expands its K words (dims
-// 8t.. of token g) and V words (dims 4g.. of tokens 2t, 2t + 1).
+// One warp per (layer, kv head, tile): lane 4g + t expands its K words (dims 8t.. of token g) and V words (dims
+// 4g.. of tokens 2t, 2t + 1), read 16 bytes at a time; a row's pieces leave as whole 32-byte sectors.
 template <int HD>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int t0 = p.first / kKv4Tile;
-  const int n_tiles = (p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1;
-  const long long items = (long long)n_tiles * p.pool.kv_heads * p.n_layers;
-  const long long item = (long long)blockIdx.x * kRowWarps + warp;
-  if (item >= items) return;
-  const int kvh = (int)(item % p.pool.kv_heads);
-  const long long r = item / p.pool.kv_heads;
-  const int tile = t0 + (int)(r % n_tiles);
+  const uint32_t n_tiles = (uint32_t)((p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1);
+  const uint32_t item = blockIdx.x * kRowWarps + warp;
+  const uint32_t r = item / (uint32_t)p.pool.kv_heads;
+  const int kvh = (int)(item - r * (uint32_t)p.pool.kv_heads);
   const int ll = (int)(r / n_tiles);
+  const int tile = t0 + (int)(r - (uint32_t)ll * n_tiles);
+  if (ll >= p.n_layers) return;
   const unsigned char* src = tile_ptr(p.pool, p.page_row, p.layer_begin + ll, kvh, tile, TB);
   auto row_of = [&](int tok) -> long long {  // element offset of tile token tok's row, or -1 outside the range
     const int i = tile * kKv4Tile + tok - p.first;
     return i >= 0 && i < p.n_tokens ? (((long long)ll * p.n_tokens + i) * p.pool.kv_heads + kvh) * HD : -1;
   };
+  // every word of the lane, and its tokens' scales
+  uint32_t kw[2][NB], vw[2][NB], vs[2][NB];
+  uint16_t ks[2][NB];
+  auto words = [&](int at, int stride, int who, uint32_t(&w)[2][NB]) {
+    if constexpr (HD == 128) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4*>(src + at + j * stride + who * 16);
+        w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+      }
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(src + at + who * 16);
+      w[0][0] = v.x; w[0][1] = v.y; w[1][0] = v.z; w[1][1] = v.w;
+    }
+  };
+  words(0, 512, lane, kw);
+  words(CB, 512, lane, vw);
+  words(2 * CB + SB, 64, t, vs);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      ks[j][b] = *reinterpret_cast<const uint16_t*>(src + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1));
+    }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const long long kr = row_of(8 * j + g);
     const long long v0 = row_of(8 * j + 2 * t), v1 = row_of(8 * j + 2 * t + 1);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const uint32_t kw = *reinterpret_cast<const uint32_t*>(src + kv4_word_at(HD, j, lane, b));
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(src + CB + kv4_word_at(HD, j, lane, b));
-      const float kd = __half2float(
-          *reinterpret_cast<const __half*>(src + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1)));
-      const float2 vd = __half22float2(
-          *reinterpret_cast<const __half2*>(src + 2 * CB + SB + kv4_scale_at(HD, j, t, b, 0)));
       if (kr >= 0) {
-        float x[4], y[4];
+        const float d = __half2float(__ushort_as_half(ks[j][b]));
+        float x[8];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          x[2 * q] = q4_value((kw >> (4 * q)) & 15u, kd);
-          x[2 * q + 1] = q4_value((kw >> (4 * q + 16)) & 15u, kd);
-          y[2 * q] = q4_value((kw >> (4 * q + 8)) & 15u, kd);
-          y[2 * q + 1] = q4_value((kw >> (4 * q + 24)) & 15u, kd);
+        for (int q = 0; q < 4; ++q) {
+          x[2 * q] = q4_value((kw[j][b] >> (4 * q)) & 15u, d);
+          x[2 * q + 1] = q4_value((kw[j][b] >> (4 * q + 16)) & 15u, d);
         }
-        store4(p.k_rows, (size_t)kr + 32 * b + 8 * t, p.rows_f16, x);
-        store4(p.k_rows, (size_t)kr + 32 * b + 8 * t + 4, p.rows_f16, y);
+        const size_t at = (size_t)kr + 32 * b + 8 * t;
+        if (p.rows_f16) {
+          *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(p.k_rows) + at) = pack8(x);
+        } else {
+          float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.k_rows) + at);
+          o[0] = make_float4(x[0], x[1], x[2], x[3]);
+          o[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
       }
+      const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&vs[j][b]));
       float x[4], y[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        x[q] = q4_value((vw >> (4 * q)) & 15u, vd.x);
-        y[q] = q4_value((vw >> (4 * q + 16)) & 15u, vd.y);
+        x[q] = q4_value((vw[j][b] >> (4 * q)) & 15u, d.x);
+        y[q] = q4_value((vw[j][b] >> (4 * q + 16)) & 15u, d.y);
       }
       if (v0 >= 0) store4(p.v_rows, (size_t)v0 + 32 * b + 4 * g, p.rows_f16, x);
       if (v1 >= 0) store4(p.v_rows, (size_t)v1 + 32 * b + 4 * g, p.rows_f16, y);
