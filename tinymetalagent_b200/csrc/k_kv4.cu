@@ -281,12 +281,16 @@ __device__ __forceinline__ uint32_t q4_bits(const float (&x)[32], int i0, int s1
   return c(i0) + (c(i0 + 1) << s1) + (c(i0 + 2) << s2) + (c(i0 + 3) << s3);
 }
 
-__device__ __forceinline__ void load32(const void* base, size_t idx, int f16, float (&x)[32]) {
-  if (f16) {
-    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(base) + idx);
-    uint4 u[4];
+// 32 consecutive values of a binary16 (64 bytes) or fp32 (128 bytes) row, as read and as fp32.
+template <bool F16>
+__device__ __forceinline__ void fetch32(const void* base, size_t idx, uint4 (&u)[F16 ? 4 : 8]) {
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + idx * (F16 ? 2 : 4));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = p[i];
+  for (int i = 0; i < (F16 ? 4 : 8); ++i) u[i] = p[i];
+}
+template <bool F16>
+__device__ __forceinline__ void widen32(const uint4 (&u)[F16 ? 4 : 8], float (&x)[32]) {
+  if constexpr (F16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float v[8];
@@ -295,11 +299,12 @@ __device__ __forceinline__ void load32(const void* base, size_t idx, int f16, fl
       for (int e = 0; e < 8; ++e) x[8 * i + e] = v[e];
     }
   } else {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + idx);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float4 v = p[i];
-      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+      x[4 * i] = __uint_as_float(u[i].x);
+      x[4 * i + 1] = __uint_as_float(u[i].y);
+      x[4 * i + 2] = __uint_as_float(u[i].z);
+      x[4 * i + 3] = __uint_as_float(u[i].w);
     }
   }
 }
@@ -319,8 +324,9 @@ __device__ __forceinline__ void store32(void* base, size_t idx, int f16, const f
 }
 
 // One warp per (layer, kv head, tile of 16 tokens), one block a lane: the tile is assembled in shared memory (with
-// the tokens it already holds, if the new ones do not fill it) and written whole.
-template <int HD>
+// the tokens it already holds, if the new ones do not fill it) and written whole.  A step's rows are read while the
+// one before is quantised.
+template <int HD, bool F16>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
   constexpr int kTokens = 32 / NB;  // tokens of a warp's step
@@ -347,17 +353,27 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
   }
   const int b = lane % NB;
   const size_t brow = ((size_t)layer * p.pool.kv_heads + kvh) * HD + 32 * b;
+  constexpr int kSteps = 2 * kKv4Tile / kTokens;
+  uint4 raw[F16 ? 4 : 8];
+  auto fetch = [&](int step) {
+    const int slot = (step % (kSteps / 2)) * kTokens + lane / NB;
+    if (step < kSteps && slot >= lo && slot < hi) {
+      const long long row = (long long)ll * p.n_tokens + (tile * kKv4Tile + slot - p.first);
+      fetch32<F16>(step >= kSteps / 2 ? p.v : p.k, (size_t)(row * p.token_stride) + (size_t)kvh * HD + 32 * b, raw);
+    }
+  };
+  fetch(0);
 #pragma unroll 1
-  for (int step = 0; step < 2 * kKv4Tile / kTokens; ++step) {
-    const bool value = step >= kKv4Tile / kTokens;
-    const int slot = (step % (kKv4Tile / kTokens)) * kTokens + lane / NB;  // token of the tile
+  for (int step = 0; step < kSteps; ++step) {
+    const bool value = step >= kSteps / 2;
+    const int slot = (step % (kSteps / 2)) * kTokens + lane / NB;  // token of the tile
     const bool in = slot >= lo && slot < hi;
-    if (__all_sync(0xffffffffu, !in)) continue;
     const int tok = tile * kKv4Tile + slot - p.first;  // index among the new tokens
     float x[32];
+    if (in) widen32<F16>(raw, x);
+    fetch(step + 1);
+    if (__all_sync(0xffffffffu, !in)) continue;
     if (in) {
-      const long long row = (long long)ll * p.n_tokens + tok;
-      load32(value ? p.v : p.k, (size_t)(row * p.token_stride) + (size_t)kvh * HD + 32 * b, p.input_f16, x);
       if (p.k_bias) {
         const float* br = (value ? p.v_bias : p.k_bias) + brow;
 #pragma unroll
@@ -1448,8 +1464,10 @@ cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream
 
 cudaError_t launch_kv4_append(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
   const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
-  if (head_dim == 128) kv4_append_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  else kv4_append_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  if (head_dim == 128 && p.input_f16) kv4_append_kernel<128, true><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else if (head_dim == 128) kv4_append_kernel<128, false><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else if (p.input_f16) kv4_append_kernel<64, true><<<grid, 32 * kRowWarps, 0, s>>>(p);
+  else kv4_append_kernel<64, false><<<grid, 32 * kRowWarps, 0, s>>>(p);
   return cudaGetLastError();
 }
 
