@@ -12,8 +12,8 @@
 #include "te_rope.cuh"
 
 // Decode launch shape.
-#ifndef KV4_WARPS
-#define KV4_WARPS 8
+#ifndef KV4_CTAS
+
 #define KV4_CTAS 2
 #define KV4_RING 2
 #endif
@@ -616,8 +616,8 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // moves it (rescaling O) only when a score exceeds it by more than 2^5.
 template <int HD>
 struct Dec {
-  static constexpr int kWarps = KV4_WARPS, kCtas = KV4_CTAS;
-  static constexpr int kStageTiles = 2;  // tiles of a copy: 32 tokens
+  static constexpr int kWarps = kKv4Warps, kCtas = KV4_CTAS;
+  static constexpr int kStageTiles = kKv4StageTiles;
   static constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
   static constexpr int kStageBytes = kStageTiles * TB;
   static constexpr int NB = HD / 32;
@@ -631,7 +631,8 @@ struct Dec {
   static constexpr int f_off = stat_off + 2 * kWarps * kKv4Heads * 4;
   static constexpr int flag_off = f_off + kKv4Heads * 4;
   static constexpr int seg_off = flag_off + 16;        // the current segment, the next, a pending one
-  static constexpr int bar_off = seg_off + 3 * 64;
+  static constexpr int feed_off = seg_off + 3 * 64;
+  static constexpr int bar_off = feed_off + kWarps * 64;
   static constexpr int smem = bar_off + kWarps * kRing * 8;
 };
 static_assert((Dec<128>::smem + 1024) * Dec<128>::kCtas <= 228 * 1024, "CTAs per SM");
@@ -968,11 +969,13 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
     vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, 2));
     float beta = 1.f;
     if (vx > w.vlim) {
+      // scales of 2^-8 .. 4 are used as they are; others are moved so that the largest is in [0.5, 1) now and at
+      // most 4 until it moves again
       const int e = min(exponent_of(vx), 15);
-      const int k = min(max(-1 - e, -16), 15);  // |V scale| 2^k in [0.5, 1) now, at most 4 until it moves again
+      const int k = e >= -8 && e < 2 ? 0 : min(max(-1 - e, -16), 15);
       beta = w.vlim > 0.f ? pow2i(k - w.vexp) : 1.f;
       w.vexp = k;
-      w.vlim = pow2i(e + 3);
+      w.vlim = k == 0 ? 4.f : pow2i(e + 3);
       const __half2 h = __float2half2_rn(pow2i(k));
       w.vmul = *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -988,6 +991,14 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
         w.o[b][i][2] *= a0;
         w.o[b][i][3] *= a1;
       }
+  }
+  if (w.vexp != 0) {
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vs[i][j][b] = h2_mul(vs[i][j][b], w.vmul);
   }
   uint32_t ph[T][2], pl[T][2], vw[T][2][NB];
 #pragma unroll
@@ -1013,7 +1024,7 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
       uint32_t hi[2], lo[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t d = h2_mul(vs[i][j][b], w.vmul);
+        const uint32_t d = vs[i][j][b];
         hi[j] = h2_mul(ph[i][j], d);
         lo[j] = h2_fma(pl[i][j], d, h2_fms(ph[i][j], d, hi[j]));
       }
@@ -1042,47 +1053,53 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
 }
 
 // A warp's copies: stages s0 + warp, + kWarps, ... of each segment of the CTA's range, in order, across segments.
+// Lane 0 keeps them, in shared memory: the other lanes' registers are the attention's.
 struct Feed {
-  int u, u0, u1;              // next segment's first unit, the CTA's range
   int stage, s1;              // next stage and end of the current segment
   int page, in;               // the next stage's page and stage within it
   const unsigned char* base;  // page 0 of the segment's layer, at its kv head
-  const unsigned char* at;    // the current page, at its kv head
   const int32_t* row;
-  int page_base;
+  int u, page_base;           // next segment's first unit; as Kv4Seq
+  long long page_bytes;       // from one page of this kv head to the next
 };
+static_assert(sizeof(Feed) <= 56, "feeds in shared memory");
 
+// Moves f to its next stage, or past the end of the CTA's range (false).
 template <int HD>
-__device__ __forceinline__ const unsigned char* feed_next(const Kv4DecodeParams& p, Feed& f, int warp) {
+__device__ __forceinline__ bool feed_seek(const Kv4DecodeParams& p, Feed& f, int warp, int u0, int u1) {
   using D = Dec<HD>;
-  const int spp = p.pool.tiles_per_page / D::kStageTiles;
-  bool moved = f.in >= spp;
   while (f.stage >= f.s1) {
-    if (f.u >= f.u1) return nullptr;
-    const Seg s = kv4_seg_at(p, f.u, f.u0, f.u1);
+    if (f.u >= u1) return false;
+    const Seg s = kv4_seg_at(p, f.u, u0, u1);
     f.u = s.next;
     f.stage = s.s0 + warp;
     f.s1 = s.s1;
     const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
     f.base = p.pool.base + rec * p.pool.tiles_per_page * D::TB;
+    f.page_bytes = (long long)p.pool.kv_heads * p.pool.tiles_per_page * D::TB;
     f.row = p.page_table + (size_t)p.seqs[s.si].slot * p.max_pages_per_seq;
     f.page_base = p.seqs[s.si].page_base;
     f.page = kv4_page_of(p.pool, f.stage * D::kStageTiles);
-    f.in = f.stage - f.page * spp;
-    moved = true;
+    f.in = f.stage - f.page * p.pool.stages_per_page;
   }
-  if (moved) {
-    while (f.in >= spp) {
-      f.in -= spp;
-      ++f.page;
-    }
-    const int id = f.page_base >= 0 ? f.page_base + f.page : f.row[f.page];
-    f.at = f.base + (long long)id * (p.pool.kv_heads * p.pool.tiles_per_page) * D::TB;
-  }
-  const unsigned char* src = f.at + f.in * D::kStageBytes;
+  return true;
+}
+
+// Issues the copy of f's stage and steps past it.
+template <int HD>
+__device__ __forceinline__ void feed_issue(const Kv4DecodeParams& p, Feed& f, unsigned char* dst, uint64_t* bar) {
+  using D = Dec<HD>;
+  const int id = f.page_base >= 0 ? f.page_base + f.page : f.row[f.page];
+  const unsigned char* src = f.base + id * f.page_bytes + f.in * D::kStageBytes;
+  mbar_arrive_expect_tx(bar, D::kStageBytes);
+  bulk_load(dst, src, D::kStageBytes, bar);
   f.stage += D::kWarps;
-  f.in += D::kWarps;
-  return src;
+  f.page += p.pool.step_pages;
+  f.in += p.pool.step_in;
+  if (f.in >= p.pool.stages_per_page) {
+    f.in -= p.pool.stages_per_page;
+    ++f.page;
+  }
 }
 
 template <int HD>
@@ -1118,29 +1135,35 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   const int u_begin = aligned ? 0 : (int)stage_start(blockIdx.x, p.total_units, p.grid);
   const int u1 = aligned ? 1 : (int)stage_start(blockIdx.x + 1, p.total_units, p.grid);
   if (threadIdx.x == 0) seg(0) = kv4_seg_at(p, u_begin, u_begin, u1);
-  Feed feed{};
-  feed.u = feed.u0 = u_begin;
-  feed.u1 = u1;
-  auto issue = [&](int slot) {
-    const unsigned char* src = feed_next<HD>(p, feed, warp);
-    if (src && lane == 0) {
-      mbar_arrive_expect_tx(&bars[slot], D::kStageBytes);
-      bulk_load(ring + slot * D::kStageBytes, src, D::kStageBytes, &bars[slot]);
-    }
-    return src != nullptr;
+  Feed& feed = *reinterpret_cast<Feed*>(smem + D::feed_off + 64 * warp);
+  int* sm_issued = reinterpret_cast<int*>(smem + D::feed_off + 64 * warp + 56);
+  bool feeding = false;
+  if (lane == 0) {
+    feed.stage = feed.s1 = 0;
+    feed.u = u_begin;
+    *sm_issued = 0;
+    feeding = feed_seek<HD>(p, feed, warp, u_begin, u1);
+  }
+  auto issue = [&](int slot) {  // lane 0
+    if (!feeding) return;
+    feed_issue<HD>(p, feed, ring + slot * D::kStageBytes, &bars[slot]);
+    ++*sm_issued;
+    feeding = feed_seek<HD>(p, feed, warp, u_begin, u1);
   };
   griddep_launch_dependents();
   griddep_wait();
+  if (lane == 0) {
+    for (int i = 0; i < D::kRing; ++i) issue(i);
+  }
   __syncthreads();
 
   constexpr int kRows = (H + W - 1) / W;  // query heads a warp prepares
   float qr[kRows][4];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) fetch_query<HD>(p, seg(0), warp + i * W, lane, qr[i]);
-  int issued = 0, used = 0;  // stages copied / consumed by this warp
+  int used = 0;              // stages consumed by this warp
   int slot = 0;
   uint32_t phase = 0;
-  for (int i = 0; i < D::kRing; ++i) issued += issue(i) ? 1 : 0;
   bool ok = true;            // false: a wait ran out; the warp computes no more
   const uint32_t magic = code_magic();
   int n_pending = 0;         // segments of this CTA that are parts of shared groups
@@ -1223,7 +1246,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
       if (cached) {
         __syncwarp();
         ++used;
-        issued += issue(slot) ? 1 : 0;
+        if (lane == 0) issue(slot);
         if (++slot == D::kRing) {
           slot = 0;
           phase ^= 1u;
@@ -1384,7 +1407,8 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   }
   if (!ok) {
     // copies of this warp may still be in flight: let them land before the CTA leaves
-    for (; used < issued; ++used) {
+    __syncwarp();
+    for (const int issued = *sm_issued; used < issued; ++used) {
       (void)mbar_wait_warp(&bars[slot], phase);
       if (++slot == D::kRing) {
         slot = 0;

@@ -36,6 +36,9 @@ Kv4Pool pool_of(const te_kv4_cache* c) {
   p.page_tokens = (int32_t)c->b.d.page_tokens;
   p.tiles_per_page = (int32_t)(c->b.d.page_tokens / kKv4Tile);
   p.tpp_magic = (uint32_t)(((1ull << 32) + (uint64_t)p.tiles_per_page - 1) / (uint64_t)p.tiles_per_page);
+  p.stages_per_page = p.tiles_per_page / kKv4StageTiles;
+  p.step_pages = kKv4Warps / p.stages_per_page;
+  p.step_in = kKv4Warps % p.stages_per_page;
   return p;
 }
 

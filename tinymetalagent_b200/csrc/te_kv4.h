@@ -33,6 +33,8 @@ namespace te {
 
 constexpr int kKv4Tile = 16;        // tokens of a tile
 constexpr int kKv4Unit = 256;       // tokens of a work unit of the decode split: one stage of 32 for each of 8 warps
+constexpr int kKv4StageTiles = 2;   // tiles of a copy of the decode kernel
+constexpr int kKv4Warps = 8;        // warps of a decode CTA, each with its own copies
 constexpr int kKv4Heads = 8;        // query heads of a work group (larger groups take several)
 constexpr int kKv4MaxSeqs = 64;     // sequences per decode launch
 
@@ -54,6 +56,8 @@ struct Kv4Pool {
   int32_t kv_heads;
   int32_t tiles_per_page;
   uint32_t tpp_magic;       // ceil(2^32 / tiles_per_page)
+  int32_t stages_per_page;  // of kKv4StageTiles tiles
+  int32_t step_pages, step_in;  // kKv4Warps stages on: whole pages, and stages past them
   int32_t page_tokens;
 };
 
