@@ -1090,7 +1090,7 @@ template <int HD>
 __device__ __forceinline__ void feed_issue(const Kv4DecodeParams& p, Feed& f, unsigned char* dst, uint64_t* bar) {
   using D = Dec<HD>;
   const int id = f.page_base >= 0 ? f.page_base + f.page : f.row[f.page];
-  const unsigned char* src = f.base + id * f.page_bytes + f.in * D::kStageBytes;
+  const unsigned char* src = f.base + id * f.page_bytes + (long long)f.in * D::kStageBytes;
   mbar_arrive_expect_tx(bar, D::kStageBytes);
   bulk_load(dst, src, D::kStageBytes, bar);
   f.stage += D::kWarps;
@@ -1143,7 +1143,13 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
     feed.u = u_begin;
     *sm_issued = 0;
     feeding = feed_seek<HD>(p, feed, warp, u_begin, u1);
+    // L2 may fetch the first stage while the previous kernel drains (a hint, coherent with that kernel's writes)
+    if (feeding && feed.page_base >= 0) {
+      bulk_prefetch_l2(feed.base + (feed.page_base + feed.page) * feed.page_bytes + (long long)feed.in * D::kStageBytes,
+                       D::kStageBytes);
+    }
   }
+  __syncthreads();
   auto issue = [&](int slot) {  // lane 0
     if (!feeding) return;
     feed_issue<HD>(p, feed, ring + slot * D::kStageBytes, &bars[slot]);
@@ -1152,15 +1158,13 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   };
   griddep_launch_dependents();
   griddep_wait();
+  constexpr int kRows = (H + W - 1) / W;  // query heads a warp prepares
+  float qr[kRows][4];  // asked for before the stages, whose first wave fills the memory system for microseconds
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) fetch_query<HD>(p, seg(0), warp + i * W, lane, qr[i]);
   if (lane == 0) {
     for (int i = 0; i < D::kRing; ++i) issue(i);
   }
-  __syncthreads();
-
-  constexpr int kRows = (H + W - 1) / W;  // query heads a warp prepares
-  float qr[kRows][4];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) fetch_query<HD>(p, seg(0), warp + i * W, lane, qr[i]);
   int used = 0;              // stages consumed by this warp
   int slot = 0;
   uint32_t phase = 0;
@@ -1350,59 +1354,57 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   // the end, where the records have long been written and no segment of this CTA waits behind a fold.
   if (n_pending > 0) {
     __syncthreads();
-    if (threadIdx.x == 0) {
-      __threadfence();
-      const Seg &a = seg(2), &b = seg(at_seg);
-      sm_flag[0] = atomicAdd(&p.counters[a.group_id], 1u) == (uint32_t)a.parts - 1u;
-      sm_flag[1] = n_pending > 1 && atomicAdd(&p.counters[b.group_id], 1u) == (uint32_t)b.parts - 1u;
-      __threadfence();
+    if (threadIdx.x < (unsigned)n_pending) {
+      const Seg& q = seg(threadIdx.x == 0 ? 2 : at_seg);
+      sm_flag[threadIdx.x] = atom_add_acq_rel_gpu(&p.counters[q.group_id], 1u) == (uint32_t)q.parts - 1u;
     }
     __syncthreads();
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < n_pending; ++i) {
       if (sm_flag[i] == 0) continue;
       const Seg& q = seg(i == 0 ? 2 : at_seg);
-      // part k is CTA c0 + k's: its first segment unless (stream split) its range began before the group
-      auto rec_of = [&](int k) {
-        const int c = q.c0 + k;
-        const int sl = aligned || stage_start(c, p.total_units, p.grid) >= q.gb ? 0 : 1;
-        return p.partials + ((size_t)c * 2 + sl) * rec;
-      };
-      float* wt = reinterpret_cast<float*>(smem);  // [parts][8] m, then weights; [parts][8] l (no copy is in flight)
-      float* tot = sm_m;                           // [8] sums, [8] reference exponents
-      for (int j = threadIdx.x; j < q.parts * 2 * H; j += 32 * W) {
-        const int k = j / (2 * H), e = j - k * 2 * H;
-        wt[(e < H ? 0 : q.parts * H) + k * H + (e & 7)] = __ldcg(rec_of(k) + H * HD + e);
-      }
-      __syncthreads();
-      if (threadIdx.x < H) {
-        float all = -INFINITY, sum = 0.f;
-        for (int k = 0; k < q.parts; ++k) all = fmaxf(all, wt[k * H + threadIdx.x]);
-        for (int k = 0; k < q.parts; ++k) {
-          const float e = part_weight(wt[k * H + threadIdx.x], all);
-          wt[k * H + threadIdx.x] = e;
-          sum = fmaf(e, wt[(q.parts + k) * H + threadIdx.x], sum);
-        }
-        tot[threadIdx.x] = sum;
-        tot[H + threadIdx.x] = all;
-      }
-      __syncthreads();
+      // part k is CTA c0 + k's: its first segment unless (stream split) its range began before the group, which
+      // only the group's first part can
+      const int slot0 = aligned || stage_start(q.c0, p.total_units, p.grid) >= q.gb ? 0 : 1;
+      auto rec_of = [&](int k) { return p.partials + ((size_t)(q.c0 + k) * 2 + (k == 0 ? slot0 : 0)) * rec; };
       for (int j = threadIdx.x; j < D::kItems; j += 32 * W) {
         const int head = 2 * (j & 3) + ((j >> 5) & 1);
         const int dim = 32 * (j >> 6) + 4 * ((j & 31) >> 2);
+        // eight records at a time, all of their loads in flight together; the running state is rescaled per batch
+        constexpr int kBatch = 8;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int k = 0; k < q.parts; ++k) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(rec_of(k)) + j);
-          const float e = wt[k * H + head];
-          acc.x = fmaf(e, x.x, acc.x);
-          acc.y = fmaf(e, x.y, acc.y);
-          acc.z = fmaf(e, x.z, acc.z);
-          acc.w = fmaf(e, x.w, acc.w);
+        float top = -INFINITY, sum = 0.f;
+        for (int k0 = 0; k0 < q.parts; k0 += kBatch) {
+          float m[kBatch], l[kBatch];
+          float4 x[kBatch];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const bool have = k0 + k < q.parts;
+            const float* r = rec_of(have ? k0 + k : 0);
+            m[k] = have ? __ldcg(r + H * HD + head) : -INFINITY;
+            l[k] = __ldcg(r + H * HD + H + head);
+            x[k] = __ldcg(reinterpret_cast<const float4*>(r) + j);
+          }
+          float all = top;
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) all = fmaxf(all, m[k]);
+          const float keep = part_weight(top, all);
+          acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+          sum *= keep;
+          top = all;
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            if (k0 + k >= q.parts) continue;
+            const float e = part_weight(m[k], all);
+            acc.x = fmaf(e, x[k].x, acc.x);
+            acc.y = fmaf(e, x[k].y, acc.y);
+            acc.z = fmaf(e, x[k].z, acc.z);
+            acc.w = fmaf(e, x[k].w, acc.w);
+            sum = fmaf(e, l[k], sum);
+          }
         }
-        write_out(q, head, dim, acc, tot[H + head], tot[head]);
+        write_out(q, head, dim, acc, top, sum);
       }
       if (threadIdx.x == 0) p.counters[q.group_id] = 0;
-      __syncthreads();
     }
   }
   if (!ok) {

@@ -399,6 +399,13 @@ __device__ __forceinline__ void st_relaxed_sys_u32(uint32_t* p, uint32_t v) {
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Counts at GPU scope, after this thread's earlier writes and those it has observed (bar.sync), before its later reads.
+__device__ __forceinline__ uint32_t atom_add_acq_rel_gpu(uint32_t* p, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+
 // GPU-scope acquire-release fence: orders this thread's earlier memory
 // operations (and those it has observed, e.g. through __syncwarp) before its
 // later ones, without the full sequential-consistency fence of __threadfence.
