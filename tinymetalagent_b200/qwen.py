@@ -21,7 +21,8 @@ into fp32 in HBM (q * scale, exact), so a token's row is a copy.
 One difference from the reference's CPU pass is by design: the KV cache is
 the engine's f16 cache (the reference's Metal path's layout), where the CPU
 pass keeps fp32 keys and values, so outputs agree to f16 rounding of K/V, not
-bit for bit.
+bit for bit.  With kv_bits=4 it is the 4-bit cache (te_kv4_*, GGUF Q4_0
+blocks): 3.56 times the context in the same memory.
 """
 from __future__ import annotations
 
@@ -30,8 +31,8 @@ from pathlib import Path
 import numpy as np
 
 from .gguf import GGML_F32, GGML_Q4_0, GGML_Q8_0, GGUFError, GGUFFile
-from .runtime import (TE_ATTN_ACCUMULATE, TE_ATTN_ADVANCE, TE_ATTN_QKV_BIAS, TE_ATTN_RMSNORM_INPUT,
-                      TE_ATTN_STEP_HEAD, TE_ATTN_SWIGLU_INPUT, AttnEngine, QwenStep)
+from .runtime import (TE_ATTN_ACCUMULATE, TE_ATTN_ADVANCE, TE_ATTN_OUTPUT_F16, TE_ATTN_QKV_BIAS,
+                      TE_ATTN_RMSNORM_INPUT, TE_ATTN_STEP_HEAD, TE_ATTN_SWIGLU_INPUT, AttnEngine, QwenStep)
 
 _QUANT = {GGML_Q4_0: 4, GGML_Q8_0: 8}  # ggml type -> TE_ATTN_QUANT_GGUF_*
 
@@ -53,13 +54,21 @@ class QwenDecoder:
     per layer; the per-op path (fused_step=False) stays available and is what
     prefill_prompt uses.  The fused step needs the same quantisation for a
     projection in every layer; otherwise the decoder takes the per-op path.
+
+    kv_bits 16 keeps the keys and values in the f16 cache; kv_bits 4 in the
+    4-bit cache, on the per-op path: a step's launch quantises the new token
+    and attends the cache as stored, a prompt attends its own rows in f16 and
+    the history as read back from the cache, and is then quantised into it.
     """
 
     def __init__(self, engine: AttnEngine, model: str | Path | GGUFFile, context_tokens: int,
-                 fused_step: bool = True):
+                 fused_step: bool = True, kv_bits: int = 16):
         import torch
 
-        self._want_step = fused_step
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 16 or 4")
+        self.kv_bits = kv_bits
+        self._want_step = fused_step and kv_bits == 16
         self.engine = engine
         self._owns_gguf = not isinstance(model, GGUFFile)
         self.gguf = model if isinstance(model, GGUFFile) else GGUFFile(model)
@@ -136,10 +145,13 @@ class QwenDecoder:
         self._q_head = quant_of(head)
         self._out_norm = f32("output_norm.weight", H)
 
-        self.cache = self.engine.kv_cache(layers=L, max_seqs=1, max_tokens_per_seq=self.context_tokens,
-                                          kv_heads=kvh, head_dim=hd, max_position=self.context_tokens,
-                                          rope_theta=d["rope_base"])
+        make = self.engine.kv4_cache if self.kv_bits == 4 else self.engine.kv_cache
+        self.cache = make(layers=L, max_seqs=1, max_tokens_per_seq=self.context_tokens, kv_heads=kvh, head_dim=hd,
+                          max_position=self.context_tokens, rope_theta=d["rope_base"])
         self.cache.set_qkv_bias(0, heads, qb, kb, vb)
+        self._prompt_cache = None  # 4-bit cache: one layer in f16, for the prompt pass
+        if self.kv_bits == 4:
+            self._qkv_bias = torch.from_numpy(np.concatenate([qb, kb, vb], axis=1)).to(dev)
         self._step = None
         quants = {k: {w["q_" + k] for w in self.layers} for k in ("qkv", "o", "gu", "down")}
         if self._want_step and all(len(v) == 1 for v in quants.values()):
@@ -292,11 +304,14 @@ class QwenDecoder:
             for c, m in chunks:
                 eng.matvec_gguf_fused(w["q_qkv"], w["qkv"], H + 2 * kv, H, X[c:c + m], qkv[c:c + m],
                                       TE_ATTN_RMSNORM_INPUT, w["attn_norm"], eps, n_vectors=m)
-            q = qkv[:, :H].contiguous()
-            k = qkv[:, H:H + kv].contiguous()
-            v = qkv[:, H + kv:].contiguous()
-            flags = TE_ATTN_QKV_BIAS | (TE_ATTN_ADVANCE if layer == L - 1 else 0)
-            self.cache.prefill(layer, 1, 0, q, k, v, T, heads, attn, flags)
+            if self.kv_bits == 4:
+                self._prefill_kv4(layer, qkv, attn, TE_ATTN_ADVANCE if layer == L - 1 else 0)
+            else:
+                q = qkv[:, :H].contiguous()
+                k = qkv[:, H:H + kv].contiguous()
+                v = qkv[:, H + kv:].contiguous()
+                flags = TE_ATTN_QKV_BIAS | (TE_ATTN_ADVANCE if layer == L - 1 else 0)
+                self.cache.prefill(layer, 1, 0, q, k, v, T, heads, attn, flags)
             for c, m in chunks:
                 eng.matvec_gguf(w["q_o"], w["o"], H, H, attn[c:c + m], X[c:c + m], n_vectors=m,
                                 flags=TE_ATTN_ACCUMULATE)
@@ -307,6 +322,29 @@ class QwenDecoder:
                 eng.matvec_gguf_fused(w["q_down"], w["down"], H, F, gu[c:c + m], X[c:c + m],
                                       TE_ATTN_SWIGLU_INPUT | TE_ATTN_ACCUMULATE, n_vectors=m)
         self.x.copy_(X[T - 1])
+
+    def _prefill_kv4(self, layer: int, qkv, attn, advance: int) -> None:
+        """One layer's causal attention of a prompt over the 4-bit cache: the history is read back into one f16
+        layer, the prompt's rows are attended there in f16, and the k and v columns are quantised into the cache."""
+        import torch
+        d = self.dims
+        H, T, kvh, hd = d["hidden"], qkv.shape[0], d["kv_heads"], d["head_dim"]
+        n = self.cache.length(0)
+        if self._prompt_cache is None:
+            self._prompt_cache = self.engine.kv_cache(
+                layers=1, max_seqs=1, max_tokens_per_seq=self.context_tokens, kv_heads=kvh, head_dim=hd,
+                max_position=self.context_tokens, rope_theta=d["rope_base"])
+        pc = self._prompt_cache
+        pc.reset(0)
+        if n:
+            k = torch.empty((1, n, kvh, hd), dtype=torch.float16, device=self._dev)
+            v = torch.empty_like(k)
+            self.cache.read(layer, 1, 0, 0, n, k, v, flags=TE_ATTN_OUTPUT_F16)
+            pc.write_f16(0, 0, 0, k[0], v[0])
+        biased = qkv + self._qkv_bias[layer]  # one fp32 addition a value, as TE_ATTN_QKV_BIAS does
+        q, k, v = biased[:, :H], biased[:, H:H + self.kv], biased[:, H + self.kv:]
+        pc.prefill(0, 1, 0, q.contiguous(), k.contiguous(), v.contiguous(), T, d["heads"], attn, 0)
+        self.cache.append(layer, 1, 0, k, v, T, flags=advance)
 
     def project_next(self) -> int:
         import torch
@@ -389,6 +427,9 @@ class QwenDecoder:
         if getattr(self, "_step", None) is not None:
             self._step.close()
             self._step = None
+        if getattr(self, "_prompt_cache", None) is not None:
+            self._prompt_cache.close()
+            self._prompt_cache = None
         if getattr(self, "cache", None) is not None:
             self.cache.close()
             self.cache = None

@@ -544,6 +544,9 @@ class KV4Cache:
         engine._caches.add(self)
         self.layers, self.max_seqs, self.kv_heads, self.head_dim = layers, max_seqs, kv_heads, head_dim
         self.page_tokens, self.max_tokens_per_seq, self.rope_theta = page_tokens, max_tokens_per_seq, rope_theta
+        self._device = engine.device
+        import torch
+        self._dtypes = {"float32": torch.float32, "float16": torch.float16, "uint8": torch.uint8}
 
     def close(self) -> None:
         if getattr(self, "handle", None) and getattr(self.engine, "handle", None):
@@ -559,16 +562,16 @@ class KV4Cache:
     def _c(self, status: int) -> None:
         self.engine.check(status)
 
-    def _tensor(self, x, name: str, values: int, *dtypes: str) -> Optional[int]:
-        """Address of a contiguous CUDA tensor of `values` values of one of `dtypes`, or of a raw address."""
+    def _tensor(self, x, name: str, values: int, dtype: str) -> Optional[int]:
+        """Address of a contiguous CUDA tensor of `values` values of type `dtype`; a raw address as it is."""
         if x is None or isinstance(x, int):
             return x
-        if not hasattr(x, "is_cuda"):
+        if not hasattr(x, "get_device"):
             raise TypeError(f"{name}: a CUDA tensor or an address")
-        if not x.is_cuda or x.device.index != self.engine.device:
+        if x.get_device() != self._device:  # -1 for a tensor on the host
             raise ValueError(f"{name}: not on the engine's device")
-        if str(x.dtype)[6:] not in dtypes:
-            raise ValueError(f"{name}: type {x.dtype}, expected {' or '.join(dtypes)}")
+        if x.dtype is not self._dtypes[dtype]:
+            raise ValueError(f"{name}: type {x.dtype}, expected {dtype}")
         if x.numel() != values or not x.is_contiguous():
             raise ValueError(f"{name}: expected {values} contiguous values")
         return x.data_ptr()
@@ -617,7 +620,7 @@ class KV4Cache:
             count *= size
         if x.stride(-1) != 1 or count != n_layers * n_tokens:
             raise ValueError(f"{name}: expected n_layers * n_tokens rows of contiguous values")
-        if not x.is_cuda or x.device.index != self.engine.device or str(x.dtype)[6:] != dtype:
+        if x.get_device() != self._device or x.dtype is not self._dtypes[dtype]:
             raise ValueError(f"{name}: expected {dtype} on the engine's device")
         return x.data_ptr(), row if stride is None else stride
 
@@ -673,14 +676,13 @@ class KV4Cache:
         dtype = "float16" if flags & TE_ATTN_INPUT_F16 else "float32"
         rows = n_layers * n
         hd, kv = self.head_dim, rows * self.kv_heads * self.head_dim
-        ids = (ctypes.c_uint32 * n)(*seq_ids)
         qp = None
         if q_positions is not None:
             if len(q_positions) != n:
                 raise ValueError("one query position per sequence")
             qp = (ctypes.c_int64 * n)(*q_positions)
         self._c(self.lib.te_kv4_attention_decode(
-            self.handle, layer_begin, n_layers, ids, n, qp, self._tensor(q, "q", rows * heads * hd, dtype),
+            self.handle, layer_begin, n_layers, (ctypes.c_uint32 * n)(*seq_ids), n, qp, self._tensor(q, "q", rows * heads * hd, dtype),
             self._tensor(k_new, "k_new", kv, dtype), self._tensor(v_new, "v_new", kv, dtype), heads,
             self._tensor(out, "out", rows * heads * (hd + (2 if flags & TE_ATTN_PARTIAL else 0)), "float32"), flags))
 
