@@ -331,6 +331,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
   constexpr int kTokens = 32 / NB;  // tokens of a warp's step
   __shared__ __align__(16) unsigned char tiles[kRowWarps][TB];
+  griddep_launch_dependents();
+  griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = p.first / kKv4Tile;
   const uint32_t n_tiles = (uint32_t)((p.first + p.n_tokens - 1) / kKv4Tile - t0 + 1);
@@ -443,6 +445,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
 template <int HD>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
+  griddep_launch_dependents();
+  griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int t0 = p.first / kKv4Tile;
@@ -1208,8 +1212,12 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
     const int len = sq.len;
     const int n_stages = s.s1 - s.s0;
     const bool appender = p.k_new != nullptr && s.last && warp == n_stages % W;
+    __syncthreads();  // the queries are in shared memory
+    w.f = sm_f[g];
+    reset_state<HD>(w);
     if (appender) {
-      // the new token: quantised into the cache (by the first head block) and into a stage of its own here
+      // the new token: quantised into the cache (by the first head block) and into a stage of its own here, by the
+      // warp that has the fewest stages, while the others attend theirs
       const size_t at = (((size_t)s.ll * p.seq_total + p.seq_base + s.si) * p.pool.kv_heads + s.kvh) * HD;
       const size_t brow = ((size_t)(p.layer_begin + s.ll) * p.pool.kv_heads + s.kvh) * HD;
       float k[4], v[4];
@@ -1224,15 +1232,13 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
                                       s.kvh, len / kKv4Tile, D::TB);
         store_row<HD>(dst, len % kKv4Tile, lane, k2, v2);
       }
+      __syncwarp();
     }
-    __syncthreads();  // the queries (and the new token) are in shared memory
-    w.f = sm_f[g];
-    reset_state<HD>(w);
-    // this warp's stages, the appended token's after them
+    // the appended token's stage, then this warp's
     int st = s.s0 + warp;
     bool extra = appender;
     while (st < s.s1 || extra) {
-      const bool cached = st < s.s1;
+      const bool cached = !extra;
       uint32_t addr = smem_u32(new_stage);
       int valid = 1;
       if (cached) {
@@ -1438,9 +1444,19 @@ cudaError_t launch_decode_t(const Kv4DecodeParams& p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kv4_decode_kernel<HD>, p);
 }
 
-long long row_items(const Kv4RowsParams& p) {
-  const long long tiles = (p.first + p.n_tokens - 1) / kKv4Tile - p.first / kKv4Tile + 1;
-  return tiles * p.pool.kv_heads * p.n_layers;
+// A warp per (layer, kv head, tile), as a programmatic dependent.
+cudaError_t launch_rows(void (*kernel)(Kv4RowsParams), const Kv4RowsParams& p, cudaStream_t s) {
+  const long long items = kv4_row_items(p);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)((items + kRowWarps - 1) / kRowWarps));
+  cfg.blockDim = dim3(32 * kRowWarps);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 }  // namespace
@@ -1489,19 +1505,12 @@ cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream
 }
 
 cudaError_t launch_kv4_append(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
-  const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
-  if (head_dim == 128 && p.input_f16) kv4_append_kernel<128, true><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  else if (head_dim == 128) kv4_append_kernel<128, false><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  else if (p.input_f16) kv4_append_kernel<64, true><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  else kv4_append_kernel<64, false><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  return cudaGetLastError();
+  if (head_dim == 128) return launch_rows(p.input_f16 ? kv4_append_kernel<128, true> : kv4_append_kernel<128, false>, p, s);
+  return launch_rows(p.input_f16 ? kv4_append_kernel<64, true> : kv4_append_kernel<64, false>, p, s);
 }
 
 cudaError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, cudaStream_t s) {
-  const unsigned grid = (unsigned)((row_items(p) + kRowWarps - 1) / kRowWarps);
-  if (head_dim == 128) kv4_read_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  else kv4_read_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_rows(head_dim == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>, p, s);
 }
 
 cudaError_t launch_kv4_raw(const Kv4RowsParams& p, int head_dim, bool to_pool, cudaStream_t s) {

@@ -226,6 +226,7 @@ TE_API te_status te_kv4_append(te_kv4_cache* c, size_t layer_begin, size_t n_lay
   p.rope = (flags & TE_ATTN_NO_ROPE) ? 0 : 1;
   p.input_f16 = (flags & TE_ATTN_INPUT_F16) ? 1 : 0;
   p.rows_f16 = (flags & TE_ATTN_OUTPUT_F16) ? 1 : 0;
+  if (kv4_row_items(p) > (long long)INT32_MAX) return fail(e, TE_STATUS_UNSUPPORTED, "too many rows for one call");
   const int prof = prof_begin(e, PK_KV4_APPEND);
   st = queue(e, launch_kv4_append(p, (int)c->b.d.head_dim, e->stream), prof, "4-bit append launch");
   if (st == TE_STATUS_OK && (flags & TE_ATTN_ADVANCE)) c->b.len[seq] = (int64_t)(first + n_tokens);
@@ -257,6 +258,7 @@ TE_API te_status te_kv4_cache_read(te_kv4_cache* c, size_t layer_begin, size_t n
   p.k_rows = k;
   p.v_rows = v;
   p.rows_f16 = (flags & TE_ATTN_OUTPUT_F16) ? 1 : 0;
+  if (kv4_row_items(p) > (long long)INT32_MAX) return fail(e, TE_STATUS_UNSUPPORTED, "too many rows for one call");
   const int prof = prof_begin(e, PK_KV4_READ);
   return queue(e, launch_kv4_read(p, (int)c->b.d.head_dim, e->stream), prof, "4-bit read launch");
 }

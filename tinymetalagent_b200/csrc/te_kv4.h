@@ -130,6 +130,11 @@ struct Kv4RowsParams {
   int32_t input_f16;        // append: k and v are binary16
   int32_t rows_f16;         // k_rows and v_rows are binary16
 };
+// Warps of an append or read call; the kernels index them in 32 bits.
+inline long long kv4_row_items(const Kv4RowsParams& p) {
+  const long long tiles = (long long)(p.first + p.n_tokens - 1) / kKv4Tile - p.first / kKv4Tile + 1;
+  return tiles * p.pool.kv_heads * p.n_layers;
+}
 cudaError_t launch_kv4_append(const Kv4RowsParams& p, int head_dim, cudaStream_t s);
 cudaError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, cudaStream_t s);
 // Raw GGUF Q4_0 blocks [n_layers][n_tokens][kv_heads][hd / 32][18 bytes] into the pool (k, v) or out of it (k_rows, v_rows).
