@@ -331,7 +331,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
   constexpr int kTokens = 32 / NB;  // tokens of a warp's step
   __shared__ __align__(16) unsigned char tiles[kRowWarps][TB];
-  griddep_launch_dependents();
   griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = p.first / kKv4Tile;
@@ -445,7 +444,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
 template <int HD>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
-  griddep_launch_dependents();
   griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -1444,7 +1442,9 @@ cudaError_t launch_decode_t(const Kv4DecodeParams& p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kv4_decode_kernel<HD>, p);
 }
 
-// A warp per (layer, kv head, tile), as a programmatic dependent.
+// A warp per (layer, kv head, tile), as a programmatic dependent.  These kernels let their own dependents start only
+// as they end: an early start's waiting CTAs take the slots of a kernel that fills the GPU once (12.9 us against 6.7
+// for 29 MB read back).
 cudaError_t launch_rows(void (*kernel)(Kv4RowsParams), const Kv4RowsParams& p, cudaStream_t s) {
   const long long items = kv4_row_items(p);
   cudaLaunchConfig_t cfg = {};
