@@ -12,12 +12,6 @@
 #include "te_rope.cuh"
 
 // Decode launch shape.
-#ifndef KV4_CTAS
-
-#define KV4_CTAS 2
-#define KV4_RING 2
-#endif
-
 namespace te {
 namespace {
 
@@ -618,12 +612,12 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // moves it (rescaling O) only when a score exceeds it by more than 2^5.
 template <int HD>
 struct Dec {
-  static constexpr int kWarps = kKv4Warps, kCtas = KV4_CTAS;
-  static constexpr int kStageTiles = kKv4StageTiles;
+  static constexpr int kWarps = kKv4Warps, kCtas = 2;
+  static constexpr int kStageTiles = kv4_stage_tiles(HD), kStageTokens = kv4_stage_tokens(HD);
   static constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
   static constexpr int kStageBytes = kStageTiles * TB;
   static constexpr int NB = HD / 32;
-  static constexpr int kRing = KV4_RING * (128 / HD);  // stages in flight per warp
+  static constexpr int kRing = 2;                       // stages in flight per warp
   static constexpr int kItems = NB * 2 * 32;           // float4 items of a warp's O
   static constexpr int ring_off = 0;
   static constexpr int new_off = kWarps * kRing * kStageBytes;  // a stage for the appended token
@@ -640,12 +634,10 @@ struct Dec {
 static_assert((Dec<128>::smem + 1024) * Dec<128>::kCtas <= 228 * 1024, "CTAs per SM");
 static_assert((Dec<64>::smem + 1024) * Dec<64>::kCtas <= 228 * 1024, "CTAs per SM");
 
-constexpr int kStageTokens4 = 32;
-
 struct Seg {
   int next;            // the CTA's next unit (global index), its end when there is none
   int ll, kvh, hb, si; // local layer, kv head, head block, sequence
-  int s0, s1;          // stages (32 tokens) of the sequence in this segment
+  int s0, s1;          // stages (copies) of the sequence in this segment
   int first;           // 1: the CTA's first segment
   int parts, c0;       // CTAs that share the group, the first of them
   int gb;              // stream split: the group's first unit (global index)
@@ -661,6 +653,7 @@ __device__ __forceinline__ int kv4_cta_of(int u, long long total, int grid) {
 }
 
 // The segment of this CTA that begins at u (stream split), or its only one (aligned split).
+template <int HD>
 __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u_begin, int u1) {
   Seg s;
   const bool aligned = p.block_parts != 0;
@@ -676,7 +669,7 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
   }
   s.si = lo;
   const int len = p.seqs[lo].len;
-  const int n = kv4_units(len);
+  const int n = kv4_units(len, HD);
   int a, b;  // units of the sequence in this segment
   if (aligned) {
     const int part = rem - p.seqs[lo].part_begin;
@@ -696,9 +689,9 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
     s.parts = kv4_cta_of(s.gb + n - 1, p.total_units, p.grid) - s.c0 + 1;
     s.first = u == u_begin;
   }
-  constexpr int kUnitStages = kKv4Unit / kStageTokens4;
+  constexpr int kUnitStages = kKv4Warps, kTokens = kv4_stage_tokens(HD);
   s.s0 = a * kUnitStages;
-  s.s1 = min(b * kUnitStages, (len + kStageTokens4 - 1) / kStageTokens4);
+  s.s1 = min(b * kUnitStages, (len + kTokens - 1) / kTokens);
   s.last = b == n;
   const uint32_t lk = blk / (uint32_t)p.head_blocks;
   s.hb = (int)(blk - lk * (uint32_t)p.head_blocks);
@@ -1072,7 +1065,7 @@ __device__ __forceinline__ bool feed_seek(const Kv4DecodeParams& p, Feed& f, int
   using D = Dec<HD>;
   while (f.stage >= f.s1) {
     if (f.u >= u1) return false;
-    const Seg s = kv4_seg_at(p, f.u, u0, u1);
+    const Seg s = kv4_seg_at<HD>(p, f.u, u0, u1);
     f.u = s.next;
     f.stage = s.s0 + warp;
     f.s1 = s.s1;
@@ -1136,7 +1129,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   const bool aligned = p.block_parts != 0;
   const int u_begin = aligned ? 0 : (int)stage_start(blockIdx.x, p.total_units, p.grid);
   const int u1 = aligned ? 1 : (int)stage_start(blockIdx.x + 1, p.total_units, p.grid);
-  if (threadIdx.x == 0) seg(0) = kv4_seg_at(p, u_begin, u_begin, u1);
+  if (threadIdx.x == 0) seg(0) = kv4_seg_at<HD>(p, u_begin, u_begin, u1);
   Feed& feed = *reinterpret_cast<Feed*>(smem + D::feed_off + 64 * warp);
   int* sm_issued = reinterpret_cast<int*>(smem + D::feed_off + 64 * warp + 56);
   bool feeding = false;
@@ -1246,7 +1239,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
           break;
         }
         addr = smem_u32(ring + slot * D::kStageBytes);
-        valid = len - st * kStageTokens4;
+        valid = len - st * D::kStageTokens;
       } else {
         extra = false;
       }
@@ -1313,7 +1306,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
         }
     }
     const bool more = s.next < u1;
-    if (more && threadIdx.x == 0) seg(at_seg ^ 1) = kv4_seg_at(p, s.next, u_begin, u1);
+    if (more && threadIdx.x == 0) seg(at_seg ^ 1) = kv4_seg_at<HD>(p, s.next, u_begin, u1);
     __syncthreads();
     if (more) {  // the next segment's query rows on their way
 #pragma unroll
@@ -1461,13 +1454,13 @@ cudaError_t launch_rows(void (*kernel)(Kv4RowsParams), const Kv4RowsParams& p, c
 
 }  // namespace
 
-int kv4_decode_ctas_per_sm() { return KV4_CTAS; }
+int kv4_decode_ctas_per_sm() { return Dec<128>::kCtas; }
 
-void plan_kv4_decode(Kv4DecodeParams& p, long long slots) {
+void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   const long long reps = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks;
   int acc = 0, longest = 1;
   for (int i = 0; i < p.n_seqs; ++i) {
-    const int n = kv4_units(p.seqs[i].len);
+    const int n = kv4_units(p.seqs[i].len, head_dim);
     p.seqs[i].unit_begin = acc;
     acc += n;
     longest = n > longest ? n : longest;
@@ -1477,7 +1470,7 @@ void plan_kv4_decode(Kv4DecodeParams& p, long long slots) {
   // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once.
   auto parts_for = [&](int most) {
     long long c = 0;
-    for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len) + most - 1) / most;
+    for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len, head_dim) + most - 1) / most;
     return c * reps;
   };
   const long long ideal = (p.total_units + slots - 1) / slots;
@@ -1490,7 +1483,7 @@ void plan_kv4_decode(Kv4DecodeParams& p, long long slots) {
     int parts = 0;
     for (int i = 0; i < p.n_seqs; ++i) {
       p.seqs[i].part_begin = parts;
-      parts += (kv4_units(p.seqs[i].len) + lo - 1) / lo;
+      parts += (kv4_units(p.seqs[i].len, head_dim) + lo - 1) / lo;
     }
     p.block_parts = parts;
     p.grid = (int32_t)(reps * parts);
