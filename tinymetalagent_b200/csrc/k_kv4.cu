@@ -11,7 +11,6 @@
 #include "te_ptx.cuh"
 #include "te_rope.cuh"
 
-// Decode launch shape.
 namespace te {
 namespace {
 
@@ -1059,23 +1058,27 @@ struct Feed {
 };
 static_assert(sizeof(Feed) <= 56, "feeds in shared memory");
 
-// Moves f to its next stage, or past the end of the CTA's range (false).
+template <int HD>
+__device__ __forceinline__ void feed_enter(const Kv4DecodeParams& p, Feed& f, const Seg& s, int warp) {
+  using D = Dec<HD>;
+  f.u = s.next;
+  f.stage = s.s0 + warp;
+  f.s1 = s.s1;
+  const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
+  f.base = p.pool.base + rec * p.pool.tiles_per_page * D::TB;
+  f.page_bytes = (long long)p.pool.kv_heads * p.pool.tiles_per_page * D::TB;
+  f.row = p.page_table + (size_t)p.seqs[s.si].slot * p.max_pages_per_seq;
+  f.page_base = p.seqs[s.si].page_base;
+  f.page = kv4_page_of(p.pool, f.stage * D::kStageTiles);
+  f.in = f.stage - f.page * p.pool.stages_per_page;
+}
+
+// Moves f to a segment in which it has a stage left; false past the end of the CTA's range.
 template <int HD>
 __device__ __forceinline__ bool feed_seek(const Kv4DecodeParams& p, Feed& f, int warp, int u0, int u1) {
-  using D = Dec<HD>;
   while (f.stage >= f.s1) {
     if (f.u >= u1) return false;
-    const Seg s = kv4_seg_at<HD>(p, f.u, u0, u1);
-    f.u = s.next;
-    f.stage = s.s0 + warp;
-    f.s1 = s.s1;
-    const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
-    f.base = p.pool.base + rec * p.pool.tiles_per_page * D::TB;
-    f.page_bytes = (long long)p.pool.kv_heads * p.pool.tiles_per_page * D::TB;
-    f.row = p.page_table + (size_t)p.seqs[s.si].slot * p.max_pages_per_seq;
-    f.page_base = p.seqs[s.si].page_base;
-    f.page = kv4_page_of(p.pool, f.stage * D::kStageTiles);
-    f.in = f.stage - f.page * p.pool.stages_per_page;
+    feed_enter<HD>(p, f, kv4_seg_at<HD>(p, f.u, u0, u1), warp);
   }
   return true;
 }
@@ -1133,9 +1136,9 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   Feed& feed = *reinterpret_cast<Feed*>(smem + D::feed_off + 64 * warp);
   int* sm_issued = reinterpret_cast<int*>(smem + D::feed_off + 64 * warp + 56);
   bool feeding = false;
+  __syncthreads();
   if (lane == 0) {
-    feed.stage = feed.s1 = 0;
-    feed.u = u_begin;
+    feed_enter<HD>(p, feed, seg(0), warp);
     *sm_issued = 0;
     feeding = feed_seek<HD>(p, feed, warp, u_begin, u1);
     // L2 may fetch the first stage while the previous kernel drains (a hint, coherent with that kernel's writes)
@@ -1144,7 +1147,6 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
                        D::kStageBytes);
     }
   }
-  __syncthreads();
   auto issue = [&](int slot) {  // lane 0
     if (!feeding) return;
     feed_issue<HD>(p, feed, ring + slot * D::kStageBytes, &bars[slot]);
