@@ -519,6 +519,37 @@ def test_decode_more_sequences_than_one_launch_takes(engine):
     cache.close()
 
 
+@pytest.mark.parametrize("hd,group,append", [(64, 3, False), (64, 9, True), (128, 2, True), (128, 8, False)])
+def test_decode_more_groups_than_resident_ctas(engine, hd, group, append):
+    """More (layer, kv head, sequence) groups than the GPU holds CTAs: ranges that begin and end inside groups, CTAs
+    with several groups, empty and one-token sequences between long ones; two launches share the scratch."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(hd + group)
+    layers, kvh, S = 3, 8, 14
+    lens = [1500, 0, 1, 37, 513, 1030, 0, 64, 700, 255, 256, 257, 1200, 5]
+    heads = kvh * group
+    cache = engine.kv4_cache(layers=layers, max_seqs=S, max_tokens_per_seq=1504, kv_heads=kvh, head_dim=hd,
+                             page_tokens=64)
+    kv = [fill(cache, s, rows(rng, layers, m, kvh, hd), rows(rng, layers, m, kvh, hd)) if m else
+          (np.zeros((layers, 0, kvh, hd)),) * 2 for s, m in enumerate(lens)]
+    kw = {}
+    if append:
+        kn, vn = rows(rng, layers, S, kvh, hd), rows(rng, layers, S, kvh, hd)
+        kw = dict(k_new=kn, v_new=vn)
+        kv = [(np.concatenate([k, values(quantise(kn[:, i:i + 1]))], 1),
+               np.concatenate([v, values(quantise(vn[:, i:i + 1]))], 1)) for i, (k, v) in enumerate(kv)]
+    for _ in range(2):
+        q = rows(rng, layers, S, heads, hd)
+        out = run_decode(cache, list(range(S)), q, heads, flags=TE_ATTN_NO_ROPE, **dict(kw))
+        for layer in range(layers):
+            for i in range(S):
+                if kv[i][0].shape[1] == 0:
+                    assert (out[layer, i] == 0).all()
+                else:
+                    check(out[layer, i], q[layer, i], kv[i][0][layer], kv[i][1][layer])
+    cache.close()
+
+
 @pytest.mark.parametrize("cut", [0, 37, 64, 299])
 def test_partial_records_merge_to_the_whole(port, engine, cut):
     """A sequence split over two caches (the second a shard at a position offset): partial records, merged."""

@@ -681,11 +681,11 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
     s.first = 1;
   } else {
     s.gb = (int)blk * per + p.seqs[lo].unit_begin;
-    s.next = min(s.gb + n, u1);
-    a = u - s.gb;
-    b = s.next - s.gb;
+    s.next = min(s.gb + n + kKv4GroupUnits, u1);
+    a = max(u - s.gb - kKv4GroupUnits, 0);
+    b = max(s.next - s.gb - kKv4GroupUnits, 0);
     s.c0 = kv4_cta_of(s.gb, p.total_units, p.grid);
-    s.parts = kv4_cta_of(s.gb + n - 1, p.total_units, p.grid) - s.c0 + 1;
+    s.parts = kv4_cta_of(s.gb + n + kKv4GroupUnits - 1, p.total_units, p.grid) - s.c0 + 1;
     s.first = u == u_begin;
   }
   constexpr int kUnitStages = kKv4Warps, kTokens = kv4_stage_tokens(HD);
@@ -1464,7 +1464,7 @@ void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   for (int i = 0; i < p.n_seqs; ++i) {
     const int n = kv4_units(p.seqs[i].len, head_dim);
     p.seqs[i].unit_begin = acc;
-    acc += n;
+    acc += n + kKv4GroupUnits;
     longest = n > longest ? n : longest;
   }
   p.block_units = acc;
