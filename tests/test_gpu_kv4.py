@@ -430,6 +430,31 @@ def test_decode_extreme_scales(engine, hd, kind):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("small", [2.0 ** -6, 2.0 ** -12])
+@pytest.mark.parametrize("at", [0, 300, 998])
+def test_decode_beside_a_token_of_huge_values(engine, hd, small, at):
+    """A token whose values are 2^17 and more times the others', and whose weight is nothing for the even heads and
+    everything for the odd ones: the even heads' outputs are as exact as without it."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(23)
+    n, heads = 1000, 7
+    k, v, q = rows(rng, 1, n, 1, hd), rows(rng, 1, n, 1, hd, gain=small), rows(rng, 1, 1, heads, hd)
+    k[..., 0] = 0
+    k[0, at] = 0
+    k[0, at, 0, 0] = -400
+    v[0, at] = np.where(rng.random((1, hd)) < 0.5, 1, -1) * 2.0 ** 17
+    q[..., 0::2, 0] = 8
+    q[..., 1::2, 0] = -8
+    cache = engine.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=1, head_dim=hd)
+    kk, vv = fill(cache, 0, k, v)
+    out = run_decode(cache, [0], q, heads, flags=TE_ATTN_NO_ROPE)[0, 0]
+    others = np.arange(n) != at
+    check(out[1::2], q[0, 0, 1::2], kk[0], vv[0])
+    check(out[0::2], q[0, 0, 0::2], kk[0, others], vv[0, others])
+    cache.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("n", [3, 16, 130])
 def test_decode_ignores_what_lies_past_the_length(engine, hd, n):
     """Blocks past the end of the sequence (here NaN and infinite scales, left by a truncation) have no part."""

@@ -720,7 +720,7 @@ __device__ __forceinline__ uint32_t code_magic() {  // opaque to the compiler, s
 // of 1024 is 1024 + c (or + 16 c), and one subtraction leaves a normal number.  Codes read as f16 subnormals
 // would need no subtraction for the keys, but the tensor core aligns the 16 products of a step by their
 // operands' nominal exponents: subnormals lose 7 to 10 bits of the fp32 sum (measured: the output was 8e-6
-// off, against 1e-6 now).
+// off, against less than 1e-6 now).
 __device__ __forceinline__ void centred(uint32_t x, uint32_t magic, uint32_t (&c)[4]) {
   const uint32_t y = x >> 8;
   c[0] = h2_add(and_or(x, 0x000f000fu, magic), 0xe408e408u);
@@ -769,15 +769,14 @@ template <int HD>
 struct WarpState {
   float f;                // S f = score in exp2 units
   float o[HD / 32][2][4];    // O^T accumulators: block, m16 tile
-  float m, l;             // reference exponent and sum of this lane's weights, head g
+  float m;                // head g: reference of the scores, an integer, so that rescaling is exact
   float mb;               // kWeightExp - m
-  float vlim;             // largest |V scale| the current vexp allows
-  uint32_t vmul;          // 2^vexp twice, f16
-  int vexp;
+  float l;                // sum of this lane's weights, head g
 };
 
 constexpr float kSlack = 5.f;      // scores may exceed the reference by this before it moves
-constexpr float kWeightExp = 8.f;  // weights are 2^(score - m + 8): at most 2^13, exact products far above f16's floor
+constexpr float kWeightExp = 9.f;  // weights are 2^(score - m + 9): at most 2^14
+constexpr float kScaleMin = 0x1p-11f, kScaleMax = 2.f;  // V scales for which weight times scale stays within f16
 
 // A query head's raw row, 4 dims a lane (lanes 0-15 at head_dim 64); zeros for a head the group has not.
 template <int HD>
@@ -841,9 +840,6 @@ __device__ __forceinline__ void reset_state(WarpState<HD>& w) {
   w.m = -INFINITY;
   w.mb = INFINITY;
   w.l = 0.f;
-  w.vlim = 0.f;
-  w.vmul = 0;
-  w.vexp = 0;
 }
 
 // Words of a lane: NB per n8 half / token-pair half j.
@@ -950,49 +946,65 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
   top *= w.f;
   const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
   const float vtop = fmaxf(vmf.x, vmf.y);
-  if (__any_sync(0xffffffffu, top > w.m + kSlack || vtop > w.vlim)) {
-    float tm = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
-    float alpha = 1.f;
-    if (tm > w.m + kSlack) {
-      alpha = ex2(w.m - tm);
-      w.m = tm;
-      w.mb = kWeightExp - tm;
-    }
-    float vx = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-    vx = fmaxf(vx, __shfl_xor_sync(0xffffffffu, vx, 2));
-    float beta = 1.f;
-    if (vx > w.vlim) {
-      // scales of 2^-8 .. 4 are used as they are; others are moved so that the largest is in [0.5, 1) now and at
-      // most 4 until it moves again
-      const int e = min(exponent_of(vx), 15);
-      const int k = e >= -8 && e < 2 ? 0 : min(max(-1 - e, -16), 15);
-      beta = w.vlim > 0.f ? pow2i(k - w.vexp) : 1.f;
-      w.vexp = k;
-      w.vlim = k == 0 ? 4.f : pow2i(e + 3);
-      const __half2 h = __float2half2_rn(pow2i(k));
-      w.vmul = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    w.l *= alpha;
-    const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t) * beta;
-    const float a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4) * beta;
+  auto rescale = [&](float x) {  // O times head g's x
+    const float x0 = __shfl_sync(0xffffffffu, x, 8 * t);
+    const float x1 = __shfl_sync(0xffffffffu, x, 8 * t + 4);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        w.o[b][i][0] *= a0;
-        w.o[b][i][1] *= a1;
-        w.o[b][i][2] *= a0;
-        w.o[b][i][3] *= a1;
+        w.o[b][i][0] *= x0;
+        w.o[b][i][1] *= x1;
+        w.o[b][i][2] *= x0;
+        w.o[b][i][3] *= x1;
       }
-  }
-  if (w.vexp != 0) {
+  };
+  int shift = 0;     // O counts 2^shift times during this stage, and l 2^min(shift, 0) times
+  bool odd = false;  // uniform: shift may be other than 0
+  if (__any_sync(0xffffffffu, top > w.m + kSlack || vtop > kScaleMax || vtop < kScaleMin)) {
+    float tm = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
+    float alpha = 1.f;
+    if (tm > w.m + kSlack) {
+      tm = ceilf(tm);
+      alpha = ex2(w.m - tm);
+      w.m = tm;
+      w.mb = kWeightExp - tm;
+    }
+    // Weight times scale has to stay between f16's ends.  With scales of kScaleMin .. kScaleMax it does; smaller ones
+    // are moved up for the stage, and beside a larger one the weights are moved down, by what its own weight asks.
+    float most = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    if (most < kScaleMin) {
+      odd = true;
+      shift = min(-1 - exponent_of(most), 15);
+      const __half2 h = __float2half2_rn(pow2i(shift));
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+      for (int i = 0; i < T; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) vs[i][j][b] = h2_mul(vs[i][j][b], w.vmul);
+          for (int b = 0; b < NB; ++b) vs[i][j][b] = h2_mul(vs[i][j][b], *reinterpret_cast<const uint32_t*>(&h));
+    } else if (most > kScaleMax) {
+      odd = true;
+      most = 0.f;
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t dm = vs[i][j][0];
+#pragma unroll
+          for (int b = 0; b < NB; ++b) dm = h2_maxabs(dm, vs[i][j][b]);
+          const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&dm));
+          most = fmaxf(most, fmaxf(ex2(fmaf(s[i][2 * j], w.f, w.mb)) * d.x, ex2(fmaf(s[i][2 * j + 1], w.f, w.mb)) * d.y));
+        }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      shift = max(min(14 - exponent_of(most), 0), -32);
+      w.mb += (float)shift;
+    }
+    w.l *= alpha * pow2i(min(shift, 0));
+    rescale(alpha * pow2i(shift));
   }
   uint32_t ph[T][2], pl[T][2], vw[T][2][NB];
 #pragma unroll
@@ -1043,6 +1055,11 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
       f2_unpack(f2_add(f2_pack(w.o[b][1][r], w.o[b][1][r + 1]), f2_pack(o1[r], o1[r + 1])), w.o[b][1][r],
                 w.o[b][1][r + 1]);
     }
+  }
+  if (odd) {
+    w.mb = kWeightExp - w.m;
+    w.l *= pow2i(-min(shift, 0));
+    rescale(pow2i(-shift));
   }
 }
 
@@ -1178,7 +1195,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
     const size_t row =
         ((size_t)q.ll * p.seq_total + p.seq_base + q.si) * (p.pool.kv_heads * p.group) + q.kvh * p.group + hg;
     if (p.partial_out) {
-      constexpr float k = 0x1p-8f;  // 2^-kWeightExp
+      const float k = pow2i(-(int)kWeightExp);
       float* o = p.out + row * (HD + 2);
       o[dim] = acc.x * k;
       o[dim + 1] = acc.y * k;
@@ -1274,9 +1291,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
         mx0 = fmaxf(mx0, sm_m[i * H + 2 * t]);
         mx1 = fmaxf(mx1, sm_m[i * H + 2 * t + 1]);
       }
-      const float vs = pow2i(-w.vexp);
-      const float c0 = part_weight(sm_m[warp * H + 2 * t], mx0) * vs;
-      const float c1 = part_weight(sm_m[warp * H + 2 * t + 1], mx1) * vs;
+      const float c0 = part_weight(sm_m[warp * H + 2 * t], mx0), c1 = part_weight(sm_m[warp * H + 2 * t + 1], mx1);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
