@@ -319,6 +319,12 @@ __device__ __forceinline__ void store32(void* base, size_t idx, int f16, const f
 // One warp per (layer, kv head, tile of 16 tokens), one block a lane: the tile is assembled in shared memory (with
 // the tokens it already holds, if the new ones do not fill it) and written whole.  A step's rows are read while the
 // one before is quantised.
+//
+// Bound by bytes with the arithmetic close behind: 36 layers x 2048 tokens x 2 kv heads x 128 binary16 values,
+// stored rows returned, 172 MB, take 35 to 36 us (4.8 TB/s, 0.74 of a plain copy's rate).  Eight lanes a block with
+// a division a value took 80 us, a block a lane with Markstein's step 39, the rows read one step ahead 35.  The
+// compiler's own choice of registers is kept: held to what 5, 6 or 8 CTAs an SM more would need, the row in flight
+// spills (42, 60, 64 us).  A single token (24 layers) is a launch: 2 us on the device.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
@@ -434,6 +440,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
 
 // One warp per (layer, kv head, tile): lane 4g + t expands its K words (dims 8t.. of token g) and V words (dims
 // 4g.. of tokens 2t, 2t + 1), read 16 bytes at a time; a row's pieces leave as whole 32-byte sectors.
+//
+// Bound by the rows it writes: 28 layers x 16384 tokens x 4 kv heads x 128 values as binary16, 1.2 GB in all, take
+// 186 to 190 us (6.4 TB/s, a plain copy's rate); 29 MB of odd range as fp32 6.7 us.  Read a word at a time where it
+// was needed, the large case took 228 us.
 template <int HD>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
@@ -517,6 +527,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsP
 
 // One thread per (layer, token, kv head, block): both sides.  A raw block is
 // 18 bytes, 2-byte aligned: the scale, then byte i = code i | code (i + 16) << 4.
+// For saving and restoring a session; not tuned.
 template <int HD>
 __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int to_pool) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
@@ -609,6 +620,29 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // exactly what the B fragment of O^T wants, so the weights never leave their
 // registers.  The online softmax keeps a reference exponent per head and
 // moves it (rescaling O) only when a score exceeds it by more than 2^5.
+//
+// Split: a warp streams copies of 32 (head_dim 64: 64) tokens through a ring
+// of its own, so no barrier stands in the loop; the CTA's warps merge at the
+// end of a segment, and a group's CTAs through records that the last of them
+// to arrive folds (plan_kv4_decode chooses who takes what).
+//
+// What bounds it is not the bytes but the conversion of the codes and the
+// products they feed: a tile of 16 tokens costs a warp about 370 instructions,
+// 32 of them matrix products of 8 to 9 clocks, and an SM some 180 clocks,
+// where HBM would deliver one in 99.  With the arithmetic taken out the same
+// loop streams 5.9 TB/s.  Measured at head_dim 128, 7 or 8 heads a group:
+//   28 layers x 4 kv heads x 32768 tokens  529 MB  147 us, 3.6 TB/s (copy rate: 81 us)
+//   64 sequences, 8192 tokens at most      153 MB   57 us, 2.7 TB/s (23 us)
+//   36 layers x 2 kv heads x 4097 tokens    43 MB   20 us, 2.2 TB/s (6.6 us)
+//   24 layers x 2 kv heads x 1000 tokens of 64, appending  12 us (0.6 us: latency)
+// Eight warps and two CTAs an SM are the best shape found at 128 registers: six
+// warps x 2 CTAs take 155 us for the first line, 4 x 3 148, 4 x 4 161.  A
+// tcgen05 form (128 rows of codes converted into shared memory, the heads as
+// the N side) was slower: a product of M = 128 takes 53 clocks however few
+// heads there are, and the codes pass shared memory once more (178 to 194 us
+// in four arrangements).  Integer products of the codes (m16n8k32) are as fast
+// as these at twice the depth, but their sums' digits need the shifts and
+// conversions that the codes then save.
 template <int HD>
 struct Dec {
   static constexpr int kWarps = kKv4Warps, kCtas = 2;
@@ -1484,7 +1518,12 @@ void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   }
   p.block_units = acc;
   p.total_units = reps * acc;
-  // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once.
+  // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once;
+  // otherwise the stream split, whose CTAs take equal ranges across groups.  A CTA with one segment saves the merges
+  // between segments, an uneven share costs its full length: aligned is taken while its longest part is within an
+  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens (4 units, 4 on
+  // average) 20.0 against 22.4 us, x 8000 30.5 against 32.5, a ragged batch 13.1 against 15.3; 28 layers x 4 kv heads
+  // x 6000 (12 of 9.5) 41.7 against 38.1, x 32768 185 against 147, 64 ragged sequences 80 against 57.
   auto parts_for = [&](int most) {
     long long c = 0;
     for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len, head_dim) + most - 1) / most;
