@@ -628,25 +628,29 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 //
 // What bounds it is not the bytes but the conversion of the codes and the
 // products they feed: a tile of 16 tokens costs a warp about 370 instructions,
-// 32 of them matrix products of 8 to 9 clocks, and an SM some 180 clocks,
-// where HBM would deliver one in 99.  With the arithmetic taken out the same
-// loop streams 5.9 TB/s.  Measured at head_dim 128, 7 or 8 heads a group:
-//   28 layers x 4 kv heads x 32768 tokens  529 MB  147 us, 3.6 TB/s (copy rate: 81 us)
-//   64 sequences, 8192 tokens at most      153 MB   57 us, 2.7 TB/s (23 us)
+// 32 of them matrix products of 9 clocks, and an SM some 160 clocks with the
+// copies taken out, where HBM would deliver one in 99; with the arithmetic
+// taken out the same loop streams 5.9 TB/s.  Measured at head_dim 128, 7 or 8
+// heads a group:
+//   28 layers x 4 kv heads x 32768 tokens  529 MB  138 us, 3.8 TB/s (copy rate: 81 us)
+//   64 sequences, 8192 tokens at most      153 MB   55 us, 2.8 TB/s (23 us)
 //   36 layers x 2 kv heads x 4097 tokens    43 MB   20 us, 2.2 TB/s (6.6 us)
 //   24 layers x 2 kv heads x 1000 tokens of 64, appending  12 us (0.6 us: latency)
-// Eight warps and two CTAs an SM are the best shape found at 128 registers: six
-// warps x 2 CTAs take 155 us for the first line, 4 x 3 148, 4 x 4 161.  A
-// tcgen05 form (128 rows of codes converted into shared memory, the heads as
-// the N side) was slower: a product of M = 128 takes 53 clocks however few
-// heads there are, and the codes pass shared memory once more (178 to 194 us
-// in four arrangements).  Integer products of the codes (m16n8k32) are as fast
-// as these at twice the depth, but their sums' digits need the shifts and
-// conversions that the codes then save.
+// Shapes: at head_dim 128, four warps x 2 CTAs with 64 tokens a step and 255
+// registers take 138 us for the first line, 16 warps with 32 tokens 147 (12
+// warps 147 too, 20 and 24 warps with 16 tokens 171 and 180); one CTA of eight
+// warps 142, and 58 for the second line, but 19.4 for the third.  At head_dim
+// 64 eight warps x 2 CTAs take 14.1 us for 24 layers x 8192 tokens, four x 2
+// 15.2, four x 4 15.7.  A tcgen05 form (128 rows of codes converted into shared
+// memory, the heads as the N side) was slower: a product of M = 128 takes 53
+// clocks however few heads there are, and the codes pass shared memory once
+// more (178 to 194 us in four arrangements).  Integer products of the codes
+// (m16n8k32) are as fast as these at twice the depth, but their sums' digits
+// need the shifts and conversions that the codes then save.
 template <int HD>
 struct Dec {
-  static constexpr int kWarps = kKv4Warps, kCtas = 2;
-  static constexpr int kStageTiles = kv4_stage_tiles(HD), kStageTokens = kv4_stage_tokens(HD);
+  static constexpr int kWarps = kv4_warps(HD), kCtas = 2;
+  static constexpr int kStageTiles = kKv4StageTiles, kStageTokens = kKv4StageTokens;
   static constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD);
   static constexpr int kStageBytes = kStageTiles * TB;
   static constexpr int NB = HD / 32;
@@ -722,7 +726,7 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
     s.parts = kv4_cta_of(s.gb + n + kKv4GroupUnits - 1, p.total_units, p.grid) - s.c0 + 1;
     s.first = u == u_begin;
   }
-  constexpr int kUnitStages = kKv4Warps, kTokens = kv4_stage_tokens(HD);
+  constexpr int kUnitStages = kv4_warps(HD), kTokens = kKv4StageTokens;
   s.s0 = a * kUnitStages;
   s.s1 = min(b * kUnitStages, (len + kTokens - 1) / kTokens);
   s.last = b == n;
@@ -930,19 +934,30 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
         const uint4 x = lds128(qf + (b * 2 + st) * 512 + lane * 16);
         qa[st][0] = x.x; qa[st][1] = x.y; qa[st][2] = x.z; qa[st][3] = x.w;
       }
+      // all conversions of the block, then its products: the registers of a product's codes are not written
+      // again right behind it (12 clocks a product instead of 9)
+      uint32_t c[T][2][4];
+      float acc[T][2][4];
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) centred(kw[i][j][b], magic, c[i][j]);
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma_zero(acc[i][j], qa[0], c[i][j][0], c[i][j][1]);
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma_add(acc[i][j], qa[1], c[i][j][2], c[i][j][3]);
 #pragma unroll
       for (int i = 0; i < T; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          uint32_t c[4];
-          centred(kw[i][j][b], magic, c);
-          float acc[4];
-          mma_zero(acc, qa[0], c[0], c[1]);
-          mma_add(acc, qa[1], c[2], c[3]);
           const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ks[i][j][b]));
           const uint64_t d2 = f2_pack(d.x, d.y);
-          s2[i][j] = b == 0 ? f2_mul(d2, f2_pack(acc[0], acc[1])) : f2_fma(d2, f2_pack(acc[0], acc[1]), s2[i][j]);
-          s2[i][j] = f2_fma(d2, f2_pack(acc[2], acc[3]), s2[i][j]);
+          const uint64_t hi = f2_pack(acc[i][j][0], acc[i][j][1]), lo = f2_pack(acc[i][j][2], acc[i][j][3]);
+          s2[i][j] = f2_fma(d2, lo, b == 0 ? f2_mul(d2, hi) : f2_fma(d2, hi, s2[i][j]));
         }
     }
 #pragma unroll
@@ -1059,28 +1074,32 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
     // the tiles' products start from zero and join O by a rounded fp32 addition: a long accumulation inside
     // the tensor core truncates at every step
     float o0[4], o1[4];
+    uint32_t hi[T][2], lo[T][2], ca[T][4], cc[T][4];  // as for the keys: all conversions first
 #pragma unroll
     for (int i = 0; i < T; ++i) {
-      uint32_t hi[2], lo[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t d = vs[i][j][b];
-        hi[j] = h2_mul(ph[i][j], d);
-        lo[j] = h2_fma(pl[i][j], d, h2_fms(ph[i][j], d, hi[j]));
+        hi[i][j] = h2_mul(ph[i][j], d);
+        lo[i][j] = h2_fma(pl[i][j], d, h2_fms(ph[i][j], d, hi[i][j]));
       }
       uint32_t c0[4], c1[4];
       centred(vw[i][0][b], magic, c0);
       centred(vw[i][1][b], magic, c1);
-      const uint32_t a[4] = {c0[0], c0[1], c1[0], c1[1]}, c[4] = {c0[2], c0[3], c1[2], c1[3]};
+      ca[i][0] = c0[0]; ca[i][1] = c0[1]; ca[i][2] = c1[0]; ca[i][3] = c1[1];
+      cc[i][0] = c0[2]; cc[i][1] = c0[3]; cc[i][2] = c1[2]; cc[i][3] = c1[3];
+    }
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
       if (i == 0) {
-        mma_zero(o0, a, lo[0], lo[1]);
-        mma_zero(o1, c, lo[0], lo[1]);
+        mma_zero(o0, ca[i], lo[i][0], lo[i][1]);
+        mma_zero(o1, cc[i], lo[i][0], lo[i][1]);
       } else {
-        mma_add(o0, a, lo[0], lo[1]);
-        mma_add(o1, c, lo[0], lo[1]);
+        mma_add(o0, ca[i], lo[i][0], lo[i][1]);
+        mma_add(o1, cc[i], lo[i][0], lo[i][1]);
       }
-      mma_add(o0, a, hi[0], hi[1]);
-      mma_add(o1, c, hi[0], hi[1]);
+      mma_add(o0, ca[i], hi[i][0], hi[i][1]);
+      mma_add(o1, cc[i], hi[i][0], hi[i][1]);
     }
 #pragma unroll
     for (int r = 0; r < 4; r += 2) {
@@ -1505,7 +1524,7 @@ cudaError_t launch_rows(void (*kernel)(Kv4RowsParams), const Kv4RowsParams& p, c
 
 }  // namespace
 
-int kv4_decode_ctas_per_sm() { return Dec<128>::kCtas; }
+int kv4_decode_ctas_per_sm(int head_dim) { return head_dim == 128 ? Dec<128>::kCtas : Dec<64>::kCtas; }
 
 void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   const long long reps = (long long)p.n_layers * p.pool.kv_heads * p.head_blocks;
@@ -1521,9 +1540,9 @@ void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once;
   // otherwise the stream split, whose CTAs take equal ranges across groups.  A CTA with one segment saves the merges
   // between segments, an uneven share costs its full length: aligned is taken while its longest part is within an
-  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens (4 units, 4 on
-  // average) 20.0 against 22.4 us, x 8000 30.5 against 32.5, a ragged batch 13.1 against 15.3; 28 layers x 4 kv heads
-  // x 6000 (12 of 9.5) 41.7 against 38.1, x 32768 185 against 147, 64 ragged sequences 80 against 57.
+  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens 19.9 against
+  // 23.9 us, x 8000 28.6 against 32.1, a ragged batch of 8 12.8 against 17.7; where the rule says stream, 28 layers x
+  // 4 kv heads x 6000 39.1 against 36.8, x 32768 173 against 138, 64 ragged sequences 75 against 55.
   auto parts_for = [&](int most) {
     long long c = 0;
     for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len, head_dim) + most - 1) / most;

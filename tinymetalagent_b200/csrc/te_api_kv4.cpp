@@ -36,9 +36,9 @@ Kv4Pool pool_of(const te_kv4_cache* c) {
   p.page_tokens = (int32_t)c->b.d.page_tokens;
   p.tiles_per_page = (int32_t)(c->b.d.page_tokens / kKv4Tile);
   p.tpp_magic = (uint32_t)(((1ull << 32) + (uint64_t)p.tiles_per_page - 1) / (uint64_t)p.tiles_per_page);
-  p.stages_per_page = p.tiles_per_page / kv4_stage_tiles((int)c->b.d.head_dim);
-  p.step_pages = kKv4Warps / p.stages_per_page;
-  p.step_in = kKv4Warps % p.stages_per_page;
+  p.stages_per_page = p.tiles_per_page / kKv4StageTiles;
+  p.step_pages = kv4_warps((int)c->b.d.head_dim) / p.stages_per_page;
+  p.step_in = kv4_warps((int)c->b.d.head_dim) % p.stages_per_page;
   return p;
 }
 
@@ -400,7 +400,7 @@ TE_API te_status te_kv4_attention_decode(te_kv4_cache* c, size_t layer_begin, si
     }
     p.n_seqs = (int32_t)nb;
     p.seq_base = (int32_t)base;
-    plan_kv4_decode(p, (int)hd, (long long)e->sm_count * kv4_decode_ctas_per_sm());
+    plan_kv4_decode(p, (int)hd, (long long)e->sm_count * kv4_decode_ctas_per_sm((int)hd));
     const size_t groups = n_layers * hkv * (size_t)p.head_blocks * nb;
     if (p.total_units > (long long)INT32_MAX || groups > (size_t)INT32_MAX) {
       return fail(e, TE_STATUS_UNSUPPORTED, "decode call too large");

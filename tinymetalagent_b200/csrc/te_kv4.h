@@ -32,17 +32,17 @@
 namespace te {
 
 constexpr int kKv4Tile = 16;        // tokens of a tile
-constexpr int kKv4Warps = 8;        // warps of a decode CTA, each with its own copies
-// Tiles of a decode copy: 4.5 KB, 32 tokens at head_dim 128 and 64 at 64 (two tiles a step leave the smaller rows'
-// step half overhead: 24 layers x 8192 tokens took 15.7 us against 14.5, a ragged batch 19.1 against 15.6; a single
-// tile at 128 cost 168 us against 162 over 28 layers x 32768 tokens).
-__host__ __device__ constexpr int kv4_stage_tiles(int hd) { return 256 / hd; }
-__host__ __device__ constexpr int kv4_stage_tokens(int hd) { return kv4_stage_tiles(hd) * kKv4Tile; }
+// A decode copy, and what a warp attends at a time: 64 tokens, 9 KB at head_dim 128.  Fewer leave too little
+// independent work beside each product (28 layers x 32768 tokens of 128: 139 us, 32 tokens 147, 16 tokens 171 or
+// more; 24 layers x 8192 of 64: 14.2, 32 tokens 15.7).
+constexpr int kKv4StageTiles = 4, kKv4StageTokens = kKv4StageTiles * kKv4Tile;
+// Warps of a decode CTA, each with its own copies; two CTAs fit an SM.
+__host__ __device__ constexpr int kv4_warps(int hd) { return hd == 128 ? 4 : 8; }
 // What a group's queries and merge cost, in units: the stream split counts them before the group's own (a ragged
-// batch of 64 took 59.0 us without, 57.1 with one, 56.0 with two; 32 short ones 15.5, 14.4, 14.5).
-constexpr int kKv4GroupUnits = 1;
+// batch of 64: 56.3 us with one, 54.9 with two, 56.6 with three; 28 layers x 6000 tokens 38.1, 36.8, 39.0).
+constexpr int kKv4GroupUnits = 2;
 // Work unit of the decode split: one copy for each warp.
-__host__ __device__ constexpr int kv4_unit(int hd) { return kv4_stage_tokens(hd) * kKv4Warps; }
+__host__ __device__ constexpr int kv4_unit(int hd) { return kKv4StageTokens * kv4_warps(hd); }
 constexpr int kKv4Heads = 8;        // query heads of a work group (larger groups take several)
 constexpr int kKv4MaxSeqs = 64;     // sequences per decode launch
 
@@ -65,7 +65,7 @@ struct Kv4Pool {
   int32_t tiles_per_page;
   uint32_t tpp_magic;       // ceil(2^32 / tiles_per_page)
   int32_t stages_per_page;  // decode copies of a page
-  int32_t step_pages, step_in;  // kKv4Warps stages on: whole pages, and stages past them
+  int32_t step_pages, step_in;  // kv4_warps stages on: whole pages, and stages past them
   int32_t page_tokens;
 };
 
@@ -116,7 +116,7 @@ constexpr int kv4_record_floats(int hd) { return kKv4Heads * hd + 2 * kKv4Heads;
 // Plans the split of p's work over `slots` resident CTAs (fills the sequences' units and parts, block_units,
 // block_parts, total_units, grid).
 void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots);
-int kv4_decode_ctas_per_sm();
+int kv4_decode_ctas_per_sm(int head_dim);
 cudaError_t launch_kv4_decode(const Kv4DecodeParams& p, int head_dim, cudaStream_t s);
 
 struct Kv4RowsParams {
