@@ -498,9 +498,9 @@ TE_API te_status te_kv4_cache_read_q4_0(te_kv4_cache *cache, size_t layer_begin,
  * fp32.  Partial records (TE_ATTN_PARTIAL) have te_attention_decode's layout
  * and meaning, except that m is a reference of the row that lies near its
  * largest score (at most 5 below it, less than 1 above), instead of the score
- * itself: te_attention_merge_partials takes both.  Results are bit-identical across
- * repeated calls.  Flags: TE_ATTN_ADVANCE, TE_ATTN_PARTIAL, TE_ATTN_NO_ROPE,
- * TE_ATTN_QKV_BIAS, TE_ATTN_INPUT_F16. */
+ * itself: te_attention_merge_partials takes both.  Results are bit-identical
+ * across repeated calls.  Flags: TE_ATTN_ADVANCE, TE_ATTN_PARTIAL,
+ * TE_ATTN_NO_ROPE, TE_ATTN_QKV_BIAS, TE_ATTN_INPUT_F16. */
 TE_API te_status te_kv4_attention_decode(te_kv4_cache *cache, size_t layer_begin, size_t n_layers,
                                          const uint32_t *seq_ids, size_t n_seqs, const int64_t *q_positions,
                                          const void *q, const void *k_new, const void *v_new, size_t heads,
