@@ -632,16 +632,16 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // copies taken out, where HBM would deliver one in 99; with the arithmetic
 // taken out the same loop streams 5.9 TB/s.  Measured at head_dim 128, 7 or 8
 // heads a group:
-//   28 layers x 4 kv heads x 32768 tokens  529 MB  138 us, 3.8 TB/s (copy rate: 81 us)
-//   64 sequences, 8192 tokens at most      153 MB   55 us, 2.8 TB/s (23 us)
-//   36 layers x 2 kv heads x 4097 tokens    43 MB   20 us, 2.2 TB/s (6.6 us)
+//   28 layers x 4 kv heads x 32768 tokens  529 MB  136 us, 3.9 TB/s (copy rate: 81 us)
+//   64 sequences, 8192 tokens at most      153 MB   54 us, 2.9 TB/s (23 us)
+//   36 layers x 2 kv heads x 4097 tokens    43 MB   19 us, 2.3 TB/s (6.6 us)
 //   24 layers x 2 kv heads x 1000 tokens of 64, appending  12 us (0.6 us: latency)
 // Shapes: at head_dim 128, four warps x 2 CTAs with 64 tokens a step and 255
-// registers take 138 us for the first line, 16 warps with 32 tokens 147 (12
-// warps 147 too, 20 and 24 warps with 16 tokens 171 and 180); one CTA of eight
-// warps 142, and 58 for the second line, but 19.4 for the third.  At head_dim
-// 64 eight warps x 2 CTAs take 14.1 us for 24 layers x 8192 tokens, four x 2
-// 15.2, four x 4 15.7.  A tcgen05 form (128 rows of codes converted into shared
+// registers take 136 us for the first line, one CTA of eight warps 142 (58 and
+// 19.5 for the next two); when the shape was chosen it took 138, 16 warps with
+// 32 tokens 147 (12 warps 147 too), 20 and 24 warps with 16 tokens 171 and 180.
+// At head_dim 64 eight warps x 2 CTAs take 14.1 us for 24 layers x 8192 tokens,
+// four x 2 15.3, four x 4 15.7.  A tcgen05 form (128 rows of codes converted into shared
 // memory, the heads as the N side) was slower: a product of M = 128 takes 53
 // clocks however few heads there are, and the codes pass shared memory once
 // more (178 to 194 us in four arrangements).  Integer products of the codes
@@ -1433,43 +1433,58 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
       // only the group's first part can
       const int slot0 = aligned || stage_start(q.c0, p.total_units, p.grid) >= q.gb ? 0 : 1;
       auto rec_of = [&](int k) { return p.partials + ((size_t)(q.c0 + k) * 2 + (k == 0 ? slot0 : 0)) * rec; };
-      for (int j = threadIdx.x; j < D::kItems; j += 32 * W) {
-        const int head = 2 * (j & 3) + ((j >> 5) & 1);
-        const int dim = 32 * (j >> 6) + 4 * ((j & 31) >> 2);
-        // eight records at a time, all of their loads in flight together; the running state is rescaled per batch
-        constexpr int kBatch = 8;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float top = -INFINITY, sum = 0.f;
-        for (int k0 = 0; k0 < q.parts; k0 += kBatch) {
-          float m[kBatch], l[kBatch];
-          float4 x[kBatch];
+      // a thread's items belong to one head; eight records at a time, all of their loads in flight together, and the
+      // running state is rescaled per batch
+      constexpr int kBatch = 8, kPer = (D::kItems + 32 * W - 1) / (32 * W);
+      static_assert((D::kItems % (32 * W) == 0 || kPer == 1) && W % 2 == 0, "items of a thread");
+      const int head = 2 * (threadIdx.x & 3) + ((threadIdx.x >> 5) & 1);
+      float4 acc[kPer];
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            const bool have = k0 + k < q.parts;
-            const float* r = rec_of(have ? k0 + k : 0);
-            m[k] = have ? __ldcg(r + H * HD + head) : -INFINITY;
-            l[k] = __ldcg(r + H * HD + H + head);
-            x[k] = __ldcg(reinterpret_cast<const float4*>(r) + j);
-          }
-          float all = top;
+      for (int n = 0; n < kPer; ++n) acc[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      float top = -INFINITY, sum = 0.f;
+      const int parts = threadIdx.x < D::kItems ? q.parts : 0;
+      for (int k0 = 0; k0 < parts; k0 += kBatch) {
+        float m[kBatch], l[kBatch];
+        float4 x[kBatch][kPer];
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k) all = fmaxf(all, m[k]);
-          const float keep = part_weight(top, all);
-          acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-          sum *= keep;
-          top = all;
+        for (int k = 0; k < kBatch; ++k) {
+          const bool have = k0 + k < q.parts;
+          const float* r = rec_of(have ? k0 + k : 0);
+          m[k] = have ? __ldcg(r + H * HD + head) : -INFINITY;
+          l[k] = __ldcg(r + H * HD + H + head);
 #pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            if (k0 + k >= q.parts) continue;
-            const float e = part_weight(m[k], all);
-            acc.x = fmaf(e, x[k].x, acc.x);
-            acc.y = fmaf(e, x[k].y, acc.y);
-            acc.z = fmaf(e, x[k].z, acc.z);
-            acc.w = fmaf(e, x[k].w, acc.w);
-            sum = fmaf(e, l[k], sum);
+          for (int n = 0; n < kPer; ++n) {
+            x[k][n] = __ldcg(reinterpret_cast<const float4*>(r) + threadIdx.x + n * 32 * W);
           }
         }
-        write_out(q, head, dim, acc, top, sum);
+        float all = top;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) all = fmaxf(all, m[k]);
+        const float keep = part_weight(top, all);
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+          acc[n].x *= keep; acc[n].y *= keep; acc[n].z *= keep; acc[n].w *= keep;
+        }
+        sum *= keep;
+        top = all;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (k0 + k >= q.parts) continue;
+          const float e = part_weight(m[k], all);
+#pragma unroll
+          for (int n = 0; n < kPer; ++n) {
+            acc[n].x = fmaf(e, x[k][n].x, acc[n].x);
+            acc[n].y = fmaf(e, x[k][n].y, acc[n].y);
+            acc[n].z = fmaf(e, x[k][n].z, acc[n].z);
+            acc[n].w = fmaf(e, x[k][n].w, acc[n].w);
+          }
+          sum = fmaf(e, l[k], sum);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) {
+        const int j = threadIdx.x + n * 32 * W;
+        if (j < D::kItems) write_out(q, head, 32 * (j >> 6) + 4 * ((j & 31) >> 2), acc[n], top, sum);
       }
       if (threadIdx.x == 0) p.counters[q.group_id] = 0;
     }
@@ -1540,9 +1555,9 @@ void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once;
   // otherwise the stream split, whose CTAs take equal ranges across groups.  A CTA with one segment saves the merges
   // between segments, an uneven share costs its full length: aligned is taken while its longest part is within an
-  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens 19.9 against
-  // 23.9 us, x 8000 28.6 against 32.1, a ragged batch of 8 12.8 against 17.7; where the rule says stream, 28 layers x
-  // 4 kv heads x 6000 39.1 against 36.8, x 32768 173 against 138, 64 ragged sequences 75 against 55.
+  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens 19.1 against
+  // 22.2 us, x 8000 27.8 against 31.1, a ragged batch of 8 11.9 against 15.9; where the rule says stream, 28 layers x
+  // 4 kv heads x 6000 38.0 against 35.3, x 32768 172 against 136, 64 ragged sequences 75 against 54.
   auto parts_for = [&](int most) {
     long long c = 0;
     for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len, head_dim) + most - 1) / most;

@@ -39,7 +39,7 @@ constexpr int kKv4StageTiles = 4, kKv4StageTokens = kKv4StageTiles * kKv4Tile;
 // Warps of a decode CTA, each with its own copies; two CTAs fit an SM.
 __host__ __device__ constexpr int kv4_warps(int hd) { return hd == 128 ? 4 : 8; }
 // What a group's queries and merge cost, in units: the stream split counts them before the group's own (a ragged
-// batch of 64: 56.3 us with one, 54.9 with two, 56.6 with three; 28 layers x 6000 tokens 38.1, 36.8, 39.0).
+// batch of 64: 54.9 us with one, 53.6 with two, 55.3 with three; 28 layers x 6000 tokens 36.5, 35.3, 38.1).
 constexpr int kKv4GroupUnits = 2;
 // Work unit of the decode split: one copy for each warp.
 __host__ __device__ constexpr int kv4_unit(int hd) { return kKv4StageTokens * kv4_warps(hd); }
