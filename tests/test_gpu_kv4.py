@@ -238,6 +238,36 @@ def test_append_returns_what_it_stored(engine, hd, f16):
     cache.close()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("f16,out16", [(False, True), (True, False), (False, False), (True, True)])
+@pytest.mark.parametrize("first,n", [(0, 1), (5, 40), (13, 3), (16, 77)])
+def test_append_returns_either_type_from_either(engine, hd, f16, out16, first, n):
+    """Returned rows of the other type, single tokens and ranges that start inside a tile; what lies around the
+    returned rows stays as it was."""
+    from tinymetalagent_b200 import TE_ATTN_ADVANCE, TE_ATTN_INPUT_F16, TE_ATTN_OUTPUT_F16
+    import torch
+    rng = np.random.default_rng(31)
+    kvh, layers = 3, 2
+    cache = engine.kv4_cache(layers=layers, max_seqs=1, max_tokens_per_seq=128, kv_heads=kvh, head_dim=hd)
+    if first:
+        fill(cache, 0, rows(rng, layers, first, kvh, hd), rows(rng, layers, first, kvh, hd))
+    typ, out_type = np.float16 if f16 else np.float32, torch.float16 if out16 else torch.float32
+    kd, vd = dev(rows(rng, layers, n, kvh, hd).astype(typ)), dev(rows(rng, layers, n, kvh, hd).astype(typ))
+    count = layers * n * kvh * hd
+    room = [torch.full((count + 64,), 7.0, device="cuda", dtype=out_type) for _ in range(2)]
+    back = [torch.zeros(count, device="cuda", dtype=out_type) for _ in range(2)]
+    ready(engine)
+    flags = TE_ATTN_OUTPUT_F16 if out16 else 0
+    cache.append(0, layers, 0, kd, vd, n, room[0][32:-32], room[1][32:-32],
+                 flags=TE_ATTN_ADVANCE | flags | (TE_ATTN_INPUT_F16 if f16 else 0))
+    cache.read(0, layers, 0, first, n, back[0], back[1], flags=flags)
+    engine.synchronize()
+    for r, b in zip(room, back):
+        assert torch.equal(r[32:-32], b)
+        assert (r[:32] == 7).all() and (r[-32:] == 7).all()
+    cache.close()
+
+
 @pytest.mark.parametrize("f16", [False, True])
 def test_append_takes_columns_of_a_wider_output(engine, f16):
     from tinymetalagent_b200 import TE_ATTN_ADVANCE, TE_ATTN_INPUT_F16, TE_ATTN_NO_ROPE

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "te_internal.h"
 #include "te_kv4.h"
@@ -268,19 +269,23 @@ __device__ __forceinline__ __half q4_quantise32(float (&x)[32]) {
   return d;
 }
 
-// Codes i0 .. i0 + 3 as bits 0, s1, s2, s3 and up, from c - 8 in fp32: 2^23 + 8 + (c - 8) holds c in its low bits.
-__device__ __forceinline__ uint32_t q4_bits(const float (&x)[32], int i0, int s1, int s2, int s3) {
-  auto c = [&](int i) { return __float_as_uint(x[i] + 8388616.f) - 0x4b000000u; };
-  return c(i0) + (c(i0 + 1) << s1) + (c(i0 + 2) << s2) + (c(i0 + 3) << s3);
+// Four codes as the low 16 bits of an fp32 number, from c - 8 in fp32: 2^23 + sum 16^i (c_i - 8 + 8) is exact.
+constexpr float kNibbles = 8388608.f + 0x8888;
+__device__ __forceinline__ uint32_t q4_half(float a, float b, float c, float d) {
+  return __float_as_uint(fmaf(d, 4096.f, fmaf(c, 256.f, fmaf(b, 16.f, a + kNibbles))));
+}
+// The K word of dims x[i0] .. x[i0 + 7]: even dims in its low half, odd ones in its high half.
+__device__ __forceinline__ uint32_t q4_word(const float (&x)[32], int i0) {
+  uint64_t v = f2_add(f2_pack(x[i0], x[i0 + 1]), f2_pack(kNibbles, kNibbles));
+  v = f2_fma(f2_pack(x[i0 + 2], x[i0 + 3]), f2_pack(16.f, 16.f), v);
+  v = f2_fma(f2_pack(x[i0 + 4], x[i0 + 5]), f2_pack(256.f, 256.f), v);
+  v = f2_fma(f2_pack(x[i0 + 6], x[i0 + 7]), f2_pack(4096.f, 4096.f), v);
+  float lo, hi;
+  f2_unpack(v, lo, hi);
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
 // 32 consecutive values of a binary16 (64 bytes) or fp32 (128 bytes) row, as read and as fp32.
-template <bool F16>
-__device__ __forceinline__ void fetch32(const void* base, size_t idx, uint4 (&u)[F16 ? 4 : 8]) {
-  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + idx * (F16 ? 2 : 4));
-#pragma unroll
-  for (int i = 0; i < (F16 ? 4 : 8); ++i) u[i] = p[i];
-}
 template <bool F16>
 __device__ __forceinline__ void widen32(const uint4 (&u)[F16 ? 4 : 8], float (&x)[32]) {
   if constexpr (F16) {
@@ -301,35 +306,55 @@ __device__ __forceinline__ void widen32(const uint4 (&u)[F16 ? 4 : 8], float (&x
     }
   }
 }
-__device__ __forceinline__ void store32(void* base, size_t idx, int f16, const float (&x)[32]) {
-  if (f16) {
-    uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<__half*>(base) + idx);
+// Byte of piece i % C of block i / C in a step's rows: C pieces of 16 bytes a block, swizzled so that neither a warp's 32
+// consecutive pieces nor the pieces of the same number of its 32 blocks meet in a bank.
+template <int C>
+__device__ __forceinline__ int row_piece(int i) {
+  const int l = i / C;
+  return (l * C + ((i % C) ^ (C == 4 ? (l >> 1) & 3 : l & 7))) * 16;
+}
+// The lane's block into a step's rows.
+template <bool F16>
+__device__ __forceinline__ void put32(unsigned char* buf, int lane, const float (&x)[32]) {
+  constexpr int C = F16 ? 4 : 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i] = make_uint4(pack_half2(x[8 * i], x[8 * i + 1]), pack_half2(x[8 * i + 2], x[8 * i + 3]),
-                        pack_half2(x[8 * i + 4], x[8 * i + 5]), pack_half2(x[8 * i + 6], x[8 * i + 7]));
+  for (int i = 0; i < C; ++i) {
+    uint4 u;
+    if constexpr (F16) {
+      u = make_uint4(pack_half2(x[8 * i], x[8 * i + 1]), pack_half2(x[8 * i + 2], x[8 * i + 3]),
+                     pack_half2(x[8 * i + 4], x[8 * i + 5]), pack_half2(x[8 * i + 6], x[8 * i + 7]));
+    } else {
+      u = make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]), __float_as_uint(x[4 * i + 2]),
+                     __float_as_uint(x[4 * i + 3]));
     }
-  } else {
-    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + idx);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    *reinterpret_cast<uint4*>(buf + row_piece<C>(lane * C + i)) = u;
   }
+}
+// An fp32 block straight to memory.
+__device__ __forceinline__ void store32(void* base, size_t idx, const float (&x)[32]) {
+  float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + idx);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
 }
 
 // One warp per (layer, kv head, tile of 16 tokens), one block a lane: the tile is assembled in shared memory (with
-// the tokens it already holds, if the new ones do not fill it) and written whole.  A step's rows are read while the
-// one before is quantised.
+// the tokens it already holds, if the new ones do not fill it) and written whole.  Rows come in, and stored rows go
+// out, through shared memory, so that a warp's accesses are whole rows while a lane's work is a block.
 //
-// Bound by bytes with the arithmetic close behind: 36 layers x 2048 tokens x 2 kv heads x 128 binary16 values,
-// stored rows returned, 172 MB, take 35 to 36 us (4.8 TB/s, 0.74 of a plain copy's rate).  Eight lanes a block with
-// a division a value took 80 us, a block a lane with Markstein's step 39, the rows read one step ahead 35.  The
-// compiler's own choice of registers is kept: held to what 5, 6 or 8 CTAs an SM more would need, the row in flight
-// spills (42, 60, 64 us).  A single token (24 layers) is a launch: 2 us on the device.
+// Bound by bytes: 36 layers x 2048 tokens x 2 kv heads x 128 values, stored rows returned in the same type, take
+// 33.2 us as binary16 (172 MB, 5.2 TB/s, 0.79 of a plain copy's rate; a seventh is ramp and tail) and 52.4 us as fp32
+// (323 MB, 6.2 TB/s); at 64 dims 18.9 and 27.5 us.  Eight lanes a block with a division a value took 80 us for the
+// first, a block a lane with Markstein's step 39, each lane reading its own block one step ahead 34.7 (fp32: 85.0,
+// 64 dims 20.6 and 44.8), codes joined in the FMA pipe 34.2.  Four CTAs an SM: held to the registers of five or six,
+// the values spill (37 to 43 us).  A single token (24 layers) is a launch: 2 us on the device.
 template <int HD, bool F16>
-__global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4RowsParams p) {
+__global__ void __launch_bounds__(32 * kRowWarps, 4) kv4_append_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
   constexpr int kTokens = 32 / NB;  // tokens of a warp's step
+  // rows come in by asynchronous copies of 16-byte pieces, whole rows at a time, kBufs steps ahead
+  constexpr int kChunks = F16 ? 4 : 8, kStepBytes = 32 * 16 * kChunks, kBufs = F16 ? 4 : 2;
   __shared__ __align__(16) unsigned char tiles[kRowWarps][TB];
+  __shared__ __align__(16) unsigned char bufs[kRowWarps][kBufs][kStepBytes];
   griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = p.first / kKv4Tile;
@@ -354,26 +379,53 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
   const int b = lane % NB;
   const size_t brow = ((size_t)layer * p.pool.kv_heads + kvh) * HD + 32 * b;
   constexpr int kSteps = 2 * kKv4Tile / kTokens;
-  uint4 raw[F16 ? 4 : 8];
-  auto fetch = [&](int step) {
-    const int slot = (step % (kSteps / 2)) * kTokens + lane / NB;
-    if (step < kSteps && slot >= lo && slot < hi) {
-      const long long row = (long long)ll * p.n_tokens + (tile * kKv4Tile + slot - p.first);
-      fetch32<F16>(step >= kSteps / 2 ? p.v : p.k, (size_t)(row * p.token_stride) + (size_t)kvh * HD + 32 * b, raw);
+  // the pieces of a step's rows that this lane copies in or out, C to a block: calls f(its byte in the buffer, token
+  // row, byte from the head's first value)
+  auto pieces = [&](auto chunks, int step, auto f) {
+    constexpr int C = chunks;
+#pragma unroll
+    for (int n = 0; n < C; ++n) {
+      const int i = n * 32 + lane, slot = (step % (kSteps / 2)) * kTokens + i / (NB * C);
+      if (slot >= lo && slot < hi) {
+        f(row_piece<C>(i), (long long)ll * p.n_tokens + (tile * kKv4Tile + slot - p.first), i % (NB * C) * 16);
+      }
     }
   };
-  fetch(0);
+  using In = std::integral_constant<int, kChunks>;
+  constexpr int kEl = F16 ? 2 : 4;
+  auto fetch = [&](int step) {
+    if (step < kSteps) {
+      const unsigned char* src = static_cast<const unsigned char*>(step >= kSteps / 2 ? p.v : p.k);
+      unsigned char* buf = bufs[warp][step % kBufs];
+      pieces(In(), step, [&](int at, long long row, int byte) {
+        cp_async_cg16(smem_u32(buf + at), src + (row * p.token_stride + (long long)kvh * HD) * kEl + byte);
+      });
+    }
+    cp_async_commit();
+  };
+  // returned rows leave through the step's buffer too, unless they are larger than what came in
+  const bool buffered = p.k_rows && (p.rows_f16 || !F16);
+#pragma unroll
+  for (int i = 0; i < kBufs; ++i) fetch(i);
 #pragma unroll 1
   for (int step = 0; step < kSteps; ++step) {
     const bool value = step >= kSteps / 2;
     const int slot = (step % (kSteps / 2)) * kTokens + lane / NB;  // token of the tile
     const bool in = slot >= lo && slot < hi;
     const int tok = tile * kKv4Tile + slot - p.first;  // index among the new tokens
+    if (__all_sync(0xffffffffu, !in)) {
+      fetch(step + kBufs);
+      continue;
+    }
+    unsigned char* buf = bufs[warp][step % kBufs];
+    cp_async_wait<kBufs - 1>();
+    __syncwarp();
     float x[32];
-    if (in) widen32<F16>(raw, x);
-    fetch(step + 1);
-    if (__all_sync(0xffffffffu, !in)) continue;
     if (in) {
+      uint4 raw[kChunks];
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) raw[i] = *reinterpret_cast<const uint4*>(buf + row_piece<kChunks>(lane * kChunks + i));
+      widen32<F16>(raw, x);
       if (p.k_bias) {
         const float* br = (value ? p.v_bias : p.k_bias) + brow;
 #pragma unroll
@@ -404,31 +456,48 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_append_kernel(const Kv4Row
         }
       }
     }
-    if (!in) continue;
-    const __half d = q4_quantise32(x);
-    const int j = slot >> 3, g = slot & 7;
-    if (!value) {
+    __syncwarp();  // every lane has read its block
+    if (in) {
+      const __half d = q4_quantise32(x);
+      const int j = slot >> 3, g = slot & 7;
+      if (!value) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        *reinterpret_cast<uint32_t*>(sm + kv4_word_at(HD, j, 4 * g + t, b)) =
-            q4_bits(x, 8 * t, 16, 4, 20) + (q4_bits(x, 8 * t + 4, 16, 4, 20) << 8);
+        for (int t = 0; t < 4; ++t) {
+          *reinterpret_cast<uint32_t*>(sm + kv4_word_at(HD, j, 4 * g + t, b)) = q4_word(x, 8 * t);
+        }
+        *reinterpret_cast<__half*>(sm + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1)) = d;
+      } else {
+#pragma unroll
+        for (int gg = 0; gg < 8; ++gg) {
+          *reinterpret_cast<uint16_t*>(sm + CB + kv4_word_at(HD, j, 4 * gg + (g >> 1), b) + 2 * (g & 1)) =
+              (uint16_t)q4_half(x[4 * gg], x[4 * gg + 1], x[4 * gg + 2], x[4 * gg + 3]);
+        }
+        *reinterpret_cast<__half*>(sm + 2 * CB + SB + kv4_scale_at(HD, j, g >> 1, b, g & 1)) = d;
       }
-      *reinterpret_cast<__half*>(sm + 2 * CB + kv4_scale_at(HD, j, g >> 1, b, g & 1)) = d;
-    } else {
+      if (p.k_rows) {
+        const float df = __half2float(d);
 #pragma unroll
-      for (int gg = 0; gg < 8; ++gg) {
-        *reinterpret_cast<uint16_t*>(sm + CB + kv4_word_at(HD, j, 4 * gg + (g >> 1), b) + 2 * (g & 1)) =
-            (uint16_t)q4_bits(x, 4 * gg, 4, 8, 12);
+        for (int i = 0; i < 32; ++i) x[i] *= df;
+        if (buffered) {
+          if (F16 || p.rows_f16) put32<true>(buf, lane, x); else put32<false>(buf, lane, x);
+        } else {
+          store32(value ? p.v_rows : p.k_rows, (((size_t)ll * p.n_tokens + tok) * p.pool.kv_heads + kvh) * HD + 32 * b, x);
+        }
       }
-      *reinterpret_cast<__half*>(sm + 2 * CB + SB + kv4_scale_at(HD, j, g >> 1, b, g & 1)) = d;
     }
-    if (p.k_rows) {
-      const float df = __half2float(d);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] *= df;
-      store32(value ? p.v_rows : p.k_rows, (((size_t)ll * p.n_tokens + tok) * p.pool.kv_heads + kvh) * HD + 32 * b,
-              p.rows_f16, x);
+    if (buffered) {
+      __syncwarp();
+      auto leave = [&](auto chunks) {
+        unsigned char* out = static_cast<unsigned char*>(value ? p.v_rows : p.k_rows);
+        pieces(chunks, step, [&](int at, long long row, int byte) {
+          *reinterpret_cast<uint4*>(out + (row * p.pool.kv_heads + kvh) * (HD / 2) * chunks() + byte) =
+              *reinterpret_cast<const uint4*>(buf + at);
+        });
+      };
+      if (F16 || p.rows_f16) leave(std::integral_constant<int, 4>()); else leave(In());
     }
+    __syncwarp();
+    fetch(step + kBufs);
   }
   __syncwarp();
   for (int i = lane * 16; i < TB; i += 512) {
