@@ -749,6 +749,7 @@ struct Seg {
   int gb;              // stream split: the group's first unit (global index)
   int last;            // 1: holds the group's last unit (and so the appended token)
   int group_id;
+  int blk;             // (layer, kv head, head block)
 };
 
 static_assert(sizeof(Seg) <= 64, "segments in shared memory");
@@ -804,7 +805,36 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
   s.ll = (int)(lk / (uint32_t)p.pool.kv_heads);
   s.kvh = (int)lk - s.ll * p.pool.kv_heads;
   s.group_id = (int)blk * p.n_seqs + lo;
+  s.blk = (int)blk;
   return s;
+}
+
+// Stream split: the segment after s, whose group begins inside this CTA's range, without kv4_seg_at's search.
+template <int HD>
+__device__ __forceinline__ void kv4_seg_after(const Kv4DecodeParams& p, const Seg& s, int u1, Seg& r) {
+  r = s;
+  r.gb = s.next;
+  r.first = 0;
+  if (++r.si == p.n_seqs) {
+    r.si = 0;
+    ++r.blk;
+    if (++r.hb == p.head_blocks) {
+      r.hb = 0;
+      if (++r.kvh == p.pool.kv_heads) {
+        r.kvh = 0;
+        ++r.ll;
+      }
+    }
+  }
+  r.group_id = r.blk * p.n_seqs + r.si;
+  const int len = p.seqs[r.si].len, n = kv4_units(len, HD), end = r.gb + n + kKv4GroupUnits;
+  r.next = min(end, u1);
+  const int b = max(r.next - r.gb - kKv4GroupUnits, 0);
+  r.s0 = 0;
+  r.s1 = min(b * kv4_warps(HD), (len + kKv4StageTokens - 1) / kKv4StageTokens);
+  r.last = b == n;
+  r.c0 = blockIdx.x;
+  r.parts = end <= u1 ? 1 : kv4_cta_of(end - 1, p.total_units, p.grid) - r.c0 + 1;
 }
 
 __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
@@ -1194,6 +1224,7 @@ struct Feed {
   const int32_t* row;
   int u, page_base;           // next segment's first unit; as Kv4Seq
   long long page_bytes;       // from one page of this kv head to the next
+  int blk, si;                // the segment's (layer, kv head, head block) and sequence
 };
 static_assert(sizeof(Feed) <= 56, "feeds in shared memory");
 
@@ -1201,6 +1232,8 @@ template <int HD>
 __device__ __forceinline__ void feed_enter(const Kv4DecodeParams& p, Feed& f, const Seg& s, int warp) {
   using D = Dec<HD>;
   f.u = s.next;
+  f.blk = s.blk;
+  f.si = s.si;
   f.stage = s.s0 + warp;
   f.s1 = s.s1;
   const long long rec = (long long)(p.layer_begin + s.ll) * p.pool.num_pages * p.pool.kv_heads + s.kvh;
@@ -1214,11 +1247,30 @@ __device__ __forceinline__ void feed_enter(const Kv4DecodeParams& p, Feed& f, co
 
 // Moves f to a segment in which it has a stage left; false past the end of the CTA's range.
 template <int HD>
-__device__ __forceinline__ bool feed_seek(const Kv4DecodeParams& p, Feed& f, int warp, int u0, int u1) {
-  while (f.stage >= f.s1) {
-    if (f.u >= u1) return false;
-    feed_enter<HD>(p, f, kv4_seg_at<HD>(p, f.u, u0, u1), warp);
-  }
+__device__ __forceinline__ bool feed_seek(const Kv4DecodeParams& p, Feed& f, int warp, int u1) {
+  using D = Dec<HD>;
+  if (f.stage < f.s1) return true;
+  int blk = f.blk, si = f.si, u = f.u, s1 = 0;
+  do {
+    if (u >= u1) {
+      f.u = u;
+      return false;
+    }
+    if (++si == p.n_seqs) si = 0, ++blk;
+    const int len = p.seqs[si].len, end = min(u + kv4_units(len, HD) + kKv4GroupUnits, u1);
+    s1 = min(max(end - u - kKv4GroupUnits, 0) * D::kWarps, (len + D::kStageTokens - 1) / D::kStageTokens);
+    u = end;
+  } while (warp >= s1);
+  Seg s;
+  s.next = u;
+  s.blk = blk;
+  s.si = si;
+  s.s0 = 0;
+  s.s1 = s1;
+  const uint32_t lk = (uint32_t)blk / (uint32_t)p.head_blocks;
+  s.ll = (int)(lk / (uint32_t)p.pool.kv_heads);
+  s.kvh = (int)lk - s.ll * p.pool.kv_heads;
+  feed_enter<HD>(p, f, s, warp);
   return true;
 }
 
@@ -1279,7 +1331,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   if (lane == 0) {
     feed_enter<HD>(p, feed, seg(0), warp);
     *sm_issued = 0;
-    feeding = feed_seek<HD>(p, feed, warp, u_begin, u1);
+    feeding = feed_seek<HD>(p, feed, warp, u1);
     // L2 may fetch the first stage while the previous kernel drains (a hint, coherent with that kernel's writes)
     if (feeding && feed.page_base >= 0) {
       bulk_prefetch_l2(feed.base + (feed.page_base + feed.page) * feed.page_bytes + (long long)feed.in * D::kStageBytes,
@@ -1290,7 +1342,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
     if (!feeding) return;
     feed_issue<HD>(p, feed, ring + slot * D::kStageBytes, &bars[slot]);
     ++*sm_issued;
-    feeding = feed_seek<HD>(p, feed, warp, u_begin, u1);
+    feeding = feed_seek<HD>(p, feed, warp, u1);
   };
   griddep_launch_dependents();
   griddep_wait();
@@ -1347,6 +1399,7 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
     __syncthreads();  // the queries are in shared memory
     w.f = sm_f[g];
     reset_state<HD>(w);
+    if (s.next < u1 && threadIdx.x == 32 * (W - 1)) kv4_seg_after<HD>(p, s, u1, seg(at_seg ^ 1));
     if (appender) {
       // the new token: quantised into the cache (by the first head block) and into a stage of its own here, by the
       // warp that has the fewest stages, while the others attend theirs
@@ -1444,9 +1497,8 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
           *sl = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
     }
-    const bool more = s.next < u1;
-    if (more && threadIdx.x == 0) seg(at_seg ^ 1) = kv4_seg_at<HD>(p, s.next, u_begin, u1);
     __syncthreads();
+    const bool more = s.next < u1;
     if (more) {  // the next segment's query rows on their way
 #pragma unroll
       for (int i = 0; i < kRows; ++i) fetch_query<HD>(p, seg(at_seg ^ 1), warp + i * W, lane, qr[i]);
