@@ -605,6 +605,34 @@ def test_decode_more_groups_than_resident_ctas(engine, hd, group, append):
     cache.close()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("layers,kvh,lens", [
+    (9, 8, [60, 0, 1, 33, 17]),            # 360 groups of one unit: every cut falls on or just inside a group
+    (5, 8, [300, 2, 0, 40, 700, 9, 64, 1, 255]),
+    (1, 1, [12000] + [3] * 63),            # one long sequence before many short ones
+    (1, 2, [3] * 40 + [20000] + [0] * 20)])
+def test_decode_short_sequences_between_cuts(engine, hd, layers, kvh, lens):
+    """Groups that are not worth splitting: a CTA's range begins with a group or has tokens of the one before."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(hd + layers)
+    S, group = len(lens), 2
+    cache = engine.kv4_cache(layers=layers, max_seqs=S, max_tokens_per_seq=max(lens), kv_heads=kvh, head_dim=hd,
+                             page_tokens=64, total_pages=sum(-(-m // 64) for m in lens))
+    kv = [fill(cache, s, rows(rng, layers, m, kvh, hd), rows(rng, layers, m, kvh, hd)) if m else None
+          for s, m in enumerate(lens)]
+    q = rows(rng, layers, S, kvh * group, hd)
+    first = run_decode(cache, list(range(S)), q, kvh * group, flags=TE_ATTN_NO_ROPE)
+    out = run_decode(cache, list(range(S)), q, kvh * group, flags=TE_ATTN_NO_ROPE)
+    assert np.array_equal(first, out)
+    for layer in range(layers):
+        for i, m in enumerate(lens):
+            if m == 0:
+                assert (out[layer, i] == 0).all()
+            else:
+                check(out[layer, i], q[layer, i], kv[i][0][layer], kv[i][1][layer])
+    cache.close()
+
+
 @pytest.mark.parametrize("cut", [0, 37, 64, 299])
 def test_partial_records_merge_to_the_whole(port, engine, cut):
     """A sequence split over two caches (the second a shard at a position offset): partial records, merged."""

@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // taken out the same loop streams 5.9 TB/s.  Measured at head_dim 128, 7 or 8
 // heads a group:
 //   28 layers x 4 kv heads x 32768 tokens  529 MB  136 us, 3.9 TB/s (copy rate: 81 us)
-//   64 sequences, 8192 tokens at most      153 MB   54 us, 2.9 TB/s (23 us)
+//   64 sequences, 8192 tokens at most      153 MB   52 us, 2.9 TB/s (23 us)
 //   36 layers x 2 kv heads x 4097 tokens    43 MB   19 us, 2.3 TB/s (6.6 us)
 //   24 layers x 2 kv heads x 1000 tokens of 64, appending  12 us (0.6 us: latency)
 // Shapes: at head_dim 128, four warps x 2 CTAs with 64 tokens a step and 255
@@ -754,7 +754,28 @@ struct Seg {
 
 static_assert(sizeof(Seg) <= 64, "segments in shared memory");
 
-// Stream split: the CTA whose range [b T / G, (b + 1) T / G) holds unit u.
+// The sequence (of block-relative position rem) by its first unit or part.
+__device__ __forceinline__ int kv4_seq_at(const Kv4DecodeParams& p, int rem, bool aligned) {
+  int lo = 0, hi = p.n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    const int begin = aligned ? p.seqs[mid].part_begin : p.seqs[mid].unit_begin;
+    if (begin <= rem) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Stream split: where CTA b's range begins: at b T / grid, or at the start of that unit's group when the cut would
+// leave the CTA before nothing but the group's fixed units (a part without a token).  The range may be empty.
+__device__ __forceinline__ int kv4_cut(const Kv4DecodeParams& p, int b) {
+  const int u = (int)stage_start(b, p.total_units, p.grid);
+  if (u >= p.total_units) return u;
+  const int blk = (int)((uint32_t)u / (uint32_t)p.block_units);
+  const int gb = blk * p.block_units + p.seqs[kv4_seq_at(p, u - blk * p.block_units, false)].unit_begin;
+  return u - gb <= kKv4GroupUnits ? gb : u;
+}
+
+// Stream split: the CTA whose range holds unit u, which is not one of its group's fixed units but the last.
 __device__ __forceinline__ int kv4_cta_of(int u, long long total, int grid) {
   return (int)div_nonneg((long long)(u + 1) * grid - 1, total);
 }
@@ -768,12 +789,7 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
   const int at = aligned ? (int)blockIdx.x : u;
   const uint32_t blk = (uint32_t)at / (uint32_t)per;
   const int rem = at - (int)blk * per;
-  int lo = 0, hi = p.n_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    const int begin = aligned ? p.seqs[mid].part_begin : p.seqs[mid].unit_begin;
-    if (begin <= rem) lo = mid; else hi = mid - 1;
-  }
+  const int lo = kv4_seq_at(p, rem, aligned);
   s.si = lo;
   const int len = p.seqs[lo].len;
   const int n = kv4_units(len, HD);
@@ -792,7 +808,7 @@ __device__ __forceinline__ Seg kv4_seg_at(const Kv4DecodeParams& p, int u, int u
     s.next = min(s.gb + n + kKv4GroupUnits, u1);
     a = max(u - s.gb - kKv4GroupUnits, 0);
     b = max(s.next - s.gb - kKv4GroupUnits, 0);
-    s.c0 = kv4_cta_of(s.gb, p.total_units, p.grid);
+    s.c0 = kv4_cta_of(s.gb + kKv4GroupUnits, p.total_units, p.grid);
     s.parts = kv4_cta_of(s.gb + n + kKv4GroupUnits - 1, p.total_units, p.grid) - s.c0 + 1;
     s.first = u == u_begin;
   }
@@ -1321,13 +1337,18 @@ __global__ void __launch_bounds__(32 * Dec<HD>::kWarps, Dec<HD>::kCtas)
   }
   __syncwarp();
   const bool aligned = p.block_parts != 0;
-  const int u_begin = aligned ? 0 : (int)stage_start(blockIdx.x, p.total_units, p.grid);
-  const int u1 = aligned ? 1 : (int)stage_start(blockIdx.x + 1, p.total_units, p.grid);
-  if (threadIdx.x == 0) seg(0) = kv4_seg_at<HD>(p, u_begin, u_begin, u1);
+  if (threadIdx.x == 0) {
+    const int u0 = aligned ? 0 : kv4_cut(p, blockIdx.x), u1 = aligned ? 1 : kv4_cut(p, blockIdx.x + 1);
+    sm_flag[2] = u1;
+    sm_flag[3] = u0 < u1;
+    if (u0 < u1) seg(0) = kv4_seg_at<HD>(p, u0, u0, u1);
+  }
   Feed& feed = *reinterpret_cast<Feed*>(smem + D::feed_off + 64 * warp);
   int* sm_issued = reinterpret_cast<int*>(smem + D::feed_off + 64 * warp + 56);
   bool feeding = false;
   __syncthreads();
+  const int u1 = sm_flag[2];
+  if (sm_flag[3] == 0) return;  // an empty range
   if (lane == 0) {
     feed_enter<HD>(p, feed, seg(0), warp);
     *sm_issued = 0;
@@ -1676,9 +1697,9 @@ void plan_kv4_decode(Kv4DecodeParams& p, int head_dim, long long slots) {
   // Aligned split: every group in equal parts of at most `most` units, one part a CTA, all of them resident at once;
   // otherwise the stream split, whose CTAs take equal ranges across groups.  A CTA with one segment saves the merges
   // between segments, an uneven share costs its full length: aligned is taken while its longest part is within an
-  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens 19.1 against
-  // 22.2 us, x 8000 27.8 against 31.1, a ragged batch of 8 11.9 against 15.9; where the rule says stream, 28 layers x
-  // 4 kv heads x 6000 38.0 against 35.3, x 32768 172 against 136, 64 ragged sequences 75 against 54.
+  // eighth of an equal share.  Measured, aligned against stream: 36 layers x 2 kv heads x 4097 tokens 19.0 against
+  // 21.3 us, x 8000 27.7 against 31.2, a ragged batch of 8 12.0 against 15.0; where the rule says stream, 28 layers x
+  // 4 kv heads x 6000 38.0 against 34.4, x 32768 172 against 136, 64 ragged sequences 75 against 52.
   auto parts_for = [&](int most) {
     long long c = 0;
     for (int i = 0; i < p.n_seqs; ++i) c += (kv4_units(p.seqs[i].len, head_dim) + most - 1) / most;

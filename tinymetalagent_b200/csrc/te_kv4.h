@@ -39,7 +39,8 @@ constexpr int kKv4StageTiles = 4, kKv4StageTokens = kKv4StageTiles * kKv4Tile;
 // Warps of a decode CTA, each with its own copies; two CTAs fit an SM.
 __host__ __device__ constexpr int kv4_warps(int hd) { return hd == 128 ? 4 : 8; }
 // What a group's queries and merge cost, in units: the stream split counts them before the group's own (a ragged
-// batch of 64: 54.9 us with one, 53.6 with two, 55.3 with three; 28 layers x 6000 tokens 36.5, 35.3, 38.1).
+// batch of 64: 52.5 us with one, 52.0 with two, 53.7 with three; 28 layers x 6000 tokens 35.6, 34.4, 38.3; the
+// geometric mean of 28 ragged batches 20.6 us with none, 20.5, 20.4, 20.6).
 constexpr int kKv4GroupUnits = 2;
 // Work unit of the decode split: one copy for each warp.
 __host__ __device__ constexpr int kv4_unit(int hd) { return kKv4StageTokens * kv4_warps(hd); }
