@@ -622,6 +622,8 @@ class KV4Cache:
             raise ValueError(f"{name}: expected n_layers * n_tokens rows of contiguous values")
         if x.get_device() != self._device or x.dtype is not self._dtypes[dtype]:
             raise ValueError(f"{name}: expected {dtype} on the engine's device")
+        if stride is not None and stride < row:  # 0 (an expanded row) would read as contiguous rows
+            raise ValueError(f"{name}: tokens share memory")
         return x.data_ptr(), row if stride is None else stride
 
     def append(self, layer_begin: int, n_layers: int, seq: int, k, v, n_tokens: int, k_stored=None, v_stored=None,
