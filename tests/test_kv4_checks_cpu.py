@@ -25,3 +25,42 @@ def test_rows_that_share_memory_are_refused():
             c._new_rows(x, "k", 3 if x.dim() == 3 and x.shape[0] == 3 else 1, 5, "float32")
     # one token, expanded or not, has no stride
     assert c._new_rows(row.expand(1, 128), "k", 1, 1, "float32") == (row.data_ptr(), 128)
+
+
+class FakeLibrary:
+    """Records the call that would reach the library."""
+
+    def __init__(self):
+        self.calls = []
+
+    def te_kv4_append(self, *args):
+        self.calls.append(args)
+        return R.TE_STATUS_OK
+
+
+def fake_cache():
+    c = bare_cache()
+    c.handle, c.lib = 1, FakeLibrary()
+    c._c = lambda status: None
+    return c, c.lib.calls
+
+
+def test_append_takes_a_stride_only_with_addresses():
+    """A token stride beside tensors has to be the tensors' own: another one walks past their ends or takes the wrong
+    rows."""
+    import torch
+    c, calls = fake_cache()
+    k, v = torch.zeros((5, 128)), torch.zeros((5, 128))
+    wide = torch.zeros((5, 512))
+    for kk, vv, stride in ((k, v, 1024), (k, v, 512), (wide[:, :128], wide[:, 128:256], 1024),
+                           (wide[:, :128], wide[:, 128:256], 128), (wide.data_ptr(), v, 512), (k, wide.data_ptr(), 512)):
+        with pytest.raises(ValueError):
+            c.append(0, 1, 0, kk, vv, 5, token_stride=stride)
+    assert calls == []
+    c.append(0, 1, 0, k, v, 5, token_stride=128)
+    c.append(0, 1, 0, wide[:, :128], wide[:, 128:256], 5, token_stride=512)
+    c.append(0, 1, 0, wide.data_ptr(), wide[:, 128:256], 5, token_stride=512)
+    c.append(0, 1, 0, wide.data_ptr(), wide.data_ptr() + 512, 5, token_stride=512)
+    c.append(0, 1, 0, wide[:, :128], wide[:, 128:256], 5)
+    c.append(0, 1, 0, wide.data_ptr(), wide.data_ptr() + 512, 5)
+    assert [a[7] for a in calls] == [128, 512, 512, 512, 512, 128]

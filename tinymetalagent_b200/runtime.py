@@ -630,16 +630,17 @@ class KV4Cache:
                flags: int = 0, token_stride: int = 0) -> None:
         """Quantises n_tokens rows per layer into the cache (te_kv4_append): k and v
         [n_layers][n_tokens][kv_heads][head_dim] fp32, or f16 with TE_ATTN_INPUT_F16, contiguous or evenly spaced
-        views (raw addresses: token_stride values apart).  k_stored / v_stored receive the rows as the cache now
-        holds them, fp32, or f16 with TE_ATTN_OUTPUT_F16."""
+        views (raw addresses: token_stride values apart; beside tensors it can only be theirs).  k_stored /
+        v_stored receive the rows as the cache now holds them, fp32, or f16 with TE_ATTN_OUTPUT_F16."""
         dtype = "float16" if flags & TE_ATTN_INPUT_F16 else "float32"
         n = n_layers * n_tokens * self.kv_heads * self.head_dim
         kp, ks = self._new_rows(k, "k", n_layers, n_tokens, dtype)
         vp, vs = self._new_rows(v, "v", n_layers, n_tokens, dtype)
-        if token_stride == 0:
-            if ks != vs and n_layers * n_tokens > 1:
-                raise ValueError("k and v: different token strides")
-            token_stride = ks
+        # a tensor's token stride is its own; an address has the given one, or contiguous rows
+        strides = {token_stride or st if isinstance(x, int) else st for x, st in ((k, ks), (v, vs))}
+        if n_layers * n_tokens > 1 and (len(strides) > 1 or token_stride not in (0, *strides)):
+            raise ValueError("k and v: token strides differ")
+        token_stride = token_stride or ks
         stored = "float16" if flags & TE_ATTN_OUTPUT_F16 else "float32"
         self._c(self.lib.te_kv4_append(self.handle, layer_begin, n_layers, seq, kp, vp, n_tokens, token_stride,
                                        self._tensor(k_stored, "k_stored", n, stored),
