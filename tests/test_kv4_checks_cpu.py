@@ -64,3 +64,17 @@ def test_append_takes_a_stride_only_with_addresses():
     c.append(0, 1, 0, wide[:, :128], wide[:, 128:256], 5)
     c.append(0, 1, 0, wide.data_ptr(), wide.data_ptr() + 512, 5)
     assert [a[7] for a in calls] == [128, 512, 512, 512, 512, 128]
+
+
+def test_append_refuses_what_is_no_tensor():
+    """Host arrays are refused by type, and a missing operand is the library's to refuse, as in the other calls."""
+    import numpy as np
+    import torch
+    c, calls = fake_cache()
+    k = torch.zeros((5, 128))
+    for kk, vv in ((np.zeros((5, 128), np.float32), k), (k, np.zeros((5, 128), np.float32))):
+        with pytest.raises(TypeError):
+            c.append(0, 1, 0, kk, vv, 5)
+    assert calls == []
+    c.append(0, 1, 0, None, k, 5)
+    assert calls[0][4] is None and calls[0][5] == k.data_ptr()

@@ -600,7 +600,7 @@ class KV4Cache:
         """(address, token stride) of new rows: a contiguous tensor, or a view whose tokens are evenly spaced
         (columns of a wider projection output, [.., n_tokens, kv_heads * head_dim] or [.., kv_heads, head_dim])."""
         row = self.kv_heads * self.head_dim
-        if isinstance(x, int) or x.is_contiguous():
+        if not hasattr(x, "get_device") or x.is_contiguous():
             return self._tensor(x, name, n_layers * n_tokens * row, dtype), row
         if x.dim() >= 2 and tuple(x.shape[-2:]) == (self.kv_heads, self.head_dim) and \
                 x.stride(-2) == self.head_dim:
@@ -637,7 +637,7 @@ class KV4Cache:
         kp, ks = self._new_rows(k, "k", n_layers, n_tokens, dtype)
         vp, vs = self._new_rows(v, "v", n_layers, n_tokens, dtype)
         # a tensor's token stride is its own; an address has the given one, or contiguous rows
-        strides = {token_stride or st if isinstance(x, int) else st for x, st in ((k, ks), (v, vs))}
+        strides = {st if hasattr(x, "get_device") else token_stride or st for x, st in ((k, ks), (v, vs))}
         if n_layers * n_tokens > 1 and (len(strides) > 1 or token_stride not in (0, *strides)):
             raise ValueError("k and v: token strides differ")
         token_stride = token_stride or ks
