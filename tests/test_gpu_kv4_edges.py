@@ -1,0 +1,57 @@
+"""The 4-bit cache where a call meets what other calls left: recorded graphs and scratch that grows, pools that run
+out; and the attention's arithmetic at the ends of its inputs' ranges."""
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import dev, fill, ready, rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["kv4", "f16"])
+def test_recorded_decode_survives_larger_scratch(kind):
+    """A recorded decode writes its partial records where the scratch was when it was recorded.  A later, larger call
+    of the same engine takes larger scratch: the recorded one's has to stay its own."""
+    import torch
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE, AttnEngine
+    rng = np.random.default_rng(41)
+    n, kvh, heads, hd = 1500, 2, 16, 128
+    eng = AttnEngine(0, stream=torch.cuda.Stream().cuda_stream)
+    make = eng.kv4_cache if kind == "kv4" else eng.kv_cache
+    cache = make(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=kvh, head_dim=hd)
+    if kind == "kv4":
+        fill(cache, 0, rows(rng, 1, n, kvh, hd), rows(rng, 1, n, kvh, hd))
+    else:
+        k, v = (dev(rows(rng, n, kvh, hd), torch.float16) for _ in range(2))
+        ready(eng)
+        cache.write_f16(0, 0, 0, k, v)
+    q, out = dev(rows(rng, 1, 1, heads, hd)), torch.zeros((1, 1, heads, hd), device="cuda")
+    ready(eng)
+    cache.decode(0, 1, [0], q, out, heads, flags=TE_ATTN_NO_ROPE)
+    eng.synchronize()
+    want = out.cpu().numpy()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(eng.stream)):
+        cache.decode(0, 1, [0], q, out, heads, flags=TE_ATTN_NO_ROPE)
+    # more than 200 CTAs' records: over 1.7 MB, where the first call's scratch is 1 MB
+    big = eng.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=80000, kv_heads=kvh, head_dim=hd)
+    kb = torch.zeros((1, 80000, kvh, hd // 32, 18), dtype=torch.uint8, device="cuda")
+    big_out = torch.full((1, 1, heads, hd), 7.0, device="cuda")
+    ready(eng)
+    big.write_q4_0(0, 1, 0, 0, 80000, kb, kb)
+    big.decode(0, 1, [0], q, big_out, heads, flags=TE_ATTN_NO_ROPE)
+    eng.synchronize()
+    assert (big_out == 0).all()
+    for _ in range(2):
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.ExternalStream(eng.stream)):
+            graph.replay()
+        eng.synchronize()
+        assert np.array_equal(out.cpu().numpy(), want)
+        big.decode(0, 1, [0], q, big_out, heads, flags=TE_ATTN_NO_ROPE)
+    eng.synchronize()
+    del graph
+    big.close()
+    cache.close()
+    eng.close()

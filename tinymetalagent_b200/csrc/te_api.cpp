@@ -257,6 +257,7 @@ TE_API void te_attn_engine_free(te_attn_engine* e) {
     if (e->stream) cudaStreamSynchronize(e->stream);
     cudaFree(e->partials);
     cudaFree(e->counters);
+    for (int i = 0; i < e->n_retired; ++i) cudaFree(e->retired[i]);
     cudaFree(e->d_error);
     cudaFree(e->io);
     cudaFree(e->qh);
@@ -698,7 +699,7 @@ static te_status decode_call(te_kv_cache* c, size_t layer_begin, size_t n_layers
     }
     (void)cudaGetLastError();  // an unregistered (pageable) pointer is not an error here
     const size_t need = (q_elems + 2 * kv_elems + out_elems) * sizeof(float);
-    cudaError_t err = grow(e, &e->io, &e->io_bytes, need, false);
+    cudaError_t err = grow(e, &e->io, &e->io_bytes, need);
     if (err != cudaSuccess) return cuda_fail(e, err, "staging allocation");
     float* base = reinterpret_cast<float*>(e->io);
     float* sq = base;
@@ -810,12 +811,7 @@ static te_status decode_call(te_kv_cache* c, size_t layer_begin, size_t n_layers
     if (!e->decode_chunk) plan_cluster(p, e->sm_count);
     auto launch = [&]() -> te_status {
       const size_t part_bytes = (size_t)p.grid * p.max_segs * G * decode_scratch_rec((int)hd) * sizeof(float);
-      cudaError_t err = grow(e, reinterpret_cast<void**>(&e->partials), &e->partials_bytes, part_bytes, false);
-      if (err == cudaSuccess) {
-        size_t bytes = e->counters_count * sizeof(uint32_t);
-        err = grow(e, reinterpret_cast<void**>(&e->counters), &bytes, n_layers * hkv * nb * sizeof(uint32_t), true);
-        e->counters_count = bytes / sizeof(uint32_t);
-      }
+      cudaError_t err = grow_decode_scratch(e, part_bytes, n_layers * hkv * nb);
       if (err != cudaSuccess) return cuda_fail(e, err, "decode scratch allocation");
       p.partials = e->partials;
       p.counters = e->counters;
@@ -1126,7 +1122,7 @@ TE_API te_status te_attention_prefill(te_kv_cache* c, size_t layer_begin, size_t
   float* dout = out;
   cudaError_t err;
   if (flags & TE_ATTN_HOST_BUFFERS) {
-    err = grow(e, &e->io, &e->io_bytes, q_bytes + 2 * kv_bytes + out_bytes + 256, false);
+    err = grow(e, &e->io, &e->io_bytes, q_bytes + 2 * kv_bytes + out_bytes + 256);
     if (err != cudaSuccess) return cuda_fail(e, err, "staging allocation");
     char* base = reinterpret_cast<char*>(e->io);
     char* sq = base;
@@ -1172,7 +1168,7 @@ TE_API te_status te_attention_prefill(te_kv_cache* c, size_t layer_begin, size_t
   const void* qf16 = dq;
   QPrepParams qp{};
   if (with_q) {
-    err = grow(e, &e->qh, &e->qh_bytes, n_layers * n_tokens * q_rows_per_token * hd * sizeof(__half), false);
+    err = grow(e, &e->qh, &e->qh_bytes, n_layers * n_tokens * q_rows_per_token * hd * sizeof(__half));
     if (err != cudaSuccess) return cuda_fail(e, err, "prefill query scratch allocation");
     qp.q = dq;
     qp.qh = reinterpret_cast<__half*>(e->qh);

@@ -406,12 +406,7 @@ TE_API te_status te_kv4_attention_decode(te_kv4_cache* c, size_t layer_begin, si
       return fail(e, TE_STATUS_UNSUPPORTED, "decode call too large");
     }
     const size_t part_bytes = (size_t)p.grid * 2 * kv4_record_floats((int)hd) * sizeof(float);
-    cudaError_t err = grow(e, reinterpret_cast<void**>(&e->partials), &e->partials_bytes, part_bytes, false);
-    if (err == cudaSuccess) {
-      size_t bytes = e->counters_count * sizeof(uint32_t);
-      err = grow(e, reinterpret_cast<void**>(&e->counters), &bytes, groups * sizeof(uint32_t), true);
-      e->counters_count = bytes / sizeof(uint32_t);
-    }
+    const cudaError_t err = grow_decode_scratch(e, part_bytes, groups);
     if (err != cudaSuccess) return cuda_fail(e, err, "decode scratch allocation");
     p.partials = e->partials;
     p.counters = e->counters;

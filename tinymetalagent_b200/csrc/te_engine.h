@@ -33,6 +33,11 @@ struct te_attn_engine {
   void* qh = nullptr;  // prefill: rotated f16 queries
   size_t qh_bytes = 0;
   uint32_t* tile_counter = nullptr;
+  // decode scratch (partials, counters) that a larger one took the place of: recorded CUDA graphs still hold its
+  // address, so it lives as long as the engine.  Sizes at least double, so all of it is no larger than what replaced it.
+  static constexpr int kMaxRetired = 64;
+  void* retired[kMaxRetired] = {};
+  int n_retired = 0;
   uint64_t launches = 0;
   std::string last_error;
   bool time_kernels = false;  // te_attn_engine_time_kernels
@@ -177,23 +182,46 @@ inline std::string prof_line(const te_attn_engine* e) {
 }
 
 // Grows a device buffer; the stream is drained first so no queued kernel uses the old one.
-inline cudaError_t grow(te_attn_engine* e, void** buf, size_t* cap, size_t need, bool zero) {
+inline cudaError_t grow(te_attn_engine* e, void** buf, size_t* cap, size_t need) {
   if (need <= *cap) return cudaSuccess;
   cudaError_t err = cudaStreamSynchronize(e->stream);
   if (err != cudaSuccess) return err;
   if (*buf) cudaFree(*buf);
   *buf = nullptr;
   *cap = 0;
-  // geometric growth: a call that needs slightly more never reallocates each time
-  size_t sz = std::max(std::max(2 * need, 2 * *cap), (size_t)1 << 20);
+  const size_t sz = std::max(2 * need, (size_t)1 << 20);  // a call that needs slightly more never reallocates each time
   err = cudaMalloc(buf, sz);
-  if (err != cudaSuccess) return err;
-  if (zero) {
-    err = cudaMemsetAsync(*buf, 0, sz, e->stream);  // ordered before the kernels that use it
+  if (err == cudaSuccess) *cap = sz;
+  return err;
+}
+
+// Grows the decode kernels' scratch to `part_bytes` of partial records and `counters` group counters (zero between
+// launches).  The old buffers are retired, not freed: decode calls can be recorded into CUDA graphs.
+inline cudaError_t grow_decode_scratch(te_attn_engine* e, size_t part_bytes, size_t counters) {
+  auto larger = [&](void** buf, size_t* cap, size_t need, bool zero) -> cudaError_t {
+    if (need <= *cap) return cudaSuccess;
+    if (e->n_retired == te_attn_engine::kMaxRetired) return cudaErrorMemoryAllocation;
+    cudaError_t err = cudaStreamSynchronize(e->stream);  // refuses a stream that is being captured, whatever the mode
     if (err != cudaSuccess) return err;
-  }
-  *cap = sz;
-  return cudaSuccess;
+    const size_t sz = std::max(2 * need, (size_t)1 << 20);
+    void* fresh = nullptr;
+    err = cudaMalloc(&fresh, sz);
+    if (err == cudaSuccess && zero) err = cudaMemsetAsync(fresh, 0, sz, e->stream);  // before the kernels that use it
+    if (err != cudaSuccess) {
+      cudaFree(fresh);
+      return err;
+    }
+    if (*buf) e->retired[e->n_retired++] = *buf;
+    *buf = fresh;
+    *cap = sz;
+    return cudaSuccess;
+  };
+  cudaError_t err = larger(reinterpret_cast<void**>(&e->partials), &e->partials_bytes, part_bytes, false);
+  if (err != cudaSuccess) return err;
+  size_t bytes = e->counters_count * sizeof(uint32_t);
+  err = larger(reinterpret_cast<void**>(&e->counters), &bytes, counters * sizeof(uint32_t), true);
+  e->counters_count = bytes / sizeof(uint32_t);
+  return err;
 }
 
 // Maps pages so that sequence `seq` can hold `tokens` tokens.
