@@ -3,7 +3,7 @@ out; and the attention's arithmetic at the ends of its inputs' ranges."""
 import numpy as np
 import pytest
 
-from test_gpu_kv4 import dev, fill, ready, rows
+from test_gpu_kv4 import blocks_of, check, dev, fill, quantise, ready, rows, run_decode, values
 
 pytestmark = pytest.mark.gpu
 
@@ -53,5 +53,29 @@ def test_recorded_decode_survives_larger_scratch(kind):
     eng.synchronize()
     del graph
     big.close()
+    cache.close()
+    eng.close()
+
+
+def test_a_batch_that_runs_out_of_pages_takes_none():
+    """Two sequences at the end of their pages, one page free: the step is refused, and the page is still free."""
+    from tinymetalagent_b200 import TE_ATTN_ADVANCE, TE_ATTN_NO_ROPE, AttnEngine, TinyEngineError
+    rng = np.random.default_rng(43)
+    kvh, heads, hd = 1, 4, 64
+    eng = AttnEngine(0)
+    cache = eng.kv4_cache(layers=1, max_seqs=3, max_tokens_per_seq=256, kv_heads=kvh, head_dim=hd, page_tokens=64,
+                          total_pages=3)
+    kv = [fill(cache, s, rows(rng, 1, 64, kvh, hd), rows(rng, 1, 64, kvh, hd)) for s in range(2)]
+    q, kn, vn = rows(rng, 1, 2, heads, hd), rows(rng, 1, 2, kvh, hd), rows(rng, 1, 2, kvh, hd)
+    with pytest.raises(TinyEngineError) as e:
+        run_decode(cache, [0, 1], q, heads, k_new=kn, v_new=vn, flags=TE_ATTN_ADVANCE | TE_ATTN_NO_ROPE)
+    assert e.value.status == 4
+    assert cache.length(0) == cache.length(1) == 64
+    cache.reserve(2, 64)  # the free page
+    cache.reset(2)
+    out = run_decode(cache, [1], q[:, 1:], heads, k_new=kn[:, 1:], v_new=vn[:, 1:],
+                     flags=TE_ATTN_ADVANCE | TE_ATTN_NO_ROPE)
+    k, v = (np.concatenate([old[0], values(quantise(new[0, 1:]))]) for old, new in zip(kv[1], (kn, vn)))
+    check(out[0, 0], q[0, 1], k, v)
     cache.close()
     eng.close()

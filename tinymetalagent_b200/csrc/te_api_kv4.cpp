@@ -351,6 +351,13 @@ TE_API te_status te_kv4_attention_decode(te_kv4_cache* c, size_t layer_begin, si
   }
   DeviceGuard dg(e->device);
   if (append) {
+    // all of the step's pages or none: a refused step leaves the pool as it was
+    size_t missing = 0;
+    for (size_t i = 0; i < n_seqs; ++i) {
+      const size_t s = seq_ids[i];
+      missing += b.h_page_table[s * b.pages_per_seq + (size_t)b.len[s] / b.d.page_tokens] < 0 ? 1 : 0;
+    }
+    if (missing > b.free_pages.size()) return fail(e, TE_STATUS_OUT_OF_MEMORY, "KV page pool exhausted");
     for (size_t i = 0; i < n_seqs; ++i) {
       te_status st = ensure_pages(&b, seq_ids[i], (size_t)b.len[seq_ids[i]] + 1);
       if (st != TE_STATUS_OK) return st;
