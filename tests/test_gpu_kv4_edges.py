@@ -79,3 +79,28 @@ def test_a_batch_that_runs_out_of_pages_takes_none():
     check(out[0, 0], q[0, 1], k, v)
     cache.close()
     eng.close()
+
+
+def one_token_wins(engine, hd, size, rest=0.0):
+    """70 tokens whose keys stand for `rest` but for one, whose keys are at the smallest scale there is, under queries
+    of about `size`: that token has all of the weight.  Its values come back, off by what two binary16 parts of a
+    weight leave (2^-22 of it) and the division (2^-23)."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(47)
+    n, heads, at = 70, 3, 13
+    k, v = np.full((1, n, 1, hd), rest, np.float32), rows(rng, 1, n, 1, hd)
+    k[0, at] = 2.0**-21
+    q = (size * (0.5 + 0.5 * rng.random((1, 1, heads, hd)))).astype(np.float32)
+    cache = engine.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=1, head_dim=hd)
+    kk, vv = fill(cache, 0, k, v)
+    assert (kk[0, at] == 2.0**-21).all() and (kk[0, at + 1:] == rest).all()
+    out = run_decode(cache, [0], q, heads, flags=TE_ATTN_NO_ROPE)[0, 0].astype(np.float64)
+    assert (np.abs(out - vv[0, at, 0]) <= 2.0**-21 * np.abs(vv[0, at, 0])).all(), np.abs(out - vv[0, at, 0]).max()
+    cache.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [2.0**40, 2.0**50, 2.0**70, 2.0**100])
+def test_decode_large_scores(engine, hd, size):
+    """Scores so large (2^23 and more) that their own rounding is larger than the exponents of the weights."""
+    one_token_wins(engine, hd, size)

@@ -1031,7 +1031,7 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
   using D = Dec<HD>;
   constexpr int NB = D::NB;
   const int t = lane & 3;
-  // s[i][2j + r]: tile i, token 8j + 2t + r, head g
+  // s[i][2j + r]: tile i, token 8j + 2t + r, head g, in exp2 units
   float s[T][4];
   {
     uint32_t kw[T][2][NB], ks[T][2][NB];
@@ -1075,10 +1075,12 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
           s2[i][j] = f2_fma(d2, lo, b == 0 ? f2_mul(d2, hi) : f2_fma(d2, hi, s2[i][j]));
         }
     }
+    // exp2 units, rounded: the reference and the weights have to see the same score, however large it is
+    const uint64_t f2 = f2_pack(w.f, w.f);
 #pragma unroll
     for (int i = 0; i < T; ++i) {
-      f2_unpack(s2[i][0], s[i][0], s[i][1]);
-      f2_unpack(s2[i][1], s[i][2], s[i][3]);
+      f2_unpack(f2_mul(s2[i][0], f2), s[i][0], s[i][1]);
+      f2_unpack(f2_mul(s2[i][1], f2), s[i][2], s[i][3]);
     }
   }
   uint32_t vs[T][2][NB];
@@ -1107,7 +1109,6 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
 #pragma unroll
     for (int b = 1; b < NB; ++b) vm = h2_maxabs(vm, h2_maxabs(vs[i][0][b], vs[i][1][b]));
   }
-  top *= w.f;
   const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
   const float vtop = fmaxf(vmf.x, vmf.y);
   auto rescale = [&](float x) {  // O times head g's x
@@ -1160,7 +1161,7 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
 #pragma unroll
           for (int b = 0; b < NB; ++b) dm = h2_maxabs(dm, vs[i][j][b]);
           const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&dm));
-          most = fmaxf(most, fmaxf(ex2(fmaf(s[i][2 * j], w.f, w.mb)) * d.x, ex2(fmaf(s[i][2 * j + 1], w.f, w.mb)) * d.y));
+          most = fmaxf(most, fmaxf(ex2(s[i][2 * j] + w.mb) * d.x, ex2(s[i][2 * j + 1] + w.mb) * d.y));
         }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -1176,7 +1177,10 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
     lds_words<HD>(addr + i * D::TB + D::CB, lane, vw[i]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float p0 = ex2(fmaf(s[i][2 * j], w.f, w.mb)), p1 = ex2(fmaf(s[i][2 * j + 1], w.f, w.mb));
+      float p0, p1;
+      f2_unpack(f2_add(f2_pack(s[i][2 * j], s[i][2 * j + 1]), f2_pack(w.mb, w.mb)), p0, p1);
+      p0 = ex2(p0);
+      p1 = ex2(p1);
       w.l += p0 + p1;
       const __half2 h = __floats2half2_rn(p0, p1);
       const float2 hf = __half22float2(h);
