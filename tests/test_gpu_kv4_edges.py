@@ -104,3 +104,9 @@ def one_token_wins(engine, hd, size, rest=0.0):
 def test_decode_large_scores(engine, hd, size):
     """Scores so large (2^23 and more) that their own rounding is larger than the exponents of the weights."""
     one_token_wins(engine, hd, size)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [2.0**117, 2.0**127])
+def test_decode_queries_up_to_the_end_of_fp32(engine, hd, size):
+    one_token_wins(engine, hd, size)

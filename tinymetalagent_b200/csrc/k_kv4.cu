@@ -962,7 +962,7 @@ __device__ __forceinline__ void stage_query(const Kv4DecodeParams& p, const Seg&
   float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
   for (int off = 1; off < HD / 4; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const int k = top > 0.f ? min(max(11 - exponent_of(top), -100), 126) : 0;
+  const int k = top > 0.f ? min(max(11 - exponent_of(top), -116), 126) : 0;
   const float sc = pow2i(k);
   if (lane == 0) f[h] = p.scale_log2 * pow2i(-k);
   uint32_t w[4];
