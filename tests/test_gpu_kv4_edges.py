@@ -110,3 +110,23 @@ def test_decode_large_scores(engine, hd, size):
 @pytest.mark.parametrize("size", [2.0**117, 2.0**127])
 def test_decode_queries_up_to_the_end_of_fp32(engine, hd, size):
     one_token_wins(engine, hd, size)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [2.0**114, 2.0**127])
+def test_decode_scores_below_fp32(engine, hd, size):
+    """Scores that overflow to minus infinity beside finite ones have no weight, also where a warp sees no others."""
+    one_token_wins(engine, hd, size, rest=-(2.0**17))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_only_scores_below_fp32(engine, hd):
+    """Every score minus infinity: nothing is attended, as over no token."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(53)
+    n, heads = 300, 2
+    cache = engine.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=1, head_dim=hd)
+    fill(cache, 0, np.full((1, n, 1, hd), -(2.0**17), np.float32), rows(rng, 1, n, 1, hd))
+    out = run_decode(cache, [0], np.full((1, 1, heads, hd), 2.0**120, np.float32), heads, flags=TE_ATTN_NO_ROPE)
+    assert (out == 0).all()
+    cache.close()

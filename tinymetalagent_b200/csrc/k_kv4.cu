@@ -923,7 +923,7 @@ struct WarpState {
   float f;                // S f = score in exp2 units
   float o[HD / 32][2][4];    // O^T accumulators: block, m16 tile
   float m;                // head g: reference of the scores, an integer, so that rescaling is exact
-  float mb;               // kWeightExp - m
+  float mb;               // kWeightExp - m; finite while m is not, so that scores of -inf get no weight
   float l;                // sum of this lane's weights, head g
 };
 
@@ -991,7 +991,7 @@ __device__ __forceinline__ void reset_state(WarpState<HD>& w) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) w.o[b][i][r] = 0.f;
   w.m = -INFINITY;
-  w.mb = INFINITY;
+  w.mb = 0.f;
   w.l = 0.f;
 }
 
@@ -1229,7 +1229,7 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
     }
   }
   if (odd) {
-    w.mb = kWeightExp - w.m;
+    w.mb = w.m > -INFINITY ? kWeightExp - w.m : 0.f;
     w.l *= pow2i(-min(shift, 0));
     rescale(pow2i(-shift));
   }
