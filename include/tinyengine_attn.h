@@ -492,15 +492,19 @@ TE_API te_status te_kv4_cache_read_q4_0(te_kv4_cache *cache, size_t layer_begin,
  * with TE_ATTN_INPUT_F16; out fp32.  With k_new / v_new each sequence's new
  * token is quantised into the cache by the same launch and attended as stored.
  * Any number of query heads per kv head.  A sequence that holds no token (and
- * appends none) gives zeros, or a partial record {0, -inf, 0}.  The queries
- * and the softmax weights enter the tensor cores as two binary16 parts each
- * (about 22 bits), the codes exactly; scores, softmax statistics and sums are
- * fp32.  Partial records (TE_ATTN_PARTIAL) have te_attention_decode's layout
- * and meaning, except that m is a reference of the row that lies near its
- * largest score (at most 5 below it, less than 1 above), instead of the score
- * itself: te_attention_merge_partials takes both.  Results are bit-identical
- * across repeated calls.  Flags: TE_ATTN_ADVANCE, TE_ATTN_PARTIAL,
- * TE_ATTN_NO_ROPE, TE_ATTN_QKV_BIAS, TE_ATTN_INPUT_F16. */
+ * appends none) gives zeros, or a partial record {0, -inf, 0}.  The queries,
+ * and the products of softmax weights and block scales, enter the tensor cores
+ * as two binary16 parts each, the codes exactly; scores, softmax statistics and
+ * sums are fp32.  Two parts keep about 22 bits: of the head's largest query
+ * value, and of each product within 2^14 of the head's largest product among
+ * the same 64 tokens (smaller ones keep the same absolute error).  Scores that
+ * overflow fp32 to minus infinity have no weight, to infinity give NaN.
+ * Partial records (TE_ATTN_PARTIAL) have te_attention_decode's layout and
+ * meaning, except that m is a reference of the row that lies near its largest
+ * score (at most 5 below it, less than 1 above), instead of the score itself:
+ * te_attention_merge_partials takes both.  Results are bit-identical across
+ * repeated calls.  Flags: TE_ATTN_ADVANCE, TE_ATTN_PARTIAL, TE_ATTN_NO_ROPE,
+ * TE_ATTN_QKV_BIAS, TE_ATTN_INPUT_F16. */
 TE_API te_status te_kv4_attention_decode(te_kv4_cache *cache, size_t layer_begin, size_t n_layers,
                                          const uint32_t *seq_ids, size_t n_seqs, const int64_t *q_positions,
                                          const void *q, const void *k_new, const void *v_new, size_t heads,

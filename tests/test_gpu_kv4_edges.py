@@ -81,14 +81,14 @@ def test_a_batch_that_runs_out_of_pages_takes_none():
     eng.close()
 
 
-def one_token_wins(engine, hd, size, rest=0.0):
+def one_token_wins(engine, hd, size, rest=0.0, gain=1.0):
     """70 tokens whose keys stand for `rest` but for one, whose keys are at the smallest scale there is, under queries
     of about `size`: that token has all of the weight.  Its values come back, off by what two binary16 parts of a
     weight leave (2^-22 of it) and the division (2^-23)."""
     from tinymetalagent_b200 import TE_ATTN_NO_ROPE
     rng = np.random.default_rng(47)
     n, heads, at = 70, 3, 13
-    k, v = np.full((1, n, 1, hd), rest, np.float32), rows(rng, 1, n, 1, hd)
+    k, v = np.full((1, n, 1, hd), rest, np.float32), rows(rng, 1, n, 1, hd, gain=gain)
     k[0, at] = 2.0**-21
     q = (size * (0.5 + 0.5 * rng.random((1, 1, heads, hd)))).astype(np.float32)
     cache = engine.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=1, head_dim=hd)
@@ -104,6 +104,13 @@ def one_token_wins(engine, hd, size, rest=0.0):
 def test_decode_large_scores(engine, hd, size):
     """Scores so large (2^23 and more) that their own rounding is larger than the exponents of the weights."""
     one_token_wins(engine, hd, size)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("gain", [2.0**-16, 2.0**-12, 2.0**6, 2.0**15])
+@pytest.mark.parametrize("size,rest", [(2.0**50, 0.0), (2.0**100, 0.0), (2.0**114, -(2.0**17))])
+def test_decode_large_scores_beside_small_and_large_values(engine, hd, size, rest, gain):
+    one_token_wins(engine, hd, size, rest, gain)
 
 
 @pytest.mark.parametrize("hd", [64, 128])
@@ -129,4 +136,66 @@ def test_decode_only_scores_below_fp32(engine, hd):
     fill(cache, 0, np.full((1, n, 1, hd), -(2.0**17), np.float32), rows(rng, 1, n, 1, hd))
     out = run_decode(cache, [0], np.full((1, 1, heads, hd), 2.0**120, np.float32), heads, flags=TE_ATTN_NO_ROPE)
     assert (out == 0).all()
+    cache.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,at", [(40, 0), (128, 0), (128, 127), (1000, 500)])
+@pytest.mark.parametrize("sigma", [1.0, 0.1, 0.02, 2.0**-13])
+def test_decode_beside_a_token_without_values(engine, hd, n, at, sigma):
+    """A token whose values are zero takes nearly all of the weight (as first tokens of trained models do), by 0 to 18
+    nats: what is left of the others is as exact as without it.
+
+    The bound counts what they contribute, A = sum(w max|v|) / sum(w), not the largest value.  A score has one term
+    here: it is off by its factor's roundings (3 2^-24 of it), the offset's (2^-21 of a weight) and the exponential's
+    (2^-22), which count in a weight and in the sum; two-part weights and products leave 2^-21 and 2^-23, and each of
+    n / 16 + 8 additions 2^-22."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(59)
+    gaps = np.array([0.0, 4, 8, 10, 12, 14, 18])
+    heads = len(gaps)
+    k, v = np.zeros((1, n, 1, hd), np.float32), rows(rng, 1, n, 1, hd, gain=sigma)
+    k[0, at, 0, 0], v[0, at] = np.sqrt(hd), 0
+    q = np.zeros((1, 1, heads, hd), np.float32)
+    q[0, 0, :, 0] = gaps
+    cache = engine.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=1, head_dim=hd)
+    kk, vv = (a[0, :, 0] for a in fill(cache, 0, k, v))
+    out = run_decode(cache, [0], q, heads, flags=TE_ATTN_NO_ROPE)[0, 0].astype(np.float64)
+    for h in range(heads):
+        s = kk @ q[0, 0, h].astype(np.float64) / np.sqrt(hd)
+        w = np.exp(s)
+        ds = 3 * 2.0**-24 * np.abs(s).max() + 2.0**-21 + 2.0**-22
+        mass = (w @ np.abs(vv).max(1)) / w.sum()
+        tol = mass * (2 * ds + 2.0**-21 + 2.0**-23 + (n / 16 + 8) * 2.0**-22)
+        err = np.abs(out[h] - (w @ vv) / w.sum()).max()
+        assert err <= tol, (gaps[h], err / mass, tol / mass)
+    cache.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 4, 70])
+@pytest.mark.parametrize("small", [2.0**-9, 2.0**-13, 2.0**-17])
+def test_decode_blocks_of_small_values_beside_ordinary_ones(engine, hd, n, small):
+    """Blocks of 32 values far below the row's others (scales of small / 4 or so, down to binary16 subnormals): their
+    outputs are exact against their own values.  All tokens have the same score, so that a weight's error cancels; it
+    is above 2^13, and beside it a product's two parts are off by 2^-24 (on the grid of binary16's subnormals) next to
+    the terms of the bound above."""
+    from tinymetalagent_b200 import TE_ATTN_NO_ROPE
+    rng = np.random.default_rng(61)
+    heads = 7
+    k, v, q = np.zeros((1, n, 1, hd), np.float32), rows(rng, 1, n, 1, hd), np.zeros((1, 1, heads, hd), np.float32)
+    k[..., 0] = 1
+    q[0, 0, :, 0] = np.linspace(0.3, 2.9, heads)
+    v[..., 32:] *= small
+    cache = engine.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=n, kv_heads=1, head_dim=hd)
+    fill(cache, 0, k, v)
+    raw = quantise(v)[0, :, 0]
+    vv, d = values(raw), np.abs(np.ascontiguousarray(raw[..., :2]).view(np.float16)[..., 0].astype(np.float64))
+    out = run_decode(cache, [0], q, heads, flags=TE_ATTN_NO_ROPE)[0, 0].astype(np.float64)
+    for b in range(hd // 32):
+        cols = slice(32 * b, 32 * b + 32)
+        mass = np.abs(vv[:, cols]).max(1).mean()
+        tol = mass * (2.0**-21 + 2.0**-23 + (n / 16 + 8) * 2.0**-22 + 2.0**-24 / (2.0**13 * d[:, b].mean()))
+        err = np.abs(out[:, cols] - vv[:, cols].mean(0)).max()
+        assert err <= tol, (b, err / mass, tol / mass)
     cache.close()

@@ -682,13 +682,19 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 //      scaled by a power of two per head; B = K codes minus 8.
 //      Per block of 32 dims S += d (A B) in fp32.
 //   O^T: A = V codes minus 8, rows = dims; B = P d as f16 hi + lo parts (an
-//      error-free product: hi = f16(P d), lo = f16 of the rest), so the
-//      weights keep about 22 bits.
+//      error-free product: hi = f16(P d), lo = f16 of the rest): about 22 bits
+//      of a product that is not below 2^-14 of the copy's largest.
 //
 // The C fragment of S holds, in lane 4g + t, head g and tokens 2t, 2t + 1:
 // exactly what the B fragment of O^T wants, so the weights never leave their
-// registers.  The online softmax keeps a reference exponent per head and
-// moves it (rescaling O) only when a score exceeds it by more than 2^5.
+// registers.  A copy's weights are counted from its own largest score, a power
+// of two per head, and its products join O by that power against the head's
+// reference, which moves (rescaling O) only when a copy exceeds it by more than
+// 2^5.  Counted from the head's reference instead, weights of 2^-17 (beside a
+// token that takes nearly all of the weight) had their products with scales
+// of 2^-7 on the grid of binary16's subnormals: where that token's values are
+// zero the output was 6e-4 off, against less than 1e-5 now, at the same speed
+// (147 and 50 to 51 us for the first two lines below, both ways in turn).
 //
 // Split: a warp streams copies of 32 (head_dim 64: 64) tokens through a ring
 // of its own, so no barrier stands in the loop; the CTA's warps merge at the
@@ -914,6 +920,10 @@ __device__ __forceinline__ uint32_t h2_maxabs(uint32_t a, uint32_t b) {
   const __half2 m = __hmax2(x, y);
   return *reinterpret_cast<const uint32_t*>(&m);
 }
+__device__ __forceinline__ uint32_t h2_min(uint32_t a, uint32_t b) {
+  const __half2 m = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
 // 2^k as fp32, -126 <= k <= 127.
 __device__ __forceinline__ float pow2i(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
@@ -923,13 +933,15 @@ struct WarpState {
   float f;                // S f = score in exp2 units
   float o[HD / 32][2][4];    // O^T accumulators: block, m16 tile
   float m;                // head g: reference of the scores, an integer, so that rescaling is exact
-  float mb;               // kWeightExp - m; finite while m is not, so that scores of -inf get no weight
   float l;                // sum of this lane's weights, head g
 };
 
-constexpr float kSlack = 5.f;      // scores may exceed the reference by this before it moves
-constexpr float kWeightExp = 9.f;  // weights are 2^(score - m + 9): at most 2^14
-constexpr float kScaleMin = 0x1p-11f, kScaleMax = 2.f;  // V scales for which weight times scale stays within f16
+constexpr float kSlack = 5.f;       // a stage's reference may exceed the head's by this before that one moves
+constexpr float kWeightExp = 14.f;  // weights are 2^(score - the stage's reference + 14): the largest is above 2^13
+// Token scales (the largest of a row's block scales) for which weight times scale stays within f16: the stage's largest
+// product is between 2^-1 and 2^15, and a product's two parts are off by 2^-25 and a part in 2^22 at most.
+constexpr float kScaleMin = 0x1p-14f, kScaleMax = 2.f;
+constexpr float kRefMax = 0x1p22f;  // references up to here leave 14 - reference exact
 
 // A query head's raw row, 4 dims a lane (lanes 0-15 at head_dim 64); zeros for a head the group has not.
 template <int HD>
@@ -991,7 +1003,6 @@ __device__ __forceinline__ void reset_state(WarpState<HD>& w) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) w.o[b][i][r] = 0.f;
   w.m = -INFINITY;
-  w.mb = 0.f;
   w.l = 0.f;
 }
 
@@ -1094,83 +1105,93 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
         if (kKv4Tile * i + 8 * (r >> 1) + 2 * t + (r & 1) >= valid) {
           s[i][r] = -INFINITY;
 #pragma unroll
-          for (int b = 0; b < NB; ++b) vs[i][r >> 1][b] &= (r & 1) ? 0x0000ffffu : 0xffff0000u;
+          for (int b = 0; b < NB; ++b) {  // a scale of 1
+            uint32_t& d = vs[i][r >> 1][b];
+            d = (r & 1) ? (d & 0x0000ffffu) | 0x3c000000u : (d & 0xffff0000u) | 0x3c00u;
+          }
         }
       }
   }
+  // Weights are counted from the stage's own largest score: a token's share of the stage keeps its bits however far
+  // the stage lies below the reference, and O takes the stage in by one power of two a head.
   float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-  uint32_t vm = h2_maxabs(vs[0][0][0], vs[0][1][0]);
 #pragma unroll
-  for (int i = 0; i < T; ++i) {
-    if (i > 0) {
-      top = fmaxf(fmaxf(top, fmaxf(s[i][0], s[i][1])), fmaxf(s[i][2], s[i][3]));
-      vm = h2_maxabs(vm, h2_maxabs(vs[i][0][0], vs[i][1][0]));
+  for (int i = 1; i < T; ++i) top = fmaxf(fmaxf(top, fmaxf(s[i][0], s[i][1])), fmaxf(s[i][2], s[i][3]));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  auto token_scale = [&](int i, int j) {  // the largest block scale of two tokens
+    uint32_t d = vs[i][j][0];
+#pragma unroll
+    for (int b = 1; b < NB; ++b) d = h2_maxabs(d, vs[i][j][b]);
+    return d;
+  };
+  uint32_t dmin = token_scale(0, 0), dmax = dmin;
+#pragma unroll
+  for (int i = 0; i < T; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (i + j == 0) continue;
+      const uint32_t d = token_scale(i, j);
+      dmin = h2_min(dmin, d);
+      dmax = h2_maxabs(dmax, d);
     }
-#pragma unroll
-    for (int b = 1; b < NB; ++b) vm = h2_maxabs(vm, h2_maxabs(vs[i][0][b], vs[i][1][b]));
-  }
-  const float2 vmf = __half22float2(*reinterpret_cast<const __half2*>(&vm));
-  const float vtop = fmaxf(vmf.x, vmf.y);
-  auto rescale = [&](float x) {  // O times head g's x
-    const float x0 = __shfl_sync(0xffffffffu, x, 8 * t);
-    const float x1 = __shfl_sync(0xffffffffu, x, 8 * t + 4);
+  const float2 lo2 = __half22float2(*reinterpret_cast<const __half2*>(&dmin));
+  const float2 hi2 = __half22float2(*reinterpret_cast<const __half2*>(&dmax));
+  const bool some = top > -INFINITY;  // false: every score is -inf or NaN
+  const float ref = some ? ceilf(top) : 0.f;
+  const bool move = some && ref > w.m + kSlack;
+  bool odd = fminf(lo2.x, lo2.y) < kScaleMin || fmaxf(hi2.x, hi2.y) > kScaleMax || fabsf(ref) > kRefMax;
+  auto pair_of = [&](float x) {  // head g's x for the two heads whose columns of O this lane holds
+    return f2_pack(__shfl_sync(0xffffffffu, x, 8 * t), __shfl_sync(0xffffffffu, x, 8 * t + 4));
+  };
+  if (__any_sync(0xffffffffu, move)) {
+    const float alpha = move ? ex2(w.m - ref) : 1.f;
+    if (move) w.m = ref;
+    w.l *= alpha;
+    const uint64_t a2 = pair_of(alpha);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        w.o[b][i][0] *= x0;
-        w.o[b][i][1] *= x1;
-        w.o[b][i][2] *= x0;
-        w.o[b][i][3] *= x1;
-      }
-  };
-  int shift = 0;     // O counts 2^shift times during this stage, and l 2^min(shift, 0) times
-  bool odd = false;  // uniform: shift may be other than 0
-  if (__any_sync(0xffffffffu, top > w.m + kSlack || vtop > kScaleMax || vtop < kScaleMin)) {
-    float tm = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
-    float alpha = 1.f;
-    if (tm > w.m + kSlack) {
-      tm = ceilf(tm);
-      alpha = ex2(w.m - tm);
-      w.m = tm;
-      w.mb = kWeightExp - tm;
-    }
-    // Weight times scale has to stay between f16's ends.  With scales of kScaleMin .. kScaleMax it does; smaller ones
-    // are moved up for the stage, and beside a larger one the weights are moved down, by what its own weight asks.
-    float most = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    if (most < kScaleMin) {
-      odd = true;
-      shift = min(-1 - exponent_of(most), 15);
-      const __half2 h = __float2half2_rn(pow2i(shift));
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int b = 0; b < NB; ++b) vs[i][j][b] = h2_mul(vs[i][j][b], *reinterpret_cast<const uint32_t*>(&h));
-    } else if (most > kScaleMax) {
-      odd = true;
-      most = 0.f;
-#pragma unroll
-      for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t dm = vs[i][j][0];
-#pragma unroll
-          for (int b = 0; b < NB; ++b) dm = h2_maxabs(dm, vs[i][j][b]);
-          const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&dm));
-          most = fmaxf(most, fmaxf(ex2(s[i][2 * j] + w.mb) * d.x, ex2(s[i][2 * j + 1] + w.mb) * d.y));
+        for (int r = 0; r < 4; r += 2) {
+          f2_unpack(f2_mul(f2_pack(w.o[b][i][r], w.o[b][i][r + 1]), a2), w.o[b][i][r], w.o[b][i][r + 1]);
         }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      shift = max(min(14 - exponent_of(most), 0), -32);
-      w.mb += (float)shift;
-    }
-    w.l *= alpha * pow2i(min(shift, 0));
-    rescale(alpha * pow2i(shift));
   }
+  float into_o = some ? ex2(ref - w.m) : 0.f, into_l = into_o;
+  float mb = kWeightExp - ref;
+  odd = __any_sync(0xffffffffu, odd);
+  if (odd) {
+    // A token whose scales lie outside the ordinary range (or scores so large that the offset cannot hold both the
+    // reference and the 14): every token's scales are brought to [1, 2) by a power of two, which its weight takes
+    // instead, and the weights are counted from the largest of these products.  The weights' sum has them without it.
+    float sum = 0.f, vtop = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sum += ex2((s[i][2 * j] - ref) + kWeightExp) + ex2((s[i][2 * j + 1] - ref) + kWeightExp);
+        const uint32_t dm = token_scale(i, j);
+        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&dm));
+        const int e0 = min(max(exponent_of(d.x), -15), 15), e1 = min(max(exponent_of(d.y), -15), 15);
+        const uint32_t k = pack_half2(pow2i(-e0), pow2i(-e1));
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vs[i][j][b] = h2_mul(vs[i][j][b], k);
+        // values of zero add nothing, whatever their weight
+        s[i][2 * j] = d.x == 0.f ? -INFINITY : (s[i][2 * j] - ref) + (float)e0;
+        s[i][2 * j + 1] = d.y == 0.f ? -INFINITY : (s[i][2 * j + 1] - ref) + (float)e1;
+        vtop = fmaxf(vtop, fmaxf(s[i][2 * j], s[i][2 * j + 1]));
+      }
+    vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+    vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
+    w.l += into_l * sum;
+    into_l = 0.f;
+    const float vref = vtop > -INFINITY ? ceilf(vtop) : 0.f;
+    into_o *= ex2(vref);
+    mb = kWeightExp - vref;
+  }
+  const uint64_t into2 = pair_of(into_o);
+  float sum = 0.f;
   uint32_t ph[T][2], pl[T][2], vw[T][2][NB];
 #pragma unroll
   for (int i = 0; i < T; ++i) {
@@ -1178,19 +1199,20 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float p0, p1;
-      f2_unpack(f2_add(f2_pack(s[i][2 * j], s[i][2 * j + 1]), f2_pack(w.mb, w.mb)), p0, p1);
+      f2_unpack(f2_add(f2_pack(s[i][2 * j], s[i][2 * j + 1]), f2_pack(mb, mb)), p0, p1);
       p0 = ex2(p0);
       p1 = ex2(p1);
-      w.l += p0 + p1;
+      sum += p0 + p1;
       const __half2 h = __floats2half2_rn(p0, p1);
       const float2 hf = __half22float2(h);
       ph[i][j] = *reinterpret_cast<const uint32_t*>(&h);
       pl[i][j] = pack_half2(p0 - hf.x, p1 - hf.y);
     }
   }
+  w.l += into_l * sum;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    // the tiles' products start from zero and join O by a rounded fp32 addition: a long accumulation inside
+    // the tiles' products start from zero and join O by a rounded fp32 FMA: a long accumulation inside
     // the tensor core truncates at every step
     float o0[4], o1[4];
     uint32_t hi[T][2], lo[T][2], ca[T][4], cc[T][4];  // as for the keys: all conversions first
@@ -1222,16 +1244,11 @@ __device__ __forceinline__ void attend(uint32_t addr, uint32_t qf, int valid, in
     }
 #pragma unroll
     for (int r = 0; r < 4; r += 2) {
-      f2_unpack(f2_add(f2_pack(w.o[b][0][r], w.o[b][0][r + 1]), f2_pack(o0[r], o0[r + 1])), w.o[b][0][r],
+      f2_unpack(f2_fma(f2_pack(o0[r], o0[r + 1]), into2, f2_pack(w.o[b][0][r], w.o[b][0][r + 1])), w.o[b][0][r],
                 w.o[b][0][r + 1]);
-      f2_unpack(f2_add(f2_pack(w.o[b][1][r], w.o[b][1][r + 1]), f2_pack(o1[r], o1[r + 1])), w.o[b][1][r],
+      f2_unpack(f2_fma(f2_pack(o1[r], o1[r + 1]), into2, f2_pack(w.o[b][1][r], w.o[b][1][r + 1])), w.o[b][1][r],
                 w.o[b][1][r + 1]);
     }
-  }
-  if (odd) {
-    w.mb = w.m > -INFINITY ? kWeightExp - w.m : 0.f;
-    w.l *= pow2i(-min(shift, 0));
-    rescale(pow2i(-shift));
   }
 }
 
