@@ -125,9 +125,9 @@ TE_API te_status te_attn_engine_set_wait_limit(te_attn_engine *engine, uint32_t 
  * but "0"), the reference's switch (c/src/qwen.c:47-73, 2216-2304); then the
  * engine prints its totals to stderr when freed.  The report is one line,
  * "tinyengine_profile: device_ms=T decode=ms/calls append=... merge=...
- * prefill_prep=... prefill_attn=... matvec=... exchange=... step=...
- * kv4_decode=... kv4_append=... kv4_read=...", the reference's
- * "name=ms/calls" format.  te_attn_engine_profile_report synchronises the
+ * prefill_prep=... prefill_attn=... matvec=... exchange=... step=...", and
+ * " kv4_decode=... kv4_append=... kv4_read=..." of those that ran; the
+ * reference's "name=ms/calls" format.  te_attn_engine_profile_report synchronises the
  * engine's stream and writes that line to buf (TE_STATUS_INVALID_ARGUMENT if
  * it does not fit). */
 TE_API te_status te_attn_engine_profile(te_attn_engine *engine, int enable);

@@ -199,3 +199,26 @@ def test_decode_blocks_of_small_values_beside_ordinary_ones(engine, hd, n, small
         err = np.abs(out[:, cols] - vv[:, cols].mean(0)).max()
         assert err <= tol, (b, err / mass, tol / mass)
     cache.close()
+
+
+def test_profile_line_of_an_engine_without_a_4_bit_cache():
+    """The line has the eight kinds that it had before there was a 4-bit cache; its kinds join as they run."""
+    import torch
+    from tinymetalagent_b200 import TE_ATTN_ADVANCE, AttnEngine
+    eng = AttnEngine(0)
+    eng.profile(True)
+
+    def kinds():
+        return [f.split("=")[0] for f in eng.profile_report().split(": ", 1)[1].split()][1:]
+
+    old = ["decode", "append", "merge", "prefill_prep", "prefill_attn", "matvec", "exchange", "step"]
+    assert kinds() == old
+    cache = eng.kv4_cache(layers=1, max_seqs=1, max_tokens_per_seq=64, kv_heads=1, head_dim=64)
+    x = torch.zeros((1, 2, 1, 64), device="cuda")
+    torch.cuda.synchronize()
+    cache.append(0, 1, 0, x, x, 2, flags=TE_ATTN_ADVANCE)
+    assert kinds() == old + ["kv4_append"]
+    cache.read(0, 1, 0, 0, 2, x, x)
+    assert kinds() == old + ["kv4_append", "kv4_read"]
+    cache.close()
+    eng.close()

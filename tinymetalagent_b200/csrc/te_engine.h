@@ -174,6 +174,8 @@ inline std::string prof_line(const te_attn_engine* e) {
   std::snprintf(buf, sizeof(buf), "tinyengine_profile: device_ms=%.3f", total);
   out += buf;
   for (int k = 0; k < PK_COUNT; ++k) {
+    // the 4-bit cache's kinds only where they ran: without it the line is what its readers' buffers were made for
+    if (k >= PK_KV4_DECODE && e->prof_calls[k] == 0) continue;
     std::snprintf(buf, sizeof(buf), " %s=%.3f/%llu", kProfNames[k], e->prof_ms[k],
                   (unsigned long long)e->prof_calls[k]);
     out += buf;
