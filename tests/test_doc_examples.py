@@ -1,4 +1,7 @@
-"""The integration examples of the 4-bit cache say what the code takes: the C example compiles against the header."""
+"""The integration examples of the 4-bit cache and of the decoder say what the code takes: the C example compiles
+against the installed header, the Python calls bind to the signatures."""
+import ast
+import inspect
 import re
 import shutil
 import subprocess
@@ -30,3 +33,16 @@ def test_c_example_of_the_4_bit_cache_compiles(tmp_path):
                             str(src)], capture_output=True, text=True)
         assert r.returncode == 0, r.stderr
 
+
+def test_decoder_calls_bind_to_its_signature():
+    from tinymetalagent_b200.qwen import QwenDecoder
+    sig = inspect.signature(QwenDecoder)
+    seen = 0
+    for p in DOCS:
+        for call in re.findall(r"QwenDecoder\([^()`]*\)", p.read_text()):
+            node = ast.parse(call, mode="eval").body
+            if any(isinstance(a, ast.Constant) and a.value is ... for a in node.args):
+                continue  # "...": the other arguments are as elsewhere
+            sig.bind(*node.args, **{k.arg: k.value for k in node.keywords})
+            seen += 1
+    assert seen > 0
