@@ -222,3 +222,26 @@ def test_profile_line_of_an_engine_without_a_4_bit_cache():
     assert kinds() == old + ["kv4_append", "kv4_read"]
     cache.close()
     eng.close()
+
+
+def test_a_refused_allocation_does_not_fail_later_calls():
+    """A cache larger than the GPU is refused; the launches after it, of either cache, report their own outcome."""
+    import torch
+    from tinymetalagent_b200 import TE_ATTN_ADVANCE, AttnEngine, TinyEngineError
+    rng = np.random.default_rng(67)
+    eng = AttnEngine(0)
+    small = dict(layers=1, max_seqs=1, max_tokens_per_seq=64, kv_heads=1, head_dim=64)
+    caches = eng.kv4_cache(**small), eng.kv_cache(**small)
+    x, kb = dev(rows(rng, 1, 3, 1, 64)), dev(quantise(rows(rng, 1, 3, 1, 64)))
+    for call in (lambda: caches[0].write_q4_0(0, 1, 0, 0, 3, kb, kb),
+                 lambda: caches[1].append_rope(0, 1, 0, x, x, 3, TE_ATTN_ADVANCE),
+                 lambda: caches[0].append(0, 1, 0, x, x, 3, flags=TE_ATTN_ADVANCE)):
+        ready(eng)
+        with pytest.raises(TinyEngineError) as e:  # 600 GB
+            eng.kv4_cache(layers=64, max_seqs=1, max_tokens_per_seq=1 << 20, kv_heads=64, head_dim=128, max_position=64)
+        assert e.value.status == 4
+        call()
+    eng.synchronize()
+    assert caches[0].length(0) == 6 and caches[1].length(0) == 3
+    torch.cuda.synchronize()
+    eng.close()

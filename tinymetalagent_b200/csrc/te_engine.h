@@ -102,6 +102,7 @@ inline te_status fail(te_attn_engine* e, te_status st, const std::string& msg) {
 }
 
 inline te_status cuda_fail(te_attn_engine* e, cudaError_t err, const char* what) {
+  (void)cudaGetLastError();  // reported here: the next launch must not report it again
   std::string m = std::string(what) + ": " + cudaGetErrorString(err);
   if (e) e->last_error = m;
   return err == cudaErrorMemoryAllocation ? TE_STATUS_OUT_OF_MEMORY : TE_STATUS_RUNTIME_ERROR;
