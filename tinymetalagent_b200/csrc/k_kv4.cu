@@ -342,11 +342,12 @@ __device__ __forceinline__ void store32(void* base, size_t idx, const float (&x)
 // out, through shared memory, so that a warp's accesses are whole rows while a lane's work is a block.
 //
 // Bound by bytes: 36 layers x 2048 tokens x 2 kv heads x 128 values, stored rows returned in the same type, take
-// 33.2 us as binary16 (172 MB, 5.2 TB/s, 0.79 of a plain copy's rate; a seventh is ramp and tail) and 52.4 us as fp32
+// 33 to 35 us as binary16 (172 MB, 5.0 TB/s, 0.76 of a copy's rate; a seventh is ramp and tail) and 52.4 us as fp32
 // (323 MB, 6.2 TB/s); at 64 dims 18.9 and 27.5 us.  Eight lanes a block with a division a value took 80 us for the
 // first, a block a lane with Markstein's step 39, each lane reading its own block one step ahead 34.7 (fp32: 85.0,
 // 64 dims 20.6 and 44.8), codes joined in the FMA pipe 34.2.  Four CTAs an SM: held to the registers of five or six,
-// the values spill (37 to 43 us).  A single token (24 layers) is a launch: 2 us on the device.
+// the values spill (37 to 43 us; at four, fp32 rows of 64 dims spill five words).  A single token (24 layers) is a
+// launch: 2 us on the device.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(32 * kRowWarps, 4) kv4_append_kernel(const Kv4RowsParams p) {
   constexpr int TB = kv4_tile_bytes(HD), CB = kv4_code_bytes(HD), SB = kv4_scale_bytes(HD), NB = HD / 32;
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) kv4_append_kernel(const Kv4
 // 4g.. of tokens 2t, 2t + 1), read 16 bytes at a time; a row's pieces leave as whole 32-byte sectors.
 //
 // Bound by the rows it writes: 28 layers x 16384 tokens x 4 kv heads x 128 values as binary16, 1.2 GB in all, take
-// 186 to 190 us (6.4 TB/s, a plain copy's rate); 29 MB of odd range as fp32 6.7 us.  Read a word at a time where it
+// 186 to 192 us (6.3 to 6.5 TB/s, a plain copy's rate); 29 MB of odd range as fp32 6.7 us.  Read a word at a time where it
 // was needed, the large case took 228 us.
 template <int HD>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_read_kernel(const Kv4RowsParams p) {
@@ -696,23 +697,24 @@ __global__ void __launch_bounds__(128) kv4_raw_kernel(const Kv4RowsParams p, int
 // zero the output was 6e-4 off, against less than 1e-5 now, at the same speed
 // (147 and 50 to 51 us for the first two lines below, both ways in turn).
 //
-// Split: a warp streams copies of 32 (head_dim 64: 64) tokens through a ring
-// of its own, so no barrier stands in the loop; the CTA's warps merge at the
-// end of a segment, and a group's CTAs through records that the last of them
+// Split: a warp streams copies of 64 tokens through a ring of its own, so no
+// barrier stands in the loop; the CTA's warps merge at the end of a segment, and a group's CTAs through records that the last of them
 // to arrive folds (plan_kv4_decode chooses who takes what).
 //
 // What bounds it is not the bytes but the conversion of the codes and the
-// products they feed: a tile of 16 tokens costs a warp about 370 instructions,
+// products they feed: a tile of 16 tokens costs a warp about 327 instructions,
 // 32 of them matrix products of 9 clocks, and an SM some 160 clocks with the
 // copies taken out, where HBM would deliver one in 99; with the arithmetic
 // taken out the same loop streams 5.9 TB/s.  Measured at head_dim 128, 7 or 8
 // heads a group:
-//   28 layers x 4 kv heads x 32768 tokens  529 MB  136 us, 3.9 TB/s (copy rate: 81 us)
-//   64 sequences, 8192 tokens at most      153 MB   52 us, 2.9 TB/s (23 us)
+//   28 layers x 4 kv heads x 32768 tokens  529 MB  135 to 148 us by GPU, 3.6 to 3.9 TB/s (copy rate: 81 us)
+//   64 sequences, 8192 tokens at most      153 MB   50 us, 3.0 TB/s (23 us)
 //   36 layers x 2 kv heads x 4097 tokens    43 MB   19 us, 2.3 TB/s (6.6 us)
 //   24 layers x 2 kv heads x 1000 tokens of 64, appending  12 us (0.6 us: latency)
+// Copies with scales outside 2^-14 .. 2 cost a tenth to a sixth more (all of
+// them outside: 156 us for the first line where the others take 135).
 // Shapes: at head_dim 128, four warps x 2 CTAs with 64 tokens a step and 255
-// registers take 136 us for the first line, one CTA of eight warps 142 (58 and
+// registers took 136 us for the first line, one CTA of eight warps 142 (58 and
 // 19.5 for the next two); when the shape was chosen it took 138, 16 warps with
 // 32 tokens 147 (12 warps 147 too), 20 and 24 warps with 16 tokens 171 and 180.
 // At head_dim 64 eight warps x 2 CTAs take 14.1 us for 24 layers x 8192 tokens,

@@ -22,7 +22,9 @@ One difference from the reference's CPU pass is by design: the KV cache is
 the engine's f16 cache (the reference's Metal path's layout), where the CPU
 pass keeps fp32 keys and values, so outputs agree to f16 rounding of K/V, not
 bit for bit.  With kv_bits=4 it is the 4-bit cache (te_kv4_*, GGUF Q4_0
-blocks): 3.56 times the context in the same memory.
+blocks), 3.56 times smaller; from the first prompt on the decoder also holds
+one layer of the context in f16, and a prompt over stored tokens reads one
+layer of them into a temporary of the same kind.
 """
 from __future__ import annotations
 
@@ -57,8 +59,10 @@ class QwenDecoder:
 
     kv_bits 16 keeps the keys and values in the f16 cache; kv_bits 4 in the
     4-bit cache, on the per-op path: a step's launch quantises the new token
-    and attends the cache as stored, a prompt attends its own rows in f16 and
-    the history as read back from the cache, and is then quantised into it.
+    and attends the cache as stored, a prompt attends its own rows and the
+    history as read back from the cache, both rounded to f16, and is then
+    quantised into it.  So a prompt given in parts attends its earlier parts
+    as stored, and its result differs from that of the prompt given at once.
     """
 
     def __init__(self, engine: AttnEngine, model: str | Path | GGUFFile, context_tokens: int,
